@@ -47,6 +47,7 @@ class hy_gguf_tensor_info(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_int64
 _DEV = ctypes.POINTER(hy_moe_dev)
 
 # name -> (restype, argtypes); every function declared in include/hymoe.h
@@ -100,6 +101,19 @@ SIGNATURES = {
     "hy_moe_decode_ws_bytes": (ctypes.c_size_t, [_DEV, _I, _I, _DEV, _I]),
     "hy_moe_decode": (_I, [_DEV, _P, _I, _P, _I, _P, _I, _I, _DEV, _P, _I, _I, _P, ctypes.c_size_t, _P]),
     "hy_moe_decode_noalloc": (_I, [_DEV, _P, _I, _P, _I, _P, _I, _I, _DEV, _P, _I, _I, _P]),
+    "hy_linear": (_I, [_I, _P, _L, _I, _I, _P, _L, _I, _P, _I, _P, _L, _P, _L, _P, _I, _L, _P]),
+    "hy_linear_glu": (_I, [_I, _P, _P, _L, _I, _I, _P, _L, _I, _F, _P, _P, _P, _L, _P]),
+    "hy_act_bwd": (_I, [_I, _I, _P, _L, _P, _L, _I, _I, _P, _L, _P]),
+    "hy_linear_dx": (_I, [_I, _P, _L, _I, _I, _P, _L, _I, _P, _L, _P, _I, _L, _P]),
+    "hy_linear_dw_ws_bytes": (ctypes.c_size_t, [_I, _I, _I]),
+    "hy_linear_dw": (_I, [_I, _P, _L, _P, _L, _I, _I, _I, _P, _I, _L, _P, _I, _P, ctypes.c_size_t, _P]),
+    "hy_moe16_gate_up": (_I, [_DEV, _P, _L, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P]),
+    "hy_moe16_down": (_I, [_DEV, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "hy_moe16_down_dx": (_I, [_DEV, _P, _L, _I, _I, _P, _P, _P, _I, _P, _I, _P]),
+    "hy_moe16_gate_up_dx": (_I, [_DEV, _P, _P, _I, _P, _P, _P, _I, _P, _I, _P]),
+    "hy_moe16_dw": (_I, [_DEV, _I, _P, _L, _I, _I, _P, _L, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P]),
+    "hy_swiglu_bwd": (_I, [_I, _P, _P, _P, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "hy_rows16": (_I, [_I, _P, _L, _I, _I, _P, _L, _P]),
     "hy_dequant_row": (_I, [_I, _P, _I, _P, _P]),
     "hy_block_ints": (_I, [_I, _P, ctypes.c_size_t, _I, _P, _I, _P, _P, _P]),
 }

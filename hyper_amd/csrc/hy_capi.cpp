@@ -106,8 +106,15 @@ size_t hy_q8_row_bytes(int vtype, int n) {
 
 int hy_upload_experts(const hy_expert_tensors *t, const int32_t *slot_host, int32_t ff, int32_t n, float clamp, hy_moe_dev *out) {
     if (!t || !slot_host || !out || !t->gate || !t->up || !t->down || t->E <= 0) { set_error("hy_upload_experts: null argument"); return HY_EINVAL; }
-    if (!dot_type(t->tg) || !dot_type(t->td)) { set_error("hy_upload_experts: unsupported expert type"); return HY_EUNSUPPORTED_TYPE; }
-    if (ff <= 0 || n <= 0 || ff % 256 || n % 256 || t->gb != (size_t) ff * (n / 256) * span_bytes(t->tg) ||
+    // F16 and BF16 matrices keep GGUF's rows (the 16-bit products read them as they are)
+    const bool plain = (t->tg == HY_F16 || t->tg == HY_BF16) && (t->td == HY_F16 || t->td == HY_BF16);
+    if (!plain && (!dot_type(t->tg) || !dot_type(t->td))) { set_error("hy_upload_experts: unsupported expert type"); return HY_EUNSUPPORTED_TYPE; }
+    if (plain) {
+        if (ff <= 0 || n <= 0 || t->gb != 2 * (size_t) ff * (size_t) n || t->db != t->gb) {
+            set_error("hy_upload_experts: gb/db must be the matrices' GGUF sizes (2 ff n bytes)");
+            return HY_EBAD_SHAPE;
+        }
+    } else if (ff <= 0 || n <= 0 || ff % 256 || n % 256 || t->gb != (size_t) ff * (n / 256) * span_bytes(t->tg) ||
         t->db != (size_t) n * (ff / 256) * span_bytes(t->td)) {
         set_error("hy_upload_experts: ff and n must be multiples of 256 and gb/db the matrices' GGUF sizes");
         return HY_EBAD_SHAPE;
@@ -132,8 +139,9 @@ int hy_upload_experts(const hy_expert_tensors *t, const int32_t *slot_host, int3
     if (err == hipSuccess) err = hipMalloc(&dd, t->db * n_alloc);
     if (err == hipSuccess) err = hipMalloc(&ds, sizeof(int32_t) * t->E);
     // GGUF rows -> 16-row tiles (tiled_off), one expert matrix at a time through a host staging buffer
-    std::vector<uint8_t> stage(std::max(t->gb, t->db));
+    std::vector<uint8_t> stage(plain ? 0 : std::max(t->gb, t->db));
     auto put = [&](uint8_t *dst, const uint8_t *src, int rows, int in_dim, int type) {
+        if (plain) return hipMemcpy(dst, src, 2 * (size_t) rows * in_dim, hipMemcpyHostToDevice);
         const int nspan = in_dim / 256, sb = span_bytes(type);
         for (int r = 0; r < rows; ++r)
             for (int sp = 0; sp < nspan; ++sp)

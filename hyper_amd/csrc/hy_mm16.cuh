@@ -1,0 +1,227 @@
+// 16-bit (bf16 / fp16) matrix products with fp32 sums: what the kernels share.
+//
+// One description covers the linear layer, the products grouped by expert and their gradients.  An output tile has rows
+// (operand Q: token or pair rows) and columns (operand P: a weight's rows or columns); KIND says where the contraction lies:
+//   NT  out[r][c] = sum_k Q[r][k] P[c][k]      forward: Q = x or h, P = W                (both contiguous along k)
+//   NN  out[r][c] = sum_k Q[r][k] P[k][c]      gradient of the rows: Q = dz, P = W
+//   TN  out[r][c] = sum_k Q[k][r] P[k][c]      gradient of the weights: Q = dz, P = x, k over the (gathered) rows
+// P is the matrix instruction's A operand and Q its B operand: lane l of a 16 x 16 product then holds columns
+// 4 (l / 16) .. + 3 of row l % 16, four neighbours of one output row, which it stores together.
+#pragma once
+#include "hy_internal.h"
+
+namespace hy {
+
+enum { NT = 0, NN = 1, TN = 2 };
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef float f4 __attribute__((ext_vector_type(4)));
+template <typename T> using v8 = T __attribute__((ext_vector_type(8)));
+template <typename T> using v4 = T __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4 mfma16(v8<bf16> a, v8<bf16> b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mfma16(v8<f16> a, v8<f16> b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+struct MMArgs {
+    // operands; P2 / Q2: the second pair of a two-part contraction (NN: up after gate) or the up matrix of a gated product (NT)
+    const void *P, *P2, *Q, *Q2;
+    int64_t ldp, ldq;        // elements between rows
+    int64_t pstride;         // elements between the experts' matrices
+    int R, N, K;             // output rows (ungrouped; TN: rows of each gradient), columns, contraction length of one part (TN: ungrouped rows)
+    // grouping: pairs order[start ..] of the egrp triples; operand row of pair p is p / kq (TN: also p / kp), output row p
+    const int *order, *order_n, *egrp, *slot, *ids;
+    int n_local, n_expert, n_pairs, max_active;
+    uint32_t kq, kp;
+    // epilogue: v = acc + bias; z = v; v = act(v) * wts[p] + resid (+ out).  Gated: h = SwiGLU(g, u), g and u on request
+    const float *bias, *wts;
+    const void *resid;
+    void *z, *g, *u, *out;
+    int64_t ldr, ldz, ldo, ostride;   // ostride (TN): elements between the experts' gradients
+    float *db;                        // TN: sums of Q's columns
+    int act, out_f32, accumulate;
+    float clamp;
+    int vec;                          // four neighbouring outputs can be moved at once (alignment of out, resid, z, g, u)
+};
+
+__device__ __forceinline__ float mm_act(int act, float z) {
+    switch (act) {
+    case HY_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;   // NaN stays NaN
+    case HY_ACT_SILU: return hy_silu(z);
+    case HY_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);
+    case HY_ACT_GELU_TANH: return z * hy_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
+    }
+    return z;
+}
+// act'(z)
+__device__ __forceinline__ float mm_act_grad(int act, float z) {
+    switch (act) {
+    case HY_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+    case HY_ACT_SILU: { const float s = hy_sigmoid(z); return s * fmaf(z, 1.0f - s, 1.0f); }
+    case HY_ACT_GELU:   // Phi(z) + z phi(z)
+        return fmaf(z * 0.39894228040143268f, hy_expf(-0.5f * z * z), 0.5f * erfcf(z * -0.70710678118654752f));
+    case HY_ACT_GELU_TANH: {   // z sigmoid(2 a): s + z s (1 - s) 2 a'
+        const float s = hy_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
+        return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);
+    }
+    }
+    return 1.0f;
+}
+
+// p / k for 0 <= p < 2^31 and 1 <= k <= 64: M = ceil(2^40 / k) is at most 1 / k + 2^-40 too large, p times that error < 2^-9 < 1 / k
+__device__ __forceinline__ int div_k(int p, uint32_t k, uint64_t M) { return k == 1 ? p : (int) (((uint64_t) (uint32_t) p * M) >> 40); }
+__host__ __device__ __forceinline__ uint64_t div_magic(uint32_t k) { return ((1ull << 40) + k - 1) / k; }
+
+template <typename T> __device__ __forceinline__ v4<T> to4(f4 v) { return {(T) v[0], (T) v[1], (T) v[2], (T) v[3]}; }
+
+// one value / four neighbours of a T or fp32 matrix
+template <typename T> __device__ __forceinline__ void put4(void *base, int64_t at, f4 v, int n, bool f32, bool vec) {
+    if (f32) {
+        float *o = (float *) base + at;
+        if (vec && n == 4) *(f4 *) o = v;
+        else
+            for (int i = 0; i < 4; ++i) if (i < n) o[i] = v[i];
+    } else {
+        T *o = (T *) base + at;
+        if (vec && n == 4) *(v4<T> *) o = to4<T>(v);
+        else
+            for (int i = 0; i < 4; ++i) if (i < n) o[i] = (T) v[i];
+    }
+}
+template <typename T> __device__ __forceinline__ f4 get4(const void *base, int64_t at, int n, bool f32, bool vec) {
+    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (f32) {
+        const float *o = (const float *) base + at;
+        if (vec && n == 4) return *(const f4 *) o;
+        for (int i = 0; i < 4; ++i) if (i < n) v[i] = o[i];
+    } else {
+        const T *o = (const T *) base + at;
+        if (vec && n == 4) { const v4<T> t = *(const v4<T> *) o; return {(float) t[0], (float) t[1], (float) t[2], (float) t[3]}; }
+        for (int i = 0; i < 4; ++i) if (i < n) v[i] = (float) o[i];
+    }
+    return v;
+}
+// outputs c .. c + 3 of output row `row` from their sums; ob: element offset of the expert's gradient (TN), w: the pair's weight
+template <typename T> __device__ __forceinline__ void epi_store(const MMArgs &a, int64_t ob, int64_t row, int c, f4 v, float w) {
+    const int n = min(4, a.N - c);
+    if (n <= 0) return;
+    const bool vec = a.vec;
+    if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < n) v[i] += a.bias[c + i];
+    }
+    if (a.z) put4<T>(a.z, row * a.ldz + c, v, n, false, vec);
+    if (a.act) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = mm_act(a.act, v[i]);
+    }
+    if (a.wts) v *= w;
+    if (a.resid) v += get4<T>(a.resid, row * a.ldr + c, n, a.out_f32, vec);
+    const int64_t at = ob + row * a.ldo + c;
+    if (a.accumulate) v += get4<T>(a.out, at, n, a.out_f32, vec);
+    put4<T>(a.out, at, v, n, a.out_f32, vec);
+}
+// gated: h (and g, u) of columns c .. c + 3
+template <typename T> __device__ __forceinline__ void epi_glu(const MMArgs &a, int64_t row, int c, f4 g, f4 u) {
+    const int n = min(4, a.N - c);
+    if (n <= 0) return;
+    const int64_t at = row * a.ldo + c;
+    if (a.g) { put4<T>(a.g, at, g, n, false, a.vec); put4<T>(a.u, at, u, n, false, a.vec); }
+    f4 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = hy_swiglu(g[i], u[i], a.clamp);
+    put4<T>(a.out, at, h, n, false, a.vec);
+}
+
+// ------------------------------------------------------------------ groups
+
+// A block's group: pairs order[start .. start + cnt) (or rows start .. of an ungrouped product) with local expert le
+struct Group { int le, start, cnt; };
+
+// triple i of egrp, with every field bounded: a group outside the pairs or without a local expert has no rows
+__device__ __forceinline__ Group load_group(const MMArgs &a, int i) {
+    const int e = a.egrp[3 * i], start = a.egrp[3 * i + 1], cnt = a.egrp[3 * i + 2];
+    Group g{-1, 0, 0};
+    if ((uint32_t) e < (uint32_t) a.n_expert && start >= 0 && cnt > 0 && cnt <= a.n_pairs - start) {
+        const int s = a.slot[e];
+        if ((uint32_t) s < (uint32_t) a.n_local) g = Group{s, start, cnt};
+    }
+    return g;
+}
+__device__ __forceinline__ int n_groups(const MMArgs &a) { return max(0, min(a.order_n[1], a.max_active)); }
+
+// The group and row tile of work item `it` (tiles of BM rows, groups in order), found by the whole block of NTH threads:
+// every thread counts the tiles of its few groups, a scan over the block places them.  false: past the last item.
+// total: the number of items.
+template <int NTH, int BM> __device__ __forceinline__ bool find_item(const MMArgs &a, int it, Group &g, int &tile, int &total) {
+    if (!a.egrp) {
+        g = Group{0, 0, a.R};
+        tile = it;
+        total = (a.R + BM - 1) / BM;
+        return it < total;
+    }
+    constexpr int PER = 1024 / NTH;
+    static_assert(PER * NTH == 1024, "at most 1024 groups");
+    __shared__ int s_w[NTH / 64], s_out[5];
+    const int tid = threadIdx.x, lane = tid & 63, ng = n_groups(a);
+    Group gs[PER];
+    int nt[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = tid * PER + j;
+        gs[j] = Group{-1, 0, 0};
+        if (i < ng) gs[j] = load_group(a, i);
+        nt[j] = (int) (((uint32_t) gs[j].cnt + BM - 1) / BM);
+        sum += nt[j];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(inc, o); if (lane >= o) inc += v; }
+    if (lane == 63) s_w[tid >> 6] = inc;
+    __syncthreads();
+    int pre = inc - sum, all = 0;
+#pragma unroll
+    for (int w = 0; w < NTH / 64; ++w) { if (w < (tid >> 6)) pre += s_w[w]; all += s_w[w]; }
+    total = all;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (it >= pre && it < pre + nt[j]) { s_out[0] = gs[j].le; s_out[1] = gs[j].start; s_out[2] = gs[j].cnt; s_out[3] = it - pre; }
+        pre += nt[j];
+    }
+    __syncthreads();
+    if (it >= all) return false;
+    g = Group{s_out[0], s_out[1], s_out[2]};
+    tile = s_out[3];
+    return true;
+}
+// The pairs of local expert `le` (TN), found by the whole block; cnt 0 when it has none
+template <int NTH> __device__ __forceinline__ Group find_expert(const MMArgs &a, int le) {
+    if (!a.egrp) return Group{0, 0, a.K};
+    __shared__ int s_g[2];
+    if (threadIdx.x == 0) { s_g[0] = 0; s_g[1] = 0; }
+    __syncthreads();
+    const int ng = n_groups(a);
+    for (int i = threadIdx.x; i < ng; i += NTH) {
+        const Group g = load_group(a, i);
+        if (g.cnt && g.le == le) { s_g[0] = g.start; s_g[1] = g.cnt; }
+    }
+    __syncthreads();
+    return Group{le, s_g[0], s_g[1]};
+}
+// pair (or plain row) number i of a group; -1 for an entry outside the pairs
+__device__ __forceinline__ int pair_of(const MMArgs &a, const Group &g, int i) {
+    if (!a.order) return g.start + i;
+    const int p = a.order[g.start + i];
+    return (uint32_t) p < (uint32_t) a.n_pairs ? p : -1;
+}
+
+// launchers (type: HY_F16 / HY_BF16)
+int launch_mm(int kind, int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
+int launch_mv(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
+int launch_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
+                   hipStream_t s);
+int launch_swiglu_bwd(int type, const void *g, const void *u, const void *dh, const float *wts, int n_pairs, int ff, float clamp,
+                      const int *order, const int *order_n, void *dg, void *du, void *hw, float *dwts, hipStream_t s);
+int launch_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, int64_t ldo, hipStream_t s);
+
+} // namespace hy

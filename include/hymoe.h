@@ -295,6 +295,77 @@ int hy_dequant_row(int type, const uint8_t *row, int n, float *out, hipStream_t 
 int hy_block_ints(int type, const uint8_t *rows, size_t row_bytes, int nrows, const void *xq, int n, int32_t *sumi, int32_t *summ,
                   hipStream_t s);
 
+/* ---- 16-bit matrix products: experts, shared experts and dense layers whose matrices GGUF holds as F16 or BF16, forward
+   and backward.  No counterpart in the reference, which converts such tensors to its fp16 fragments (src/dense.cu).
+   `type` is HY_F16 or HY_BF16, the type of every 16-bit operand of a call; products are summed in fp32 and rounded once, to
+   the nearest even value of the output's type (out_type: `type` or HY_F32).  Matrices are row-major; ld* is the number of
+   elements between the rows (an input may repeat rows with 0).  Any size and any alignment to the values' own size is
+   taken; rows of multiples of 8 values that start on 16 bytes are fastest.  Results do not depend on anything but the
+   arguments (no atomics).  Sizes up to HY_MM_MAX. */
+#define HY_F32 0
+#define HY_F16 1
+#define HY_BF16 30
+#define HY_MM_MAX (1 << 30)
+#define HY_ACT_NONE 0
+#define HY_ACT_RELU 1
+#define HY_ACT_SILU 2
+#define HY_ACT_GELU 3        /* z Phi(z) */
+#define HY_ACT_GELU_TANH 4   /* its tanh form: z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+
+/* out[i] = act(x[i] W^T + bias) + resid[i] for m rows x [m][k], W [n][k].  bias: n floats (NULL: none); resid (NULL:
+   none): of out's type, may be out itself; z (NULL: none): the values before act, of `type`, for hy_act_bwd. */
+int hy_linear(int type, const void *W, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, const float *bias, int act,
+              const void *resid, int64_t ldr, void *z, int64_t ldz, void *out, int out_type, int64_t ldo, hipStream_t s);
+/* Gated: g = x Wg^T, u = x Wu^T, h = silu(min(g, clamp)) * max(-clamp, min(u, clamp)) (clamp 0: no limits), a shared
+   expert's gate/up.  g and u (both or neither, row distance ldh) keep the products for hy_swiglu_bwd. */
+int hy_linear_glu(int type, const void *Wg, const void *Wu, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, float clamp,
+                  void *g, void *u, void *h, int64_t ldh, hipStream_t s);
+/* dz = dy act'(z), [m][n].  dz may be dy or z. */
+int hy_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
+               hipStream_t s);
+/* dx = dz W + resid for dz [m][n], W [n][k], dx [m][k] (resid as hy_linear's) */
+int hy_linear_dx(int type, const void *W, int64_t ldw, int n, int k, const void *dz, int64_t lddz, int m, const void *resid, int64_t ldr,
+                 void *dx, int out_type, int64_t lddx, hipStream_t s);
+/* dW = dz^T x [n][k] and db[r] = sum of dz[i][r] (NULL: none), added to what is there with accumulate != 0.  m = 0 gives
+   zeros.  ws: at least hy_linear_dw_ws_bytes(m, n, k) bytes (which may be 0), 16-byte aligned, for calls on one stream;
+   nothing in it is kept between calls. */
+size_t hy_linear_dw_ws_bytes(int m, int n, int k);
+int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t ldx, int m, int n, int k, void *dW, int out_type,
+                 int64_t lddw, float *db, int accumulate, void *ws, size_t ws_bytes, hipStream_t s);
+
+/* Experts in 16 bits.  The descriptor is hy_moe_dev with tg / td HY_F16 or HY_BF16 and plain row-major matrices: gate, up
+   [n_local][ff][n] and down [n_local][n][ff], gate_bytes = down_bytes = 2 ff n, ff and n of any size (hy_upload_experts
+   copies them from GGUF rows as they are).  hy_moe_order takes the same descriptor.  Pairs p = t k + j: either grouped by
+   order, order_n, egrp of hy_moe_order (max_active >= order_n[1], at most 1024), or, with order NULL, each by its expert
+   ids[p] (single tokens: every pair reads its expert's matrices; up to 65535 pairs).  Rows of pairs whose expert is not
+   local are left as they were.
+   gate_up: h[p] = SwiGLU(gate_e x[p / k], up_e x[p / k]) with the descriptor's clamp, g and u on request as in
+   hy_linear_glu; h, g, u [n_pairs][ff].  down: y[p] = wts[p] (down_e h[p]) (wts NULL: 1), [n_pairs][n]; with out_type
+   HY_F32 hy_moe_reduce combines the rows. */
+int hy_moe16_gate_up(const hy_moe_dev *m, const void *x, int64_t ldx, int k, const int32_t *ids, int n_pairs, const int32_t *order,
+                     const int32_t *order_n, const int32_t *egrp, int max_active, void *g, void *u, void *h, hipStream_t s);
+int hy_moe16_down(const hy_moe_dev *m, const void *h, const int32_t *ids, int n_pairs, const int32_t *order, const int32_t *order_n,
+                  const int32_t *egrp, int max_active, const float *wts, void *y, int out_type, hipStream_t s);
+/* The backward pass of a layer y[t] = sum_j wts[p] down_e h[p], from dy [tokens][n]:
+     hy_moe16_down_dx     dh[p] = dy[p / k] down_e (not yet weighted), [n_pairs][ff]
+     hy_swiglu_bwd        from g, u, dh: dwts[p] = sum dh h,  hw = wts h,  dg, du of wts dh       (wts NULL: 1)
+     hy_moe16_gate_up_dx  dx[p] = dg[p] gate_e + du[p] up_e, [n_pairs][n]; hy_moe_reduce sums a token's pairs
+     hy_moe16_dw          dW[slot[e]] = sum over e's pairs of a[p / ka]^T b[p / kb], [n_local][rows][cols] (zeros for an
+                          expert without pairs): gate from (dg, x), up from (du, x), down from (dy, hw)
+   hy_swiglu_bwd takes all n_pairs rows, or with order and order_n the pairs listed there; hw and dwts may be NULL; dg, du
+   and hw may each be one of g, u, dh.  Where g (u) lies beyond the clamp its gradient is 0. */
+int hy_moe16_down_dx(const hy_moe_dev *m, const void *dy, int64_t lddy, int k, int n_pairs, const int32_t *order, const int32_t *order_n,
+                     const int32_t *egrp, int max_active, void *dh, int out_type, hipStream_t s);
+int hy_moe16_gate_up_dx(const hy_moe_dev *m, const void *dg, const void *du, int n_pairs, const int32_t *order, const int32_t *order_n,
+                        const int32_t *egrp, int max_active, void *dx, int out_type, hipStream_t s);
+int hy_moe16_dw(const hy_moe_dev *m, int type, const void *a, int64_t lda, int ka, int rows, const void *b, int64_t ldb, int kb, int cols,
+                int n_pairs, const int32_t *order, const int32_t *order_n, const int32_t *egrp, int max_active, void *dW, int out_type,
+                int accumulate, hipStream_t s);
+int hy_swiglu_bwd(int type, const void *g, const void *u, const void *dh, const float *wts, int n_pairs, int ff, float clamp,
+                  const int32_t *order, const int32_t *order_n, void *dg, void *du, void *hw, float *dwts, hipStream_t s);
+/* fp32 rows x[t * xs ..][0..n) rounded to `type` (the router's rows for the calls above) */
+int hy_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, int64_t ldo, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -230,4 +230,55 @@ inline void deq_row_test(int type, const uint8_t *row, int n, float *out, hipStr
     check(hy_dequant_row(type, row, n, out, s));
 }
 
+// ---- 16-bit matrix products (hymoe.h: hy_linear and the experts' hy_moe16_* calls), std::runtime_error on failure
+inline void linear(int type, const void *W, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, const float *bias, int act,
+                   const void *resid, int64_t ldr, void *z, int64_t ldz, void *out, int out_type, int64_t ldo, hipStream_t s) {
+    check(hy_linear(type, W, ldw, n, k, x, ldx, m, bias, act, resid, ldr, z, ldz, out, out_type, ldo, s));
+}
+inline void linear_glu(int type, const void *Wg, const void *Wu, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, float clamp,
+                       void *g, void *u, void *h, int64_t ldh, hipStream_t s) {
+    check(hy_linear_glu(type, Wg, Wu, ldw, n, k, x, ldx, m, clamp, g, u, h, ldh, s));
+}
+inline void act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
+                    hipStream_t s) {
+    check(hy_act_bwd(type, act, z, ldz, dy, lddy, m, n, dz, lddz, s));
+}
+inline void linear_dx(int type, const void *W, int64_t ldw, int n, int k, const void *dz, int64_t lddz, int m, const void *resid, int64_t ldr,
+                      void *dx, int out_type, int64_t lddx, hipStream_t s) {
+    check(hy_linear_dx(type, W, ldw, n, k, dz, lddz, m, resid, ldr, dx, out_type, lddx, s));
+}
+inline size_t linear_dw_ws_bytes(int m, int n, int k) { return hy_linear_dw_ws_bytes(m, n, k); }
+inline void linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t ldx, int m, int n, int k, void *dW, int out_type,
+                      int64_t lddw, float *db, bool accumulate, void *ws, size_t ws_bytes, hipStream_t s) {
+    check(hy_linear_dw(type, dz, lddz, x, ldx, m, n, k, dW, out_type, lddw, db, accumulate, ws, ws_bytes, s));
+}
+inline void moe16_gate_up(const MoeDev &m, const void *x, int64_t ldx, int k, const int *ids, int n_pairs, const int *order, const int *order_n,
+                          const int *egrp, int max_active, void *g, void *u, void *h, hipStream_t s) {
+    check(hy_moe16_gate_up(&m, x, ldx, k, ids, n_pairs, order, order_n, egrp, max_active, g, u, h, s));
+}
+inline void moe16_down(const MoeDev &m, const void *h, const int *ids, int n_pairs, const int *order, const int *order_n, const int *egrp,
+                       int max_active, const float *wts, void *y, int out_type, hipStream_t s) {
+    check(hy_moe16_down(&m, h, ids, n_pairs, order, order_n, egrp, max_active, wts, y, out_type, s));
+}
+inline void moe16_down_dx(const MoeDev &m, const void *dy, int64_t lddy, int k, int n_pairs, const int *order, const int *order_n,
+                          const int *egrp, int max_active, void *dh, int out_type, hipStream_t s) {
+    check(hy_moe16_down_dx(&m, dy, lddy, k, n_pairs, order, order_n, egrp, max_active, dh, out_type, s));
+}
+inline void moe16_gate_up_dx(const MoeDev &m, const void *dg, const void *du, int n_pairs, const int *order, const int *order_n,
+                             const int *egrp, int max_active, void *dx, int out_type, hipStream_t s) {
+    check(hy_moe16_gate_up_dx(&m, dg, du, n_pairs, order, order_n, egrp, max_active, dx, out_type, s));
+}
+inline void moe16_dw(const MoeDev &m, int type, const void *a, int64_t lda, int ka, int rows, const void *b, int64_t ldb, int kb, int cols,
+                     int n_pairs, const int *order, const int *order_n, const int *egrp, int max_active, void *dW, int out_type,
+                     bool accumulate, hipStream_t s) {
+    check(hy_moe16_dw(&m, type, a, lda, ka, rows, b, ldb, kb, cols, n_pairs, order, order_n, egrp, max_active, dW, out_type, accumulate, s));
+}
+inline void swiglu_bwd(int type, const void *g, const void *u, const void *dh, const float *wts, int n_pairs, int ff, float clamp,
+                       const int *order, const int *order_n, void *dg, void *du, void *hw, float *dwts, hipStream_t s) {
+    check(hy_swiglu_bwd(type, g, u, dh, wts, n_pairs, ff, clamp, order, order_n, dg, du, hw, dwts, s));
+}
+inline void rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, int64_t ldo, hipStream_t s) {
+    check(hy_rows16(type, x, xs, n, nt, out, ldo, s));
+}
+
 } // namespace hymoe
