@@ -24,7 +24,7 @@ OUT = PKG / "libhymoe.so"
 OUT_STAMPS = PKG / "libhymoe_stamps.so"
 BUILD = PKG / "_build"
 
-SOURCES = ["hy_route.hip", "hy_gemv.hip", "hy_gemm.hip", "hy_decode.hip", "hy_mm16.hip", "hy_mv16.hip", "hy_capi.cpp", "hy_mm16_api.cpp", "hy_step.cpp", "hy_gguf.cpp"]
+SOURCES = ["hy_route.hip", "hy_gemv.hip", "hy_gemm.hip", "hy_decode.hip", "hy_mm16.hip", "hy_mm16_nt.hip", "hy_mm16_nn.hip", "hy_mm16_tn.hip", "hy_mv16.hip", "hy_capi.cpp", "hy_mm16_api.cpp", "hy_step.cpp", "hy_gguf.cpp"]
 ARCH = os.environ.get("HYMOE_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -51,7 +51,7 @@ def _compile(src: str, stamps: bool = False) -> Path:
 def build(verbose: bool = False, stamps: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     out = OUT_STAMPS if stamps else OUT
-    with ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
         objs = list(ex.map(lambda src: _compile(src, stamps), SOURCES))
     tmp = out.with_suffix(".so.tmp")
     r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)],

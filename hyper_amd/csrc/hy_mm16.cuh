@@ -10,6 +10,8 @@
 #pragma once
 #include "hy_internal.h"
 
+#include <algorithm>
+
 namespace hy {
 
 enum { NT = 0, NN = 1, TN = 2 };
@@ -150,19 +152,18 @@ __device__ __forceinline__ Group load_group(const MMArgs &a, int i) {
 }
 __device__ __forceinline__ int n_groups(const MMArgs &a) { return max(0, min(a.order_n[1], a.max_active)); }
 
-// The group and row tile of work item `it` (tiles of BM rows, groups in order), found by the whole block of NTH threads:
-// every thread counts the tiles of its few groups, a scan over the block places them.  false: past the last item.
-// total: the number of items.
-template <int NTH, int BM> __device__ __forceinline__ bool find_item(const MMArgs &a, int it, Group &g, int &tile, int &total) {
+// The group and row tile of this block (tiles of BM rows, groups in order), found by the whole block of NTH threads: every
+// thread counts the tiles of its few groups, a scan over the block places them.  place(items) says which of the `items`
+// tiles is this block's (below 0: none); the result is false then.
+template <int NTH, int BM, typename F> __device__ __forceinline__ bool find_item(const MMArgs &a, F place, Group &g, int &tile) {
     if (!a.egrp) {
         g = Group{0, 0, a.R};
-        tile = it;
-        total = (a.R + BM - 1) / BM;
-        return it < total;
+        tile = place((int) (((uint32_t) a.R + BM - 1) / BM));
+        return tile >= 0;
     }
     constexpr int PER = 1024 / NTH;
     static_assert(PER * NTH == 1024, "at most 1024 groups");
-    __shared__ int s_w[NTH / 64], s_out[5];
+    __shared__ int s_w[NTH / 64], s_out[4];
     const int tid = threadIdx.x, lane = tid & 63, ng = n_groups(a);
     Group gs[PER];
     int nt[PER], sum = 0;
@@ -182,16 +183,16 @@ template <int NTH, int BM> __device__ __forceinline__ bool find_item(const MMArg
     int pre = inc - sum, all = 0;
 #pragma unroll
     for (int w = 0; w < NTH / 64; ++w) { if (w < (tid >> 6)) pre += s_w[w]; all += s_w[w]; }
-    total = all;
+    const int it = place(all);
+    if (it < 0) return false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         if (it >= pre && it < pre + nt[j]) { s_out[0] = gs[j].le; s_out[1] = gs[j].start; s_out[2] = gs[j].cnt; s_out[3] = it - pre; }
         pre += nt[j];
     }
     __syncthreads();
-    if (it >= all) return false;
-    g = Group{s_out[0], s_out[1], s_out[2]};
-    tile = s_out[3];
+    g = Group{__builtin_amdgcn_readfirstlane(s_out[0]), __builtin_amdgcn_readfirstlane(s_out[1]), __builtin_amdgcn_readfirstlane(s_out[2])};
+    tile = __builtin_amdgcn_readfirstlane(s_out[3]);
     return true;
 }
 // The pairs of local expert `le` (TN), found by the whole block; cnt 0 when it has none
@@ -215,8 +216,23 @@ __device__ __forceinline__ int pair_of(const MMArgs &a, const Group &g, int i) {
     return (uint32_t) p < (uint32_t) a.n_pairs ? p : -1;
 }
 
+// Tile number t of an items x ncol grid from the block number: blocks b, b + 8, .. run on one XCD, whose L2 they share, so
+// XCD x gets the tiles from x / 8 of the way on; there, bands of G row tiles go column by column, so that the blocks that
+// run together read few row and few column tiles.  Returns the row tile (-1: no tile) and sets col.
+template <int G> __device__ __forceinline__ int place_tile(uint32_t b, int items, int ncol, int &col) {
+    const uint32_t T = (uint32_t) items * (uint32_t) ncol;
+    if (b >= T) return -1;
+    const uint32_t q = T >> 3, r = T & 7, x = b & 7, t = x * q + min(x, r) + (b >> 3);
+    const uint32_t per = (uint32_t) G * ncol, band = t / per, in = t - band * per, rows = min((uint32_t) G, (uint32_t) items - band * G);
+    col = (int) (in / rows);
+    return (int) (band * G + in % rows);
+}
+
 // launchers (type: HY_F16 / HY_BF16)
 int launch_mm(int kind, int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
+int launch_tiles_nt(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
+int launch_tiles_nn(int type, const MMArgs &a, hipStream_t s, const char *what);
+int launch_tiles_tn(int type, const MMArgs &a, hipStream_t s, const char *what);
 int launch_mv(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
 int launch_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
                    hipStream_t s);

@@ -16,14 +16,15 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
     constexpr int BN = DUAL ? 32 : 64;
     const int ncol = (a.N + BN - 1) / BN;
     Group g;
-    int tile, total;
+    int tile, col;
     if constexpr (KIND == TN) {
         g = find_expert<256>(a, blockIdx.y);
         tile = blockIdx.x / ncol;
+        col = blockIdx.x % ncol;
     } else {
-        if (!find_item<256, 64>(a, blockIdx.x / ncol, g, tile, total)) return;
+        if (!find_item<256, 64>(a, [&](int items) { return place_tile<4>(blockIdx.x, items, ncol, col); }, g, tile)) return;
     }
-    const int c0 = (int) (blockIdx.x % ncol) * BN, r0 = tile * 64;
+    const int c0 = col * BN, r0 = tile * 64;
     const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);
     if constexpr (KIND != TN) {
         if (tid < 64) {
@@ -153,7 +154,17 @@ template <typename T> static int launch_any(int kind, bool dual, const MMArgs &a
     return check_launch(what);
 }
 
+// 16-byte rows: what the tile kernels read in 16-byte pieces starts and repeats on 16 bytes, and no piece passes the end of
+// its row
+static bool rows16b(const void *p, int64_t ld, int64_t stride, int len) { return ((uintptr_t) p & 15) == 0 && ld % 8 == 0 && stride % 8 == 0 && len % 8 == 0; }
+
 int launch_mm(int kind, int type, bool dual, const MMArgs &a, hipStream_t s, const char *what) {
+    const int plen = kind == NT ? a.K : a.N, qlen = kind == TN ? a.R : a.K;
+    if (rows16b(a.P, a.ldp, a.pstride, plen) && rows16b(a.P2, a.ldp, a.pstride, plen) && rows16b(a.Q, a.ldq, 0, qlen) && rows16b(a.Q2, a.ldq, 0, qlen)) {
+        if (kind == NT) return launch_tiles_nt(type, dual, a, s, what);
+        if (kind == NN) return launch_tiles_nn(type, a, s, what);
+        return launch_tiles_tn(type, a, s, what);
+    }
     return type == HY_BF16 ? launch_any<bf16>(kind, dual, a, s, what) : launch_any<f16>(kind, dual, a, s, what);
 }
 
