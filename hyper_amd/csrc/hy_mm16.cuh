@@ -43,7 +43,7 @@ struct MMArgs {
     float *db;                        // TN: sums of Q's columns
     int act, out_f32, accumulate;
     float clamp;
-    int vec;                          // four neighbouring outputs can be moved at once (alignment of out, resid, z, g, u)
+    int vec;                          // out, resid, z, g and u can be moved in 16-byte pieces
 };
 
 __device__ __forceinline__ float mm_act(int act, float z) {
@@ -74,65 +74,96 @@ __device__ __forceinline__ float mm_act_grad(int act, float z) {
 __device__ __forceinline__ int div_k(int p, uint32_t k, uint64_t M) { return k == 1 ? p : (int) (((uint64_t) (uint32_t) p * M) >> 40); }
 __host__ __device__ __forceinline__ uint64_t div_magic(uint32_t k) { return ((1ull << 40) + k - 1) / k; }
 
-template <typename T> __device__ __forceinline__ v4<T> to4(f4 v) { return {(T) v[0], (T) v[1], (T) v[2], (T) v[3]}; }
-
-// one value / four neighbours of a T or fp32 matrix
-template <typename T> __device__ __forceinline__ void put4(void *base, int64_t at, f4 v, int n, bool f32, bool vec) {
+// W neighbours (4 or 8) of a T or fp32 matrix, the first n of them; vec: they can be moved in 16-byte pieces
+template <typename T, int W> __device__ __forceinline__ void put_n(void *base, int64_t at, const float *v, int n, bool f32, bool vec) {
     if (f32) {
         float *o = (float *) base + at;
-        if (vec && n == 4) *(f4 *) o = v;
-        else
-            for (int i = 0; i < 4; ++i) if (i < n) o[i] = v[i];
+        if (vec && n == W) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) *(f4 *) (o + i) = f4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) if (i < n) o[i] = v[i];
+        }
     } else {
+        typedef T vt __attribute__((ext_vector_type(W)));
         T *o = (T *) base + at;
-        if (vec && n == 4) *(v4<T> *) o = to4<T>(v);
-        else
-            for (int i = 0; i < 4; ++i) if (i < n) o[i] = (T) v[i];
+        vt t;
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = (T) v[i];
+        if (vec && n == W) *(vt *) o = t;
+        else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) if (i < n) o[i] = t[i];
+        }
     }
 }
-template <typename T> __device__ __forceinline__ f4 get4(const void *base, int64_t at, int n, bool f32, bool vec) {
-    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+template <typename T, int W> __device__ __forceinline__ void add_n(const void *base, int64_t at, float *v, int n, bool f32, bool vec) {
     if (f32) {
         const float *o = (const float *) base + at;
-        if (vec && n == 4) return *(const f4 *) o;
-        for (int i = 0; i < 4; ++i) if (i < n) v[i] = o[i];
+        if (vec && n == W) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const f4 t = *(const f4 *) (o + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i + j] += t[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) if (i < n) v[i] += o[i];
+        }
     } else {
+        typedef T vt __attribute__((ext_vector_type(W)));
         const T *o = (const T *) base + at;
-        if (vec && n == 4) { const v4<T> t = *(const v4<T> *) o; return {(float) t[0], (float) t[1], (float) t[2], (float) t[3]}; }
-        for (int i = 0; i < 4; ++i) if (i < n) v[i] = (float) o[i];
+        if (vec && n == W) {
+            const vt t = *(const vt *) o;
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] += (float) t[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) if (i < n) v[i] += (float) o[i];
+        }
     }
-    return v;
 }
-// outputs c .. c + 3 of output row `row` from their sums; ob: element offset of the expert's gradient (TN), w: the pair's weight
-template <typename T> __device__ __forceinline__ void epi_store(const MMArgs &a, int64_t ob, int64_t row, int c, f4 v, float w) {
-    const int n = min(4, a.N - c);
+template <int ACT, int W> __device__ __forceinline__ void act_n(float *v) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = mm_act(ACT, v[i]);
+}
+// outputs c .. c + W - 1 of output row `row` from their sums; ob: element offset of the expert's gradient (TN), w: the pair's weight
+template <typename T, int W> __device__ __forceinline__ void epi_store(const MMArgs &a, int64_t ob, int64_t row, int c, float *v, float w) {
+    const int n = min(W, a.N - c);
     if (n <= 0) return;
     const bool vec = a.vec;
     if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < n) v[i] += a.bias[c + i];
+        for (int i = 0; i < W; ++i) if (i < n) v[i] += a.bias[c + i];
     }
-    if (a.z) put4<T>(a.z, row * a.ldz + c, v, n, false, vec);
-    if (a.act) {
+    if (a.z) put_n<T, W>(a.z, row * a.ldz + c, v, n, false, vec);
+    switch (a.act) {
+    case HY_ACT_RELU: act_n<HY_ACT_RELU, W>(v); break;
+    case HY_ACT_SILU: act_n<HY_ACT_SILU, W>(v); break;
+    case HY_ACT_GELU: act_n<HY_ACT_GELU, W>(v); break;
+    case HY_ACT_GELU_TANH: act_n<HY_ACT_GELU_TANH, W>(v); break;
+    }
+    if (a.wts) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = mm_act(a.act, v[i]);
+        for (int i = 0; i < W; ++i) v[i] *= w;
     }
-    if (a.wts) v *= w;
-    if (a.resid) v += get4<T>(a.resid, row * a.ldr + c, n, a.out_f32, vec);
+    if (a.resid) add_n<T, W>(a.resid, row * a.ldr + c, v, n, a.out_f32, vec);
     const int64_t at = ob + row * a.ldo + c;
-    if (a.accumulate) v += get4<T>(a.out, at, n, a.out_f32, vec);
-    put4<T>(a.out, at, v, n, a.out_f32, vec);
+    if (a.accumulate) add_n<T, W>(a.out, at, v, n, a.out_f32, vec);
+    put_n<T, W>(a.out, at, v, n, a.out_f32, vec);
 }
-// gated: h (and g, u) of columns c .. c + 3
-template <typename T> __device__ __forceinline__ void epi_glu(const MMArgs &a, int64_t row, int c, f4 g, f4 u) {
-    const int n = min(4, a.N - c);
+// gated: h (and g, u) of columns c .. c + W - 1
+template <typename T, int W> __device__ __forceinline__ void epi_glu(const MMArgs &a, int64_t row, int c, const float *g, const float *u) {
+    const int n = min(W, a.N - c);
     if (n <= 0) return;
     const int64_t at = row * a.ldo + c;
-    if (a.g) { put4<T>(a.g, at, g, n, false, a.vec); put4<T>(a.u, at, u, n, false, a.vec); }
-    f4 h;
+    if (a.g) { put_n<T, W>(a.g, at, g, n, false, a.vec); put_n<T, W>(a.u, at, u, n, false, a.vec); }
+    float h[W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = hy_swiglu(g[i], u[i], a.clamp);
-    put4<T>(a.out, at, h, n, false, a.vec);
+    for (int i = 0; i < W; ++i) h[i] = hy_swiglu(g[i], u[i], a.clamp);
+    put_n<T, W>(a.out, at, h, n, false, a.vec);
 }
 
 // ------------------------------------------------------------------ groups

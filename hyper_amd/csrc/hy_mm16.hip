@@ -119,10 +119,15 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
             if (a.wts && row >= 0) w = a.wts[row];
         }
         if (row < 0) continue;
-        if constexpr (DUAL) epi_glu<T>(a, row, c0 + wc * 16 + 4 * (lane >> 4), acc[0][j], acc[1][j]);
+        float v[2][4];
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i2][e] = acc[i2][j][e];
+        if constexpr (DUAL) epi_glu<T, 4>(a, row, c0 + wc * 16 + 4 * (lane >> 4), v[0], v[1]);
         else
 #pragma unroll
-            for (int i2 = 0; i2 < 2; ++i2) epi_store<T>(a, ob, row, c0 + wc * 32 + i2 * 16 + 4 * (lane >> 4), acc[i2][j], w);
+            for (int i2 = 0; i2 < 2; ++i2) epi_store<T, 4>(a, ob, row, c0 + wc * 32 + i2 * 16 + 4 * (lane >> 4), v[i2], w);
     }
     if constexpr (KIND == TN) {
         if (a.db && c0 == 0) {

@@ -24,8 +24,8 @@ static int check_out_type(const char *what, int type, int out_type) {
     if (out_type != HY_F32 && out_type != type) { set_error("%s: output type %d (HY_F32 or the operands' type)", what, out_type); return HY_EUNSUPPORTED_TYPE; }
     return HY_OK;
 }
-// four neighbouring values at columns that are multiples of 4 start on their own multiple
-static bool vec4(const void *p, int64_t ld, int bytes) { return !p || (ld % 4 == 0 && !misaligned(p, 4 * bytes)); }
+// eight neighbouring values at columns that are multiples of 8 start on 16 bytes
+static bool vec16(const void *p, int64_t ld, int bytes) { return !p || (ld % (16 / bytes) == 0 && !misaligned(p, 16)); }
 
 #define HY_TRY(e) do { const int rc_ = (e); if (rc_ != HY_OK) return rc_; } while (0)
 
@@ -114,7 +114,7 @@ int hy_linear(int type, const void *W, int64_t ldw, int n, int k, const void *x,
     a.P = W; a.ldp = ldw; a.Q = x; a.ldq = ldx; a.R = m; a.N = n; a.K = k;
     a.bias = bias; a.act = act; a.resid = resid; a.ldr = ldr; a.z = z; a.ldz = ldz; a.out = out; a.ldo = ldo;
     a.out_f32 = out_type == HY_F32;
-    a.vec = vec4(out, ldo, ob) && vec4(resid, ldr, ob) && vec4(z, ldz, 2);
+    a.vec = vec16(out, ldo, ob) && vec16(resid, ldr, ob) && vec16(z, ldz, 2);
     return m <= 4 ? launch_mv(type, false, a, s, what) : launch_mm(NT, type, false, a, s, what);
 }
 
@@ -132,7 +132,7 @@ int hy_linear_glu(int type, const void *Wg, const void *Wu, int64_t ldw, int n, 
     MMArgs a = args();
     a.P = Wg; a.P2 = Wu; a.ldp = ldw; a.Q = x; a.ldq = ldx; a.R = m; a.N = n; a.K = k;
     a.g = g; a.u = u; a.out = h; a.ldo = ldh; a.clamp = clamp;
-    a.vec = vec4(h, ldh, 2) && vec4(g, ldh, 2) && vec4(u, ldh, 2);
+    a.vec = vec16(h, ldh, 2) && vec16(g, ldh, 2) && vec16(u, ldh, 2);
     return m <= 4 ? launch_mv(type, true, a, s, what) : launch_mm(NT, type, true, a, s, what);
 }
 
@@ -161,7 +161,7 @@ int hy_linear_dx(int type, const void *W, int64_t ldw, int n, int k, const void 
     MMArgs a = args();
     a.P = W; a.ldp = ldw; a.Q = dz; a.ldq = lddz; a.R = m; a.N = k; a.K = n;
     a.resid = resid; a.ldr = ldr; a.out = dx; a.ldo = lddx; a.out_f32 = out_type == HY_F32;
-    a.vec = vec4(dx, lddx, ob) && vec4(resid, ldr, ob);
+    a.vec = vec16(dx, lddx, ob) && vec16(resid, ldr, ob);
     return launch_mm(NN, type, false, a, s, what);
 }
 
@@ -182,7 +182,7 @@ int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t 
     MMArgs a = args();
     a.P = x; a.ldp = ldx; a.Q = dz; a.ldq = lddz; a.R = n; a.N = k; a.K = m;
     a.out = dW; a.ldo = lddw; a.out_f32 = out_type == HY_F32; a.db = db; a.accumulate = accumulate != 0;
-    a.vec = vec4(dW, lddw, ob);
+    a.vec = vec16(dW, lddw, ob);
     return launch_mm(TN, type, false, a, s, what);
 }
 
@@ -200,7 +200,7 @@ int hy_moe16_gate_up(const hy_moe_dev *m, const void *x, int64_t ldx, int k, con
     MMArgs a = moe_args(m, n_pairs, ids, order, order_n, egrp, max_active);
     a.P = m->gate; a.P2 = m->up; a.ldp = m->n; a.Q = x; a.ldq = ldx; a.kq = (uint32_t) k; a.N = m->ff; a.K = m->n; a.R = 1;
     a.g = g; a.u = u; a.out = h; a.ldo = m->ff; a.clamp = m->clamp;
-    a.vec = vec4(h, m->ff, 2) && vec4(g, m->ff, 2) && vec4(u, m->ff, 2);
+    a.vec = vec16(h, m->ff, 2) && vec16(g, m->ff, 2) && vec16(u, m->ff, 2);
     return order ? launch_mm(NT, m->tg, true, a, s, what) : launch_mv(m->tg, true, a, s, what);
 }
 
@@ -218,7 +218,7 @@ int hy_moe16_down(const hy_moe_dev *m, const void *h, const int32_t *ids, int n_
     MMArgs a = moe_args(m, n_pairs, ids, order, order_n, egrp, max_active);
     a.P = m->down; a.ldp = m->ff; a.Q = h; a.ldq = m->ff; a.N = m->n; a.K = m->ff; a.R = 1;
     a.wts = wts; a.out = y; a.ldo = m->n; a.out_f32 = out_type == HY_F32;
-    a.vec = vec4(y, m->n, ob);
+    a.vec = vec16(y, m->n, ob);
     return order ? launch_mm(NT, m->td, false, a, s, what) : launch_mv(m->td, false, a, s, what);
 }
 
@@ -236,7 +236,7 @@ int hy_moe16_down_dx(const hy_moe_dev *m, const void *dy, int64_t lddy, int k, i
     MMArgs a = moe_args(m, n_pairs, nullptr, order, order_n, egrp, max_active);
     a.P = m->down; a.ldp = m->ff; a.Q = dy; a.ldq = lddy; a.kq = (uint32_t) k; a.N = m->ff; a.K = m->n;
     a.out = dh; a.ldo = m->ff; a.out_f32 = out_type == HY_F32;
-    a.vec = vec4(dh, m->ff, ob);
+    a.vec = vec16(dh, m->ff, ob);
     return launch_mm(NN, m->td, false, a, s, what);
 }
 
@@ -254,7 +254,7 @@ int hy_moe16_gate_up_dx(const hy_moe_dev *m, const void *dg, const void *du, int
     MMArgs a = moe_args(m, n_pairs, nullptr, order, order_n, egrp, max_active);
     a.P = m->gate; a.P2 = m->up; a.ldp = m->n; a.Q = dg; a.Q2 = du; a.ldq = m->ff; a.N = m->n; a.K = m->ff;
     a.out = dx; a.ldo = m->n; a.out_f32 = out_type == HY_F32;
-    a.vec = vec4(dx, m->n, ob);
+    a.vec = vec16(dx, m->n, ob);
     return launch_mm(NN, m->tg, false, a, s, what);
 }
 
@@ -275,7 +275,7 @@ int hy_moe16_dw(const hy_moe_dev *m, int type, const void *a_, int64_t lda, int 
     MMArgs a = moe_args(m, n_pairs, nullptr, order, order_n, egrp, max_active);
     a.P = b; a.ldp = ldb; a.kp = (uint32_t) kb; a.Q = a_; a.ldq = lda; a.kq = (uint32_t) ka; a.R = rows; a.N = cols;
     a.out = dW; a.ldo = cols; a.ostride = (int64_t) rows * cols; a.out_f32 = out_type == HY_F32; a.accumulate = accumulate != 0;
-    a.vec = vec4(dW, cols, ob);
+    a.vec = vec16(dW, cols, ob);
     return launch_mm(TN, type, false, a, s, what);
 }
 

@@ -218,7 +218,10 @@ template <typename T, int V> __global__ __launch_bounds__(256) void k_rows16(con
     for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t) gridDim.x * 256) {
         const int64_t r = i / per;
         const int c = (int) (i - r * per) * V;
-        if constexpr (V == 4) *(v4<T> *) (out + r * ldo + c) = to4<T>(*(const f4 *) (x + r * xs + c));
+        if constexpr (V == 4) {
+            const f4 v = *(const f4 *) (x + r * xs + c);
+            *(v4<T> *) (out + r * ldo + c) = v4<T>{(T) v[0], (T) v[1], (T) v[2], (T) v[3]};
+        }
         else out[r * ldo + c] = (T) x[r * xs + c];
     }
 }
