@@ -86,7 +86,6 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
     using OQ = Operand<KIND == TN, BM, NW, BK>;
     constexpr int NDMA = OP::N + OQ::N, STAGE = OP::BYTES + OQ::BYTES;
     constexpr int WN = BN / WP;                                  // columns a wave
-    static_assert(NST * STAGE >= NW * 16 * WN * 4, "the epilogue's rows fit the stages");
     constexpr int CH = 512;                                      // TN: contraction rows looked up at a time
     __shared__ __attribute__((aligned(1024))) uint8_t s_mem[NST * STAGE];
     __shared__ int s_pair[KIND == TN ? 1 : BM], s_look[KIND == TN ? 4 * CH : 1];
@@ -276,25 +275,28 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
     wait_vm<0>();
     __syncthreads();
 
-    // Epilogue, 16 rows of the wave at a time through its own part of the stages (row r's 16-byte piece c at c ^ r), so that a
-    // lane holds eight neighbouring columns and a row's lanes write whole lines
+    // Epilogue, 16 JP rows of the wave at a time through its own part of the stages (row r's 16-byte piece c at c ^ r), so
+    // that a lane holds eight neighbouring columns and a row's lanes write whole lines
     constexpr int PCS = WN / 4, X = PCS < 16 ? PCS - 1 : 15;
     constexpr int LPR = (DUAL ? WN / 2 : WN) / 8, RPI = 64 / LPR;   // lanes a row, rows at a time
-    const uint32_t own = lds0 + (uint32_t) wave * 16 * WN * 4;
+    constexpr int FIT = NST * STAGE / (NW * 16 * WN * 4), JP = FIT >= FQ ? FQ : FIT >= 4 && FQ % 4 == 0 ? 4 : FIT >= 2 && FQ % 2 == 0 ? 2 : 1;
+    static_assert(FIT >= 1 && FQ % JP == 0, "the epilogue's rows fit the stages");
+    const uint32_t own = lds0 + (uint32_t) wave * JP * 16 * WN * 4;
     const int cl = c0 + wp * (CN / WP) + lane % LPR * 8;
 #pragma unroll
-    for (int j = 0; j < FQ; ++j) {
-        {
+    for (int j0 = 0; j0 < FQ; j0 += JP) {
+#pragma unroll
+        for (int j = 0; j < JP; ++j) {
             const uint32_t r = lane & 15;
 #pragma unroll
             for (int i = 0; i < FP; ++i)
-                *(__attribute__((address_space(3))) f4 *) (uintptr_t) (own + r * (WN * 4) + (((uint32_t) (i * 4 + (lane >> 4)) ^ (r & X)) * 16)) = acc[i][j];
+                *(__attribute__((address_space(3))) f4 *) (uintptr_t) (own + (r + 16 * j) * (WN * 4) + (((uint32_t) (i * 4 + (lane >> 4)) ^ (r & X)) * 16)) = acc[i][j0 + j];
         }
         wave_sync();
 #pragma unroll 1
-        for (int h = 0; h < 16; h += RPI) {
-            const int r = (h + lane / LPR) & 15;
-            const int i0 = wq * (BM / WQ) + j * 16 + r;
+        for (int h = 0; h < 16 * JP; h += RPI) {
+            const int r = RPI <= 16 ? h + lane / LPR : h + (lane / LPR) % (16 * JP);
+            const int i0 = wq * (BM / WQ) + j0 * 16 + r;
             int row;
             int64_t ob = 0;
             float w = 1.0f;
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
                 row = s_pair[i0];
                 if (a.wts && row >= 0) w = a.wts[row];
             }
-            if (RPI > 16 && lane / LPR >= 16) row = -1;   // lanes without a row
+            if (RPI > 16 * JP && lane / LPR >= 16 * JP) row = -1;   // lanes without a row
             auto piece = [&](int c) { return lds_get<f4>(own + (uint32_t) r * (WN * 4) + (((uint32_t) c ^ ((uint32_t) r & X)) * 16)); };
             union { f4 q[2]; float v[8]; } u, g2;
             if constexpr (DUAL) {
@@ -322,9 +324,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
             }
         }
         wave_sync();
-        if constexpr (KIND == TN) {
-            const int row = r0 + wq * (BM / WQ) + j * 16 + lane;
-            if (do_db && lane < 16 && row < a.R) a.db[row] = a.accumulate ? a.db[row] + dbs[j][0] : dbs[j][0];
+    }
+    if constexpr (KIND == TN) {
+        if (do_db && lane < 16) {
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) {
+                const int row = r0 + wq * (BM / WQ) + j * 16 + lane;
+                if (row < a.R) a.db[row] = a.accumulate ? a.db[row] + dbs[j][0] : dbs[j][0];
+            }
         }
     }
 }
