@@ -4,11 +4,10 @@
 
 namespace hy {
 
-// 16 bytes a lane from per-lane addresses to 1 KB of LDS at `lds` (lane l's bytes at lds + 16 l), in flight when it returns
+// 16 bytes a lane from per-lane addresses to 1 KB of LDS at `lds` (lane l's bytes at lds + 16 l), in flight when it returns.
+// M0 holds the LDS address; the compiler uses M0 only within sequences of its own, which set it themselves.
 __device__ __forceinline__ void dma16(const char *src, uint32_t lds) {
-    uint32_t keep;   // M0 holds the LDS address of a DMA; it is saved and restored around it
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
 }
 template <typename V> __device__ __forceinline__ V lds_get(uint32_t addr) { return *(const __attribute__((address_space(3))) V *) (uintptr_t) addr; }
 // what the wave's lanes wrote to LDS before is what its lanes read behind (LDS operations of a wave keep their order; this
@@ -25,65 +24,69 @@ __device__ __forceinline__ s4 lds_get_tr(uint32_t addr) {
 }
 static __device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
 
-// How an operand's tile of S rows (or columns) by BK contraction values lies in LDS, in 16-byte pieces:
-//  along the contraction (TR false): row r at r * 2 BK, its piece c at c ^ (r & 7) (BK 64) or c ^ (r >> 2 & 3) (BK 32): a
-//  fragment read takes one piece of each of 16 rows, 16 lanes at a time in 16 different places of 256 bytes
-//  across it (TR true): contraction row k at k * 2 S, its pair of pieces u at u ^ F(k), F = k & 3 | bit 3 of k << 2: a
-//  transposing read takes 32 bytes of the rows 8 q + 0..3 (or 4..7) of two quarters q at a time, eight different F
-// Both read at 240 bytes a clock and CU (256 is the most).
-template <bool TR, int S, int NW, int BK> struct Operand {
+// How an operand's tile of S rows (or columns) by BK = 64 contraction values lies in LDS, in 16-byte pieces:
+//  along the contraction (TR false): row r at r * 128, its piece c at c ^ (r & 7): a fragment read takes one piece of each of 16
+//  rows, 16 lanes at a time in different places of 256 bytes
+//  across it (TR true): contraction row k at k * 2 S, its pair of pieces u at u ^ F(k), F = k & 3 | bit 3 of k << 2 (S 64:
+//  k & 3): a transposing read takes 32 bytes of the rows 8 q + 0..3 (or 4..7) of two quarters q at a time, eight different F
+// Both read at 240 bytes a clock and CU (256 is the most).  Rows of 128 bytes are whole lines: 32 values a stage (64 bytes)
+// halved the rate at which all CUs together fetch from L2 (67 against 133 bytes / ns and CU).
+constexpr int BK = 64;
+template <bool TR, int S, int NW> struct Operand {
     static constexpr int N = S * BK / 512 / NW;   // DMAs (of 1 KB) a wave and stage
     static_assert(N * 512 * NW == S * BK, "whole DMAs");
     static constexpr int BYTES = S * BK * 2;
-    static constexpr int CPR = TR ? S / 8 : BK / 8, RPI = 64 / CPR;   // pieces a stored row, stored rows a DMA
-    const char *p[N];
+    static constexpr int CPR = TR ? S / 8 : 8, RPI = 64 / CPR;   // pieces a stored row, stored rows a DMA
+    const char *p[N];     // the lanes' places in the first stage
+    const char *cur[N];   // and in the next one to fetch
 
     // the DMA's contraction row within the stage (TR) / first contraction value of the lane's piece (not TR)
     static __device__ __forceinline__ int krow(int wave, int lane, int i) {
         if constexpr (TR) return (wave * N + i) * RPI + lane / CPR;
-        else if constexpr (BK == 64) return ((lane & 7) ^ (lane >> 3)) * 8;
-        else return ((lane & 3) ^ (lane >> 4)) * 8;
+        else return ((lane & 7) ^ (lane >> 3)) * 8;
     }
     // the lane's row (not TR) / first column (TR) within the tile
     static __device__ __forceinline__ int at(int wave, int lane, int i) {
         if constexpr (TR) {
-            const int k = krow(wave, lane, i), pc = lane % CPR, F = (k & 3) | ((k >> 1) & 4);
+            const int k = krow(wave, lane, i), pc = lane % CPR, F = (k & 3) | (S >= 128 ? (k >> 1) & 4 : 0);
             return (((pc >> 1) ^ F) * 2 + (pc & 1)) * 8;
         } else return (wave * N + i) * RPI + lane / CPR;
     }
-    static __device__ __forceinline__ uint32_t dst(uint32_t tile, int wave, int i) { return tile + (uint32_t) (wave * N + i) * 1024; }
-
-    // lane's part of the address of a fragment (16 rows / columns from `base`, a multiple of 16, on; 32 contraction values kk)
+    // lane's part of the address of a fragment (16 rows / columns; 32 contraction values)
     static __device__ __forceinline__ uint32_t frag_addr(int lane) {
         if constexpr (TR) {
-            const int F = ((lane >> 2) & 3) | ((lane >> 2) & 4);
+            const int F = ((lane >> 2) & 3) | (S >= 128 ? (lane >> 2) & 4 : 0);
             return (uint32_t) (((lane >> 4) * 8 + ((lane >> 2) & 3)) * 2 * S + F * 32 + (lane & 3) * 8);
-        } else if constexpr (BK == 64) return (uint32_t) ((lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16));
-        else return (uint32_t) ((lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16));
+        } else return (uint32_t) ((lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16));
     }
-    template <typename T> static __device__ __forceinline__ v8<T> frag(uint32_t tile, uint32_t fa, int base, int kk) {
+    // fragment i of the wave's rows / columns from w0 (a multiple of 64, or of 32 with S >= 64), half kk of the stage;
+    // fa: frag_addr, `base` the stage's place in LDS
+    template <typename T> static __device__ __forceinline__ v8<T> frag(uint32_t base, uint32_t fa, int w0, int i, int kk) {
         if constexpr (TR) {
-            const uint32_t ad = tile + (fa ^ (uint32_t) (base * 2)) + (uint32_t) (kk * 64 * S);
+            const uint32_t ad = base + (fa ^ (uint32_t) ((w0 + i * 16) * 2));
             union { s4 h[2]; v8<T> v; } r;
-            r.h[0] = lds_get_tr(ad);
-            r.h[1] = lds_get_tr(ad + 8 * S);
+            r.h[0] = lds_get_tr(ad + (uint32_t) (kk * 64 * S));
+            r.h[1] = lds_get_tr(ad + (uint32_t) (kk * 64 * S + 8 * S));
             return r.v;
-        } else return lds_get<v8<T>>(tile + (fa ^ (uint32_t) (kk * 64)) + (uint32_t) (base * 2 * BK));
+        } else return lds_get<v8<T>>(base + (fa ^ (uint32_t) (kk * 64)) + (uint32_t) (w0 * 128) + (uint32_t) (i * 2048));
     }
 };
+__device__ __forceinline__ void mfma_acc(f4 &c, v8<bf16> a, v8<bf16> b) { asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void mfma_acc(f4 &c, v8<f16> a, v8<f16> b) { asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 
-// One BM x BN tile (output rows x columns) a block of WP x WQ waves, BN / WP columns by BM / WQ rows each; stages of BK
-// contraction values, NST of them in LDS.
+// One BM x BN tile (output rows x columns) a block of WP x WQ waves, BN / WP columns by BM / WQ rows each; stages of 64
+// contraction values, NST of them in LDS, one barrier a stage.
 //
-// Eight waves (two a SIMD) work in turns: a barrier ends every part, and the second four waves are one part behind, so that
-// on each SIMD one wave multiplies while the other reads its next fragments and starts the DMAs three stages on.
-template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int BK, int NST>
-__global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
+// A stage is two halves of 32 values.  While one half's products run, the wave reads the next half's fragments into the other
+// registers and, behind the barrier, starts the DMAs of the stage NST on (whose place every wave has read by then): the reads
+// and DMAs go between the products one at a time, since a wave issues in order and two or three instructions hide behind a
+// product of 16 clocks.
+template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
+__global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) void k_mm(const MMArgs a) {
     constexpr int NW = WP * WQ, NTH = 64 * NW, FP = BN / WP / 16, FQ = BM / WQ / 16;
-    constexpr bool TURNS = NW == 8;
-    static_assert(!TURNS || (BK == 32 && NST == 4), "the turns' DMA distance");
-    using OP = Operand<KIND != NT, BN, NW, BK>;
-    using OQ = Operand<KIND == TN, BM, NW, BK>;
+    constexpr bool WIDE = FP * FQ == 64;   // 256 sums a lane: in the accumulation registers
+    using OP = Operand<KIND != NT, BN, NW>;
+    using OQ = Operand<KIND == TN, BM, NW>;
     constexpr int NDMA = OP::N + OQ::N, STAGE = OP::BYTES + OQ::BYTES;
     constexpr int WN = BN / WP;                                  // columns a wave
     constexpr int CH = 512;                                      // TN: contraction rows looked up at a time
@@ -122,7 +125,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
             P.p[i] = M + c * ldp2 + OP::krow(wave, lane, i) * 2;
         } else {
             const int c = c0 + at < a.N ? c0 + at : c0;
-            P.p[i] = Pb + c * 2 + (KIND == NN ? OP::krow(wave, lane, i) * ldp2 : 0);
+            P.p[i] = Pb + c * 2 + (KIND == TN && a.order ? 0 : OP::krow(wave, lane, i) * ldp2);
         }
     }
 #pragma unroll
@@ -130,13 +133,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
         const int at = OQ::at(wave, lane, i);
         if constexpr (KIND == TN) {
             const int r = r0 + at < a.R ? r0 + at : r0;
-            Q.p[i] = (const char *) a.Q + r * 2;
+            Q.p[i] = (const char *) a.Q + r * 2 + (a.order ? 0 : OQ::krow(wave, lane, i) * ldq2);
         } else {
             const int p = max(s_pair[at], 0);
             Q.p[i] = (const char *) a.Q + div_k(p, a.kq, mq) * ldq2 + OQ::krow(wave, lane, i) * 2;
         }
     }
-    const uint32_t lds0 = lds_addr(s_mem);
+    const uint32_t lds0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds_addr(s_mem));
     const int per_part = (K + BK - 1) / BK, nstage = KIND == NN && a.P2 ? 2 * per_part : per_part;
     const char *zero = (const char *) g_zero16;
 
@@ -151,46 +154,54 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
             }
         }
     };
-    auto issue = [&](int s, int buf) {
-        const uint32_t tp = lds0 + (uint32_t) buf * STAGE, tq = tp + OP::BYTES;
-        if constexpr (KIND == TN) {
+    // The places to fetch stage s from.  They move on by a constant distance, but where a part begins or ends: at stage
+    // `event` they are made anew.  By pairs (TN) every stage makes them anew.
+    int64_t step_p = 0, step_q = 0;
+    int event = 0;
+    auto places = [&](int s) {
+        if (KIND == TN && a.order) {
+            if constexpr (KIND == TN) {
 #pragma unroll
-            for (int i = 0; i < OP::N; ++i) {
-                const int k = s * BK + OP::krow(wave, lane, i);
-                int r = k < K ? k : -1;
-                if (a.order && r >= 0) r = s_look[k & (2 * CH - 1)];
-                dma16(r >= 0 ? P.p[i] + r * ldp2 : zero, OP::dst(tp, wave, i));
-            }
+                for (int i = 0; i < OP::N; ++i) {
+                    const int r = s_look[(s * BK + OP::krow(wave, lane, i)) & (2 * CH - 1)];
+                    P.cur[i] = s < nstage && r >= 0 ? P.p[i] + r * ldp2 : zero;
+                }
 #pragma unroll
-            for (int i = 0; i < OQ::N; ++i) {
-                const int k = s * BK + OQ::krow(wave, lane, i);
-                int r = k < K ? k : -1;
-                if (a.order && r >= 0) r = s_look[2 * CH + (k & (2 * CH - 1))];
-                dma16(r >= 0 ? Q.p[i] + r * ldq2 : zero, OQ::dst(tq, wave, i));
+                for (int i = 0; i < OQ::N; ++i) {
+                    const int r = s_look[2 * CH + ((s * BK + OQ::krow(wave, lane, i)) & (2 * CH - 1))];
+                    Q.cur[i] = s < nstage && r >= 0 ? Q.p[i] + r * ldq2 : zero;
+                }
             }
+            return;
+        }
+        if (s < event) return;
+        int64_t dp = 0, dq = 0;
+        int sl = s;
+        if (KIND == NN && a.P2 && s >= per_part) {   // the second part's matrices
+            sl = s - per_part;
+            dp = (const char *) a.P2 - (const char *) a.P;
+            dq = (const char *) a.Q2 - (const char *) a.Q;
+        }
+        const int left = s < nstage ? K - sl * BK : 0;   // contraction values left of the part
+        step_p = left > 0 ? (KIND == NT ? 2 * BK : BK * ldp2) : 0;
+        step_q = left > 0 ? (KIND == TN ? BK * ldq2 : 2 * BK) : 0;
+        dp += (KIND == NT ? 2 * BK : BK * ldp2) * (int64_t) sl;
+        dq += (KIND == TN ? BK * ldq2 : 2 * BK) * (int64_t) sl;
+#pragma unroll
+        for (int i = 0; i < OP::N; ++i) P.cur[i] = OP::krow(wave, lane, i) < left ? P.p[i] + dp : zero;
+#pragma unroll
+        for (int i = 0; i < OQ::N; ++i) Q.cur[i] = OQ::krow(wave, lane, i) < left ? Q.p[i] + dq : zero;
+        // whole stages follow up to the part's last, partial one (or the next part)
+        event = left <= 0 ? 0x7fffffff : left < 2 * BK ? s + 1 : s + left / BK;
+    };
+    auto fetch = [&](int i, uint32_t stage) {   // the i-th DMA of the stage at LDS address `stage`
+        if (i < OP::N) {
+            dma16(P.cur[i < OP::N ? i : 0], stage + (uint32_t) (wave * OP::N + i) * 1024);
+            P.cur[i < OP::N ? i : 0] += step_p;
         } else {
-            int64_t dp = 0, dq = 0;
-            int sl = s;
-            if (KIND == NN && a.P2 && s >= per_part) {   // the second part's matrices
-                sl = s - per_part;
-                dp = (const char *) a.P2 - (const char *) a.P;
-                dq = (const char *) a.Q2 - (const char *) a.Q;
-            }
-            dp += (KIND == NT ? 2 * BK : BK * ldp2) * (int64_t) sl;
-            dq += 2 * BK * (int64_t) sl;
-            const bool full = sl * BK + BK <= K;
-#pragma unroll
-            for (int i = 0; i < OP::N; ++i) {
-                const char *src = P.p[i] + dp;
-                if (!full && sl * BK + OP::krow(wave, lane, i) >= K) src = zero;
-                dma16(src, OP::dst(tp, wave, i));
-            }
-#pragma unroll
-            for (int i = 0; i < OQ::N; ++i) {
-                const char *src = Q.p[i] + dq;
-                if (!full && sl * BK + OQ::krow(wave, lane, i) >= K) src = zero;
-                dma16(src, OQ::dst(tq, wave, i));
-            }
+            const int j = i < OP::N ? 0 : i - OP::N;
+            dma16(Q.cur[j], stage + OP::BYTES + (uint32_t) (wave * OQ::N + j) * 1024);
+            Q.cur[j] += step_q;
         }
     };
 
@@ -198,79 +209,91 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
     f4 dbs[KIND == TN ? FQ : 1] = {};
     const bool do_db = KIND == TN && a.db && col == 0 && wp == 0;
     const uint32_t fap = OP::frag_addr(lane), faq = OQ::frag_addr(lane);
-    auto read = [&](v8<T> (&fp)[FP], v8<T> (&fq)[FQ], uint32_t tp, int kk) {
-#pragma unroll
-        for (int j = 0; j < FQ; ++j) fq[j] = OQ::template frag<T>(tp + OP::BYTES, faq, wq * (BM / WQ) + j * 16, kk);
-#pragma unroll
-        for (int i = 0; i < FP; ++i) fp[i] = OP::template frag<T>(tp, fap, wp * WN + i * 16, kk);
+    v8<T> fp[2][FP], fq[2][FQ];
+    // the o-th fragment of half kk: the first column's, the rows', then the other columns' (the order of their use)
+    auto read = [&](int o, int kk, uint32_t bp, uint32_t bq) {
+        if (o == 0) fp[kk][0] = OP::template frag<T>(bp, fap, wp * WN, 0, kk);
+        else if (o <= FQ) fq[kk][o <= FQ && o > 0 ? o - 1 : 0] = OQ::template frag<T>(bq, faq, wq * (BM / WQ), o - 1, kk);
+        else fp[kk][o > FQ ? o - FQ : 0] = OP::template frag<T>(bp, fap, wp * WN, o - FQ, kk);
     };
-    auto multiply = [&](const v8<T> (&fp)[FP], const v8<T> (&fq)[FQ]) {
-#pragma unroll
-        for (int i = 0; i < FP; ++i)
-#pragma unroll
-            for (int j = 0; j < FQ; ++j) acc[i][j] = mfma16(fp[i], fq[j], acc[i][j]);
+    auto product = [&](int m, int kk) {
+        if constexpr (WIDE) mfma_acc(acc[m / FQ][m % FQ], fp[kk][m / FQ], fq[kk][m % FQ]);
+        else acc[m / FQ][m % FQ] = mfma16(fp[kk][m / FQ], fq[kk][m % FQ], acc[m / FQ][m % FQ]);
+    };
+    auto db_product = [&](int kk) {   // the rows' sums as a product with ones
         if constexpr (KIND == TN) {
-            if (do_db) {   // the rows' sums as a product with ones
+            if (do_db) {
                 v8<T> one;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) one[e] = (T) 1.0f;
 #pragma unroll
-                for (int j = 0; j < FQ; ++j) dbs[j] = mfma16(one, fq[j], dbs[j]);
+                for (int j = 0; j < FQ; ++j) dbs[j] = mfma16(one, fq[kk][j], dbs[j]);
             }
         }
     };
+    constexpr int NM = FP * FQ, NR = FP + FQ;
     if constexpr (KIND == TN) {
         look_up(0);
         look_up(1);
         __syncthreads();
     }
-    // one chunk is looked up while the one before is in use: behind its last DMA, before the next chunk's first
-    auto look_ahead = [&](int s) {
+    // stages behind the last are DMAs of zeros, so that the counts of DMAs in flight stay the same
+    for (int s = 0; s < NST; ++s) {
+        places(s);
+#pragma unroll
+        for (int i = 0; i < NDMA; ++i) fetch(i, lds0 + (uint32_t) s * STAGE);
+    }
+    wait_vm<(NST - 1) * NDMA>();
+    lds_barrier();
+#pragma unroll
+    for (int o = 0; o < NR; ++o) read(o, 0, lds0, lds0 + OP::BYTES);
+    uint32_t at = lds0;
+    for (int s = 0; s < nstage; ++s) {
+        uint32_t nx = at + STAGE;
+        if (nx == lds0 + NST * STAGE) nx = lds0;
         if constexpr (KIND == TN) {
+            // one chunk is looked up while the one before is in use: behind its last DMA, before the next chunk's first
             constexpr int SPC = CH / BK;   // stages a chunk
+            static_assert(KIND != TN || NST < SPC / 2, "a chunk is in place before its first DMA");
             if (a.order && s % SPC == SPC / 2 && s > SPC) look_up(s / SPC + 1);
         }
-    };
-    if constexpr (TURNS) {
-        // stages behind the last are DMAs of zeros, so that the counts of DMAs in flight stay the same
-        for (int s = 0; s < 3; ++s) issue(s, s);
-        wait_vm<2 * NDMA>();
-        lds_barrier();
-        if (wave >= 4) __builtin_amdgcn_s_barrier();
-        for (int s = 0; s < nstage; ++s) {
-            v8<T> fp[FP], fq[FQ];
-            read(fp, fq, lds0 + (uint32_t) (s & 3) * STAGE, 0);
-            look_ahead(s);
-            issue(s + 3, (s + 3) & 3);
-            wait_vm<2 * NDMA>();   // stage s + 1 is in place
-            lds_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(1);
-            multiply(fp, fq);
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
-            lds_barrier();
-        }
-        if (wave < 4) __builtin_amdgcn_s_barrier();
-    } else {
-        for (int s = 0; s < NST - 1; ++s)
-            if (s < nstage) issue(s, s);
-        int buf = 0;
-        for (int s = 0; s < nstage; ++s) {
-            // this stage has landed for every wave, and every wave is done with the one before
-            if (NST > 2 && s + NST - 2 < nstage) wait_vm<(NST - 2) * NDMA>();
-            else wait_vm<0>();
-            lds_barrier();
-            look_ahead(s);
-            if (s + NST - 1 < nstage) issue(s + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+        places(s + NST);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t bp = at, bq = at + OP::BYTES;
 #pragma unroll
-            for (int kk = 0; kk < BK / 32; ++kk) {
-                v8<T> fp[FP], fq[FQ];
-                read(fp, fq, lds0 + (uint32_t) buf * STAGE, kk);
-                multiply(fp, fq);
-            }
-            buf = buf == NST - 1 ? 0 : buf + 1;
+        for (int m = 0; m < NM; ++m) {
+            product(m, 0);
+#pragma unroll
+            for (int o = m * NR / NM; o < (m + 1) * NR / NM; ++o) read(o, 1, bp, bq);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        db_product(0);
+        wait_vm<(NST - 2) * NDMA>();   // stage s + 1 is in place
+        lds_barrier();                 // for every wave, and every wave has read this one
+        bp = nx;
+        bq = nx + OP::BYTES;
+        constexpr int NO = NR + NDMA;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            product(m, 1);
+#pragma unroll
+            for (int o = m * NO / NM; o < (m + 1) * NO / NM; ++o) {
+                // reads and DMAs in turn
+                const int rd = (o + 1) * NR / NO, rd0 = o * NR / NO;
+                if (rd > rd0) read(rd0, 0, bp, bq);
+                else fetch(o - rd0, at);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        db_product(1);
+        at = nx;
+    }
+    if constexpr (WIDE) {   // the last products end before their sums are read
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) asm volatile("" : "+a"(acc[i][j]));
     }
     wait_vm<0>();
     __syncthreads();
@@ -336,14 +359,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_mm(const MMArgs a) {
     }
 }
 
-template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int BK, int NST>
+template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
 static int launch_tile(const MMArgs &a, hipStream_t s, const char *what) {
     const int64_t ncol = (a.N + (DUAL ? BN / 2 : BN) - 1) / (DUAL ? BN / 2 : BN);
     const int64_t items = KIND == TN || !a.egrp ? ((int64_t) a.R + BM - 1) / BM : ((int64_t) a.n_pairs + BM - 1) / BM + a.max_active;
     const int64_t blocks = ncol * items;
     if (blocks <= 0) return HY_OK;
     if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
-    k_mm<T, KIND, DUAL, BM, BN, WP, WQ, BK, NST><<<dim3((uint32_t) blocks, KIND == TN && a.egrp ? (uint32_t) a.n_local : 1u), 64 * WP * WQ, 0, s>>>(a);
+    k_mm<T, KIND, DUAL, BM, BN, WP, WQ, NST><<<dim3((uint32_t) blocks, KIND == TN && a.egrp ? (uint32_t) a.n_local : 1u), 64 * WP * WQ, 0, s>>>(a);
     return check_launch(what);
 }
 
