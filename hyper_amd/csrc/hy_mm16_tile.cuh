@@ -2,6 +2,8 @@
 #pragma once
 #include "hy_mm16.cuh"
 
+#include <cmath>
+
 namespace hy {
 
 // 16 bytes a lane from per-lane addresses to 1 KB of LDS at `lds` (lane l's bytes at lds + 16 l), in flight when it returns.
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) v
         for (int m = 0; m < NM; ++m) {
             product(m, 0);
 #pragma unroll
-            for (int o = m * NR / NM; o < (m + 1) * NR / NM; ++o) read(o, 1, bp, bq);
+            for (int o = min(NR, m * NR * 3 / (NM * 2)); o < min(NR, (m + 1) * NR * 3 / (NM * 2)); ++o) read(o, 1, bp, bq);   // done by two thirds: the barrier waits for them
             __builtin_amdgcn_sched_barrier(0);
         }
         db_product(0);
@@ -368,6 +370,44 @@ static int launch_tile(const MMArgs &a, hipStream_t s, const char *what) {
     if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
     k_mm<T, KIND, DUAL, BM, BN, WP, WQ, NST><<<dim3((uint32_t) blocks, KIND == TN && a.egrp ? (uint32_t) a.n_local : 1u), 64 * WP * WQ, 0, s>>>(a);
     return check_launch(what);
+}
+
+// ------------------------------------------------------------------ which tile
+
+// A tile's rows, columns, tiles that run at once (256 CUs times those that fit a CU), and its cost in microseconds: of one stage
+// when few tiles run, when 256 run, when all of `slots` run, and of its start and epilogue.  Measured on bf16 forward products:
+// 4096^3 (as many rounds of full slots as tiles ask), 256 tiles and fewer of 2048 .. 4096 contraction values.
+struct TileCost { int bm, bn, slots; float few, t256, full, ends; };
+constexpr TileCost T256x256{256, 256, 256, 1.37f, 2.07f, 2.07f, 7.0f}, T128x128{128, 128, 512, 0.66f, 0.88f, 1.19f, 3.0f},
+    T64x128{64, 128, 512, 0.345f, 0.40f, 0.708f, 2.0f}, T64x64{64, 64, 512, 0.26f, 0.272f, 0.5f, 1.5f},
+    T32x128{32, 128, 512, 0.286f, 0.30f, 0.574f, 1.5f}, T32x64{32, 64, 512, 0.20f, 0.22f, 0.334f, 1.2f};
+
+// rounds of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, half a tile over
+// in each group that has more than half a tile.
+inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual) {
+    const int cn = dual ? t.bn / 2 : t.bn;
+    const double ncol = (a.N + cn - 1) / cn, groups = a.egrp ? std::max(1, std::min({a.max_active, a.n_expert, a.n_pairs})) : 1;
+    double rows = kind == TN ? (double) ((a.R + t.bm - 1) / t.bm) * (a.egrp ? a.n_local : 1)
+                  : !a.egrp  ? (double) (((int64_t) a.R + t.bm - 1) / t.bm)
+                             : groups * std::max(1.0, a.n_pairs / groups / t.bm + 0.5);
+    const double stages = kind == TN ? (a.egrp ? a.n_pairs / groups : a.K) / BK + 1 : (double) (a.K + BK - 1) / BK * (kind == NN && a.P2 ? 2 : 1);
+    const double tiles = rows * ncol, whole = std::floor(tiles / t.slots), left = tiles - whole * t.slots;
+    double part = 0;
+    if (left >= 1) {
+        const double st = left <= 256 ? t.few + (t.t256 - t.few) * left / 256 : t.t256 + (t.full - t.t256) * (left - 256) / std::max(1, t.slots - 256);
+        part = stages * st + t.ends;
+    }
+    return (float) (whole * (stages * t.full + t.ends) + part);
+}
+// the cheapest of the tiles
+template <int N> inline int cheapest(const TileCost (&t)[N], const MMArgs &a, int kind, bool dual) {
+    int best = 0;
+    float least = tile_cost(t[0], a, kind, dual);
+    for (int i = 1; i < N; ++i) {
+        const float c = tile_cost(t[i], a, kind, dual);
+        if (c < least) { least = c; best = i; }
+    }
+    return best;
 }
 
 } // namespace hy

@@ -69,7 +69,7 @@ template <typename T, bool DUAL, int NR, bool AL> __global__ __launch_bounds__(2
         if constexpr (DUAL) {
             const int64_t at = row * a.ldo + c0;
             if (a.g) { ((T *) a.g)[at] = (T) acc[0][r]; ((T *) a.u)[at] = (T) acc[1][r]; }
-            ((T *) a.out)[at] = (T) hy_swiglu(acc[0][r], acc[1][r], a.clamp);
+            ((T *) a.out)[at] = (T) mm_swiglu(acc[0][r], acc[1][r], a.clamp);
         } else {
             const float wt = a.wts ? a.wts[row] : 1.0f;
 #pragma unroll
@@ -176,7 +176,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void k_swiglu_bwd
                 gg = fminf(gg, L);
                 uu = fminf(fmaxf(uu, -L), L);
             }
-            const float s = hy_sigmoid(gg), silu = gg * s, h = silu * uu;
+            const float s = mm_sigmoid(gg), silu = gg * s, h = silu * uu;
             sum = fmaf(d, h, sum);
             oh[j] = (T) (w * h);
             og[j] = (T) (gin ? w * d * uu * fmaf(silu, 1.0f - s, s) : 0.0f);

@@ -24,7 +24,7 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 def _type16(t: torch.Tensor) -> int:
     v = _TYPE.get(t.dtype)
-    if v not in (HY_F16, HY_BF16):
+    if v != HY_BF16 and v != HY_F16:
         raise ValueError(f"expected bfloat16 or float16, got {t.dtype}")
     return v
 
@@ -33,46 +33,45 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """the call's device and stream: every tensor on one GPU, which is current while the call launches"""
-
-    def __init__(self, ref: torch.Tensor, stream, *others: Optional[torch.Tensor]):
-        dev = ref.device
-        if dev.type != "cuda":
-            raise ValueError(f"tensors must be on a GPU, got {dev}")
-        for t in others:
-            if t is not None and t.device != dev:
-                raise ValueError(f"tensors on {dev} and {t.device}")
-        if stream is not None and stream.device != dev:
-            raise ValueError(f"a stream of {stream.device} for tensors on {dev}")
-        self.stream = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
-        self.guard = None if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(fn, ref: torch.Tensor, stream, others, *args) -> None:
+    """fn(*args, stream) on ref's GPU, which is current while the call launches; every tensor must be on it.  (Written for
+    few Python steps: a decode call's kernel takes about as long as its checks.)"""
+    dev = ref.get_device()
+    if dev < 0:
+        raise ValueError(f"tensors must be on a GPU, got {ref.device}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {ref.device} and {t.device}")
+    if stream is None:
+        raw = torch._C._cuda_getCurrentRawStream(dev)
+    elif stream.device_index != dev:
+        raise ValueError(f"a stream of cuda:{stream.device_index} for tensors on {ref.device}")
+    else:
+        raw = stream.cuda_stream
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, raw)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, raw)
+    if rc:
+        check(rc)
 
 
 def _mat(name: str, t: torch.Tensor, rows: Optional[int], cols: int, *dtypes, least: bool = False) -> int:
     """checks a row-major matrix and returns the elements between its rows (least: it may have more rows)"""
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and (t.shape[0] < rows if least else t.shape[0] != rows)):
-        raise ValueError(f"{name} must be [{'*' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or (rows is not None and (shape[0] < rows if least else shape[0] != rows)):
+        raise ValueError(f"{name} must be [{'*' if rows is None else rows}, {cols}], got {tuple(shape)}")
     if dtypes and t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if cols > 1 and t.stride(1) != 1:
+    between, step = t.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{name} must have contiguous rows")
-    return max(t.stride(0), 0) if t.shape[0] > 1 else cols
+    return between if shape[0] > 1 else cols
 
 
 def _vec(name: str, t: Optional[torch.Tensor], n: int, dtype) -> None:
-    if t is None:
-        return
-    if t.numel() < n or t.dtype != dtype or not t.is_contiguous():
+    if t is not None and (t.dtype != dtype or t.numel() < n or not t.is_contiguous()):
         raise ValueError(f"{name} must hold {n} contiguous {dtype} values, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -93,9 +92,8 @@ def linear(W, x, out, bias=None, act="none", resid=None, z=None, stream=None):
     ldr = _mat("resid", resid, m, n, out.dtype) if resid is not None else 0
     ldz = _mat("z", z, m, n, W.dtype) if z is not None else 0
     _vec("bias", bias, n, torch.float32)
-    with _On(W, stream, x, out, bias, resid, z) as s:
-        check(lib().hy_linear(ty, _p(W), ldw, n, k, _p(x), ldx, m, _p(bias), _act(act), _p(resid), ldr, _p(z), ldz, _p(out),
-                              _TYPE[out.dtype], ldo, s))
+    _call(lib().hy_linear, W, stream, (x, out, bias, resid, z),
+          ty, _p(W), ldw, n, k, _p(x), ldx, m, _p(bias), _act(act), _p(resid), ldr, _p(z), ldz, _p(out), _TYPE[out.dtype], ldo)
 
 
 def linear_glu(Wg, Wu, x, h, clamp=0.0, g=None, u=None, stream=None):
@@ -108,16 +106,15 @@ def linear_glu(Wg, Wu, x, h, clamp=0.0, g=None, u=None, stream=None):
     for name, t in (("g", g), ("u", u)):
         if t is not None and _mat(name, t, m, n, Wg.dtype) != ldh:
             raise ValueError(f"{name} must have h's row stride")
-    with _On(Wg, stream, Wu, x, h, g, u) as s:
-        check(lib().hy_linear_glu(ty, _p(Wg), _p(Wu), ldw, n, k, _p(x), ldx, m, float(clamp), _p(g), _p(u), _p(h), ldh, s))
+    _call(lib().hy_linear_glu, Wg, stream, (Wu, x, h, g, u),
+          ty, _p(Wg), _p(Wu), ldw, n, k, _p(x), ldx, m, float(clamp), _p(g), _p(u), _p(h), ldh)
 
 
 def act_bwd(act, z, dy, dz, stream=None):
     """dz = dy act'(z), all [m, n] of one 16-bit type."""
     ty, (m, n) = _type16(z), z.shape
     ldz, ldd, ldo = _mat("z", z, m, n), _mat("dy", dy, m, n, z.dtype), _mat("dz", dz, m, n, z.dtype)
-    with _On(z, stream, dy, dz) as s:
-        check(lib().hy_act_bwd(ty, _act(act), _p(z), ldz, _p(dy), ldd, m, n, _p(dz), ldo, s))
+    _call(lib().hy_act_bwd, z, stream, (dy, dz), ty, _act(act), _p(z), ldz, _p(dy), ldd, m, n, _p(dz), ldo)
 
 
 def linear_dx(W, dz, dx, resid=None, stream=None):
@@ -126,8 +123,8 @@ def linear_dx(W, dz, dx, resid=None, stream=None):
     ldw, ldd = _mat("W", W, n, k), _mat("dz", dz, m, n, W.dtype)
     ldo = _mat("dx", dx, m, k, W.dtype, torch.float32)
     ldr = _mat("resid", resid, m, k, dx.dtype) if resid is not None else 0
-    with _On(W, stream, dz, dx, resid) as s:
-        check(lib().hy_linear_dx(ty, _p(W), ldw, n, k, _p(dz), ldd, m, _p(resid), ldr, _p(dx), _TYPE[dx.dtype], ldo, s))
+    _call(lib().hy_linear_dx, W, stream, (dz, dx, resid),
+          ty, _p(W), ldw, n, k, _p(dz), ldd, m, _p(resid), ldr, _p(dx), _TYPE[dx.dtype], ldo)
 
 
 def linear_dw_ws_bytes(m: int, n: int, k: int) -> int:
@@ -143,17 +140,16 @@ def linear_dw(dz, x, dW, db=None, accumulate=False, ws=None, stream=None):
     ldw = _mat("dW", dW, n, k, dz.dtype, torch.float32)
     _vec("db", db, n, torch.float32)
     _vec("ws", ws, 0, torch.uint8)
-    with _On(dW, stream, dz, x, db, ws) as s:
-        check(lib().hy_linear_dw(ty, _p(dz), ldd, _p(x), ldx, m, n, k, _p(dW), _TYPE[dW.dtype], ldw, _p(db), int(bool(accumulate)),
-                                 _p(ws), 0 if ws is None else ws.numel(), s))
+    _call(lib().hy_linear_dw, dW, stream, (dz, x, db, ws),
+          ty, _p(dz), ldd, _p(x), ldx, m, n, k, _p(dW), _TYPE[dW.dtype], ldw, _p(db), int(bool(accumulate)), _p(ws),
+          0 if ws is None else ws.numel())
 
 
 def rows16(x, out, stream=None):
     """float32 rows rounded to out's 16-bit type."""
     ty, (m, n) = _type16(out), out.shape
     xs, ldo = _mat("x", x, m, n, torch.float32), _mat("out", out, m, n)
-    with _On(out, stream, x) as s:
-        check(lib().hy_rows16(ty, _p(x), xs, n, m, _p(out), ldo, s))
+    _call(lib().hy_rows16, out, stream, (x,), ty, _p(x), xs, n, m, _p(out), ldo)
 
 
 # ------------------------------------------------------------------ experts
@@ -235,9 +231,8 @@ def moe16_gate_up(m: Moe16Dev, x, k, n_pairs, h, ids=None, order=None, order_n=N
         if t is not None:
             _pairs(name, t, n_pairs, m.ff, dt)
     _groups(n_pairs, ids, order, order_n, egrp, max_active)
-    with _On(m.slot, stream, x, h, ids, order, order_n, egrp, g, u) as s:
-        check(lib().hy_moe16_gate_up(m.ref, _p(x), ldx, k, _p(ids), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(g), _p(u),
-                                     _p(h), s))
+    _call(lib().hy_moe16_gate_up, m.slot, stream, (x, h, ids, order, order_n, egrp, g, u),
+          m.ref, _p(x), ldx, k, _p(ids), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(g), _p(u), _p(h))
 
 
 def moe16_down(m: Moe16Dev, h, n_pairs, y, wts=None, ids=None, order=None, order_n=None, egrp=None, max_active=0, stream=None):
@@ -249,9 +244,8 @@ def moe16_down(m: Moe16Dev, h, n_pairs, y, wts=None, ids=None, order=None, order
     _pairs("y", y, n_pairs, m.n, dt, torch.float32)
     _vec("wts", wts, n_pairs, torch.float32)
     _groups(n_pairs, ids, order, order_n, egrp, max_active)
-    with _On(m.slot, stream, h, y, wts, ids, order, order_n, egrp) as s:
-        check(lib().hy_moe16_down(m.ref, _p(h), _p(ids), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(wts), _p(y),
-                                  _TYPE[y.dtype], s))
+    _call(lib().hy_moe16_down, m.slot, stream, (h, y, wts, ids, order, order_n, egrp),
+          m.ref, _p(h), _p(ids), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(wts), _p(y), _TYPE[y.dtype])
 
 
 def moe16_down_dx(m: Moe16Dev, dy, k, n_pairs, order, order_n, egrp, max_active, dh, stream=None):
@@ -262,9 +256,8 @@ def moe16_down_dx(m: Moe16Dev, dy, k, n_pairs, order, order_n, egrp, max_active,
     ldd = _mat("dy", dy, (n_pairs + k - 1) // max(k, 1), m.n, dt, least=True)
     _pairs("dh", dh, n_pairs, m.ff, dt, torch.float32)
     _groups(n_pairs, None, order, order_n, egrp, max_active)
-    with _On(m.slot, stream, dy, dh, order, order_n, egrp) as s:
-        check(lib().hy_moe16_down_dx(m.ref, _p(dy), ldd, k, n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(dh),
-                                     _TYPE[dh.dtype], s))
+    _call(lib().hy_moe16_down_dx, m.slot, stream, (dy, dh, order, order_n, egrp),
+          m.ref, _p(dy), ldd, k, n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(dh), _TYPE[dh.dtype])
 
 
 def moe16_gate_up_dx(m: Moe16Dev, dg, du, n_pairs, order, order_n, egrp, max_active, dx, stream=None):
@@ -276,9 +269,8 @@ def moe16_gate_up_dx(m: Moe16Dev, dg, du, n_pairs, order, order_n, egrp, max_act
     _pairs("du", du, n_pairs, m.ff, dt)
     _pairs("dx", dx, n_pairs, m.n, dt, torch.float32)
     _groups(n_pairs, None, order, order_n, egrp, max_active)
-    with _On(m.slot, stream, dg, du, dx, order, order_n, egrp) as s:
-        check(lib().hy_moe16_gate_up_dx(m.ref, _p(dg), _p(du), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(dx),
-                                        _TYPE[dx.dtype], s))
+    _call(lib().hy_moe16_gate_up_dx, m.slot, stream, (dg, du, dx, order, order_n, egrp),
+          m.ref, _p(dg), _p(du), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(dx), _TYPE[dx.dtype])
 
 
 def moe16_dw(m: Moe16Dev, a, ka, b, kb, n_pairs, order, order_n, egrp, max_active, dW, accumulate=False, stream=None):
@@ -289,9 +281,9 @@ def moe16_dw(m: Moe16Dev, a, ka, b, kb, n_pairs, order, order_n, egrp, max_activ
     if tuple(dW.shape) != (m.n_local, rows, cols) or not dW.is_contiguous() or dW.dtype not in (a.dtype, torch.float32):
         raise ValueError(f"dW must be contiguous [{m.n_local}, {rows}, {cols}] of {a.dtype} or float32, got {dW.dtype} {tuple(dW.shape)}")
     _groups(n_pairs, None, order, order_n, egrp, max_active)
-    with _On(m.slot, stream, a, b, dW, order, order_n, egrp) as s:
-        check(lib().hy_moe16_dw(m.ref, ty, _p(a), lda, ka, rows, _p(b), ldb, kb, cols, n_pairs, _p(order), _p(order_n), _p(egrp),
-                                max_active, _p(dW), _TYPE[dW.dtype], int(bool(accumulate)), s))
+    _call(lib().hy_moe16_dw, m.slot, stream, (a, b, dW, order, order_n, egrp),
+          m.ref, ty, _p(a), lda, ka, rows, _p(b), ldb, kb, cols, n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(dW),
+          _TYPE[dW.dtype], int(bool(accumulate)))
 
 
 def swiglu_bwd(g, u, dh, wts, dg, du, hw=None, dwts=None, clamp=0.0, order=None, order_n=None, stream=None):
@@ -304,9 +296,8 @@ def swiglu_bwd(g, u, dh, wts, dg, du, hw=None, dwts=None, clamp=0.0, order=None,
     _vec("dwts", dwts, P, torch.float32)
     _vec("order", order, P, torch.int32)
     _vec("order_n", order_n, 1, torch.int32)
-    with _On(g, stream, u, dh, wts, dg, du, hw, dwts, order, order_n) as s:
-        check(lib().hy_swiglu_bwd(ty, _p(g), _p(u), _p(dh), _p(wts), P, ff, float(clamp), _p(order), _p(order_n), _p(dg), _p(du), _p(hw),
-                                  _p(dwts), s))
+    _call(lib().hy_swiglu_bwd, g, stream, (u, dh, wts, dg, du, hw, dwts, order, order_n),
+          ty, _p(g), _p(u), _p(dh), _p(wts), P, ff, float(clamp), _p(order), _p(order_n), _p(dg), _p(du), _p(hw), _p(dwts))
 
 
 # ------------------------------------------------------------------ one MoE layer

@@ -84,9 +84,9 @@ def within(got, want, err, what=""):
 
 
 def glu_err(want, u):
-    """evaluation of silu(g) u for exact g and u: a few 2^-24, and below g = -88.72, where exp(-g) leaves float32 and silu
-    is 0, the value itself: |g| exp(g) < 88.73 exp(-88.72) < 2.7e-37 there, times |u|"""
-    return 16 * 2.0 ** -24 * want.abs() + 2.7e-37 * u.abs()
+    """evaluation of silu(g) u for exact g and u: a few 2^-24, and below g = -87.33, where 1 / (1 + exp(-g)) leaves the normal
+    numbers and is 0, the value itself: |g| exp(g) < 87.34 exp(-87.33) < 1.04e-36 there, times |u|"""
+    return 16 * 2.0 ** -24 * want.abs() + 1.04e-36 * u.abs()
 
 
 # (rows, outputs, inputs): one row to many, sizes around the tiles, odd ones, rows that are and are not multiples of 16 bytes
