@@ -43,6 +43,7 @@ struct MMArgs {
     float *db;                        // TN: sums of Q's columns
     int act, out_f32, accumulate;
     float clamp;
+    int bias16;                       // the bias starts on 16 bytes
     int vec;                          // out, resid, z, g and u can be moved in 16-byte pieces
 };
 

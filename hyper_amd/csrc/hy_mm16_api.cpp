@@ -114,6 +114,7 @@ int hy_linear(int type, const void *W, int64_t ldw, int n, int k, const void *x,
     a.P = W; a.ldp = ldw; a.Q = x; a.ldq = ldx; a.R = m; a.N = n; a.K = k;
     a.bias = bias; a.act = act; a.resid = resid; a.ldr = ldr; a.z = z; a.ldz = ldz; a.out = out; a.ldo = ldo;
     a.out_f32 = out_type == HY_F32;
+    a.bias16 = !misaligned(bias, 16);
     a.vec = vec16(out, ldo, ob) && vec16(resid, ldr, ob) && vec16(z, ldz, 2);
     return m <= 4 ? launch_mv(type, false, a, s, what) : launch_mm(NT, type, false, a, s, what);
 }

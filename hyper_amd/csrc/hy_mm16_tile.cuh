@@ -308,6 +308,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) v
     static_assert(FIT >= 1 && FQ % JP == 0, "the epilogue's rows fit the stages");
     const uint32_t own = lds0 + (uint32_t) wave * JP * 16 * WN * 4;
     const int cl = c0 + wp * (CN / WP) + lane % LPR * 8;
+    const int64_t ob = KIND == TN ? (int64_t) blockIdx.y * a.ostride : 0;
 #pragma unroll
     for (int j0 = 0; j0 < FQ; j0 += JP) {
 #pragma unroll
@@ -318,34 +319,109 @@ __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) v
                 *(__attribute__((address_space(3))) f4 *) (uintptr_t) (own + (r + 16 * j) * (WN * 4) + (((uint32_t) (i * 4 + (lane >> 4)) ^ (r & X)) * 16)) = acc[i][j0 + j];
         }
         wave_sync();
-#pragma unroll 1
-        for (int h = 0; h < 16 * JP; h += RPI) {
-            const int r = RPI <= 16 ? h + lane / LPR : h + (lane / LPR) % (16 * JP);
+        auto row_of = [&](int r) -> int {   // the output row of the wave's row r of this pass (-1: none)
             const int i0 = wq * (BM / WQ) + j0 * 16 + r;
-            int row;
-            int64_t ob = 0;
-            float w = 1.0f;
-            if constexpr (KIND == TN) {
-                row = r0 + i0 < a.R ? r0 + i0 : -1;
-                ob = (int64_t) blockIdx.y * a.ostride;
-            } else {
-                row = s_pair[i0];
-                if (a.wts && row >= 0) w = a.wts[row];
+            if constexpr (KIND == TN) return r0 + i0 < a.R ? r0 + i0 : -1;
+            else return s_pair[i0];
+        };
+        auto piece = [&](int r, int c) { return lds_get<f4>(own + (uint32_t) r * (WN * 4) + (((uint32_t) c ^ ((uint32_t) r & X)) * 16)); };
+        const int pc = DUAL ? (lane % LPR >> 1) * 8 + (lane % LPR * 2 & 3) : lane % LPR * 2;   // the lane's first piece (gated: 16 gate, 16 up, ..)
+        if (a.vec && cl + 8 <= a.N) {
+            // U rows at a time, so that their reads and stores are in flight together
+            constexpr int NIT = 16 * JP / RPI > 0 ? 16 * JP / RPI : 1, U = NIT % 4 == 0 ? 4 : NIT % 2 == 0 ? 2 : 1;
+#pragma unroll 1
+            for (int h = 0; h < NIT * RPI; h += U * RPI) {
+                float v[U][8];
+                int row[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = (h + u * RPI + lane / LPR) % (16 * JP);
+                    row[u] = RPI > 16 * JP && lane / LPR >= 16 * JP ? -1 : row_of(r);
+                    const f4 p0 = piece(r, pc), p1 = piece(r, pc + 1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[u][e] = p0[e]; v[u][e + 4] = p1[e]; }
+                }
+                if constexpr (DUAL) {
+                    float w[U][8];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int r = (h + u * RPI + lane / LPR) % (16 * JP);
+                        const f4 p0 = piece(r, pc + 4), p1 = piece(r, pc + 5);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { w[u][e] = p0[e]; w[u][e + 4] = p1[e]; }
+                    }
+                    if (a.g) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (row[u] >= 0) {
+                                put_n<T, 8>(a.g, row[u] * a.ldo + cl, v[u], 8, false, true);
+                                put_n<T, 8>(a.u, row[u] * a.ldo + cl, w[u], 8, false, true);
+                            }
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[u][e] = mm_swiglu(v[u][e], w[u][e], a.clamp);
+                } else {
+                    if (a.bias) {
+                        const f4 *b = (const f4 *) (a.bias + cl);
+                        float bb[8];
+                        if (a.bias16) {
+                            const f4 b0 = b[0], b1 = b[1];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { bb[e] = b0[e]; bb[e + 4] = b1[e]; }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) bb[e] = a.bias[cl + e];
+                        }
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[u][e] += bb[e];
+                    }
+                    if (a.z) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) if (row[u] >= 0) put_n<T, 8>(a.z, row[u] * a.ldz + cl, v[u], 8, false, true);
+                    }
+                    switch (a.act) {
+                    case HY_ACT_RELU: act_n<HY_ACT_RELU, U * 8>(&v[0][0]); break;
+                    case HY_ACT_SILU: act_n<HY_ACT_SILU, U * 8>(&v[0][0]); break;
+                    case HY_ACT_GELU: act_n<HY_ACT_GELU, U * 8>(&v[0][0]); break;
+                    case HY_ACT_GELU_TANH: act_n<HY_ACT_GELU_TANH, U * 8>(&v[0][0]); break;
+                    }
+                    if (a.wts) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const float w = row[u] >= 0 ? a.wts[row[u]] : 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[u][e] *= w;
+                        }
+                    }
+                    if (a.resid) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) if (row[u] >= 0) add_n<T, 8>(a.resid, row[u] * a.ldr + cl, v[u], 8, a.out_f32, true);
+                    }
+                    if (a.accumulate) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) if (row[u] >= 0) add_n<T, 8>(a.out, ob + row[u] * a.ldo + cl, v[u], 8, a.out_f32, true);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) if (row[u] >= 0) put_n<T, 8>(a.out, ob + row[u] * a.ldo + cl, v[u], 8, a.out_f32, true);
             }
-            if (RPI > 16 * JP && lane / LPR >= 16 * JP) row = -1;   // lanes without a row
-            auto piece = [&](int c) { return lds_get<f4>(own + (uint32_t) r * (WN * 4) + (((uint32_t) c ^ ((uint32_t) r & X)) * 16)); };
-            union { f4 q[2]; float v[8]; } u, g2;
-            if constexpr (DUAL) {
-                const int c = lane % LPR * 2, at = (c >> 2) * 8 + (c & 3);   // 16 gate columns, 16 up columns, ..
-                u.q[0] = piece(at);
-                u.q[1] = piece(at + 1);
-                g2.q[0] = piece(at + 4);
-                g2.q[1] = piece(at + 5);
-                if (row >= 0) epi_glu<T, 8>(a, row, cl, u.v, g2.v);
-            } else {
-                u.q[0] = piece(lane % LPR * 2);
-                u.q[1] = piece(lane % LPR * 2 + 1);
-                if (row >= 0) epi_store<T, 8>(a, ob, row, cl, u.v, w);
+        } else if (cl < a.N) {   // the last columns, or matrices that cannot be moved in 16-byte pieces
+#pragma unroll 1
+            for (int h = 0; h < 16 * JP; h += RPI) {
+                const int r = (h + lane / LPR) % (16 * JP), row = RPI > 16 * JP && lane / LPR >= 16 * JP ? -1 : row_of(r);
+                if (row < 0) continue;
+                union { f4 q[2]; float v[8]; } u, g2;
+                u.q[0] = piece(r, pc);
+                u.q[1] = piece(r, pc + 1);
+                if constexpr (DUAL) {
+                    g2.q[0] = piece(r, pc + 4);
+                    g2.q[1] = piece(r, pc + 5);
+                    epi_glu<T, 8>(a, row, cl, u.v, g2.v);
+                } else epi_store<T, 8>(a, ob, row, cl, u.v, a.wts ? a.wts[row] : 1.0f);
             }
         }
         wave_sync();
