@@ -233,18 +233,11 @@ __device__ __forceinline__ Group load_group(const MMArgs &a, int i) {
 }
 __device__ __forceinline__ int n_groups(const MMArgs &a) { return max(0, min(a.order_n[1], a.max_active)); }
 
-// The group and row tile of this block (tiles of BM rows, groups in order), found by the whole block of NTH threads: every
-// thread counts the tiles of its few groups, a scan over the block places them.  place(items) says which of the `items`
-// tiles is this block's (below 0: none); the result is false then.  count(i, n): the items of group i with n row tiles, of which
-// `tile` becomes this block's; gi its group's number.
-template <int NTH, int BM, typename F, typename C>
-__device__ __forceinline__ bool find_item(const MMArgs &a, F place, C count, Group &g, int &tile, int &gi) {
-    if (!a.egrp) {
-        g = Group{0, 0, a.R};
-        gi = 0;
-        tile = place((int) (((uint32_t) a.R + BM - 1) / BM));
-        return tile >= 0;
-    }
+// The group of this block's work item, found by the whole block of NTH threads: count(i, rows) is the number of items of group i;
+// every thread counts those of its few groups and a scan over the block places them.  place(total) says which of the `total`
+// items is the block's (below 0: none; the result is false then); `item` becomes its number within the group, gi the group's.
+template <int NTH, typename C, typename F>
+__device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Group &g, int &item, int &gi) {
     constexpr int PER = 1024 / NTH;
     static_assert(PER * NTH == 1024, "at most 1024 groups");
     __shared__ int s_w[NTH / 64], s_out[5];
@@ -256,7 +249,7 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, F place, C count, Gro
         const int i = tid * PER + j;
         gs[j] = Group{-1, 0, 0};
         if (i < ng) gs[j] = load_group(a, i);
-        nt[j] = count(i, (int) (((uint32_t) gs[j].cnt + BM - 1) / BM));
+        nt[j] = count(i, gs[j].cnt);
         sum += nt[j];
     }
     int inc = sum;
@@ -276,7 +269,7 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, F place, C count, Gro
     }
     __syncthreads();
     g = Group{__builtin_amdgcn_readfirstlane(s_out[0]), __builtin_amdgcn_readfirstlane(s_out[1]), __builtin_amdgcn_readfirstlane(s_out[2])};
-    tile = __builtin_amdgcn_readfirstlane(s_out[3]);
+    item = __builtin_amdgcn_readfirstlane(s_out[3]);
     gi = __builtin_amdgcn_readfirstlane(s_out[4]);
     return true;
 }
@@ -301,31 +294,45 @@ __device__ __forceinline__ int pair_of(const MMArgs &a, const Group &g, int i) {
     return (uint32_t) p < (uint32_t) a.n_pairs ? p : -1;
 }
 
-// Tile number t of an items x ncol grid from the block number: blocks b, b + 8, .. run on one XCD, whose L2 they share, so
-// XCD x gets the tiles from x / 8 of the way on; there, bands of G row tiles go column by column, so that the blocks that
-// run together read few row and few column tiles.  Returns the row tile (-1: no tile) and sets col.
-template <int G> __device__ __forceinline__ int place_tile(uint32_t b, int items, int ncol, int &col) {
-    const uint32_t T = (uint32_t) items * (uint32_t) ncol;
+// Blocks b, b + 8, .. run on one XCD, whose L2 they share: XCD x gets the tiles from x / 8 of the T tiles on.  -1: no tile.
+__device__ __forceinline__ int xcd_tile(uint32_t b, uint32_t T) {
     if (b >= T) return -1;
-    const uint32_t q = T >> 3, r = T & 7, x = b & 7, t = x * q + min(x, r) + (b >> 3);
-    const uint32_t per = (uint32_t) G * ncol, band = t / per, in = t - band * per, rows = min((uint32_t) G, (uint32_t) items - band * G);
-    col = (int) (in / rows);
-    return (int) (band * G + in % rows);
+    const uint32_t q = T >> 3, r = T & 7, x = b & 7;
+    return (int) (x * q + min(x, r) + (b >> 3));
 }
-
-// Grouped, few rows a group: the time is the weights' bytes, of which every XCD should fetch as many, and a group's row tiles of
-// one column tile should share the L2 that holds it.  Column tile c of group i goes to XCD (i ncol + c) % 8; in a group an XCD
-// goes through bands of 8 row tiles column by column.  (Tiles dealt out in order instead gave the XCDs of large groups fewer
-// bytes: 128 experts, 512 tokens routed by Zipf(1.1): 179 us.)
+// tile t of rows x ncol tiles: bands of G row tiles go column by column, so that the blocks that run together read few row and
+// few column tiles
+template <int G> __device__ __forceinline__ void band_tile(int t, int rows, int ncol, int &tile, int &col) {
+    const int band = t / (G * ncol), in = t - band * G * ncol, n = min(G, rows - band * G);
+    col = in / n;
+    tile = band * G + in % n;
+}
+// The block's tile of BM rows.  Ungrouped: bands of 4.  Grouped: the groups in order, bands of 8 that do not reach into the next
+// group, whose weights are others.  (Groups' ends dealt out behind all whole tiles, to fill the last round, read the weights
+// once more: 64 experts of about 256 rows 160 against 149 us, 128 of about 256 rows 376 against 346.)
+// Grouped with few rows a group (spread): the time is the weights' bytes, of which every XCD should fetch as many.  Column tile c
+// of group i goes to XCD (i ncol + c) % 8 (tiles dealt out in order instead gave the XCDs of large groups fewer bytes: 288
+// experts, 1000 tokens routed by Zipf(1.1): 860 against 785 us).
 __device__ __forceinline__ int spread_first(int i, int ncol, int x) { return (x - i * ncol) & 7; }   // XCD x's first column of group i
 __device__ __forceinline__ int spread_cols(int i, int ncol, int x) { const int c = spread_first(i, ncol, x); return c < ncol ? (ncol - 1 - c) / 8 + 1 : 0; }
-template <int NTH, int BM> __device__ __forceinline__ bool find_spread(const MMArgs &a, int ncol, Group &g, int &tile, int &col) {
-    const int x = blockIdx.x & 7, it = blockIdx.x >> 3;
-    int gi, r;
-    if (!find_item<NTH, BM>(a, [&](int total) { return it < total ? it : -1; }, [&](int i, int n) { return n * spread_cols(i, ncol, x); }, g, r, gi)) return false;
-    const int n = spread_cols(gi, ncol, x), mt = (g.cnt + BM - 1) / BM, band = r / (8 * n), in = r - band * 8 * n, rows = min(8, mt - band * 8);
-    tile = band * 8 + in % rows;
-    col = spread_first(gi, ncol, x) + 8 * (in / rows);
+template <int NTH, int BM> __device__ __forceinline__ bool find_tile(const MMArgs &a, int ncol, bool spread, Group &g, int &tile, int &col) {
+    auto tiles = [](int rows) { return (int) (((uint32_t) rows + BM - 1) / BM); };
+    const int x = blockIdx.x & 7;
+    int gi, t;
+    if (!a.egrp) {
+        t = xcd_tile(blockIdx.x, (uint32_t) tiles(a.R) * (uint32_t) ncol);
+        if (t < 0) return false;
+        g = Group{0, 0, a.R};
+        band_tile<4>(t, tiles(a.R), ncol, tile, col);
+    } else if (spread) {
+        const int it = blockIdx.x >> 3;
+        if (!find_item<NTH>(a, [&](int i, int rows) { return tiles(rows) * spread_cols(i, ncol, x); }, [&](int n) { return it < n ? it : -1; }, g, t, gi)) return false;
+        band_tile<8>(t, tiles(g.cnt), spread_cols(gi, ncol, x), tile, col);
+        col = spread_first(gi, ncol, x) + 8 * col;
+    } else {
+        if (!find_item<NTH>(a, [&](int, int rows) { return tiles(rows) * ncol; }, [&](int n) { return xcd_tile(blockIdx.x, (uint32_t) n); }, g, t, gi)) return false;
+        band_tile<8>(t, tiles(g.cnt), ncol, tile, col);
+    }
     return true;
 }
 

@@ -16,13 +16,13 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
     constexpr int BN = DUAL ? 32 : 64;
     const int ncol = (a.N + BN - 1) / BN;
     Group g;
-    int tile, col, gi;
+    int tile, col;
     if constexpr (KIND == TN) {
         g = find_expert<256>(a, blockIdx.y);
         tile = blockIdx.x / ncol;
         col = blockIdx.x % ncol;
     } else {
-        if (!find_item<256, 64>(a, [&](int items) { return place_tile<4>(blockIdx.x, items, ncol, col); }, [](int, int n) { return n; }, g, tile, gi)) return;
+        if (!find_tile<256, 64>(a, ncol, false, g, tile, col)) return;
     }
     const int c0 = col * BN, r0 = tile * 64;
     const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);

@@ -76,39 +76,29 @@ template <bool TR, int S, int NW> struct Operand {
 __device__ __forceinline__ void mfma_acc(f4 &c, v8<bf16> a, v8<bf16> b) { asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void mfma_acc(f4 &c, v8<f16> a, v8<f16> b) { asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 
-// One BM x BN tile (output rows x columns) a block of WP x WQ waves, BN / WP columns by BM / WQ rows each; stages of 64
-// contraction values, NST of them in LDS, one barrier a stage.
+// One BM x BN tile (output rows x columns, from r0 and column tile col on) by a block of WP x WQ waves, BN / WP columns by
+// BM / WQ rows each; stages of 64 contraction values, NST of them in LDS, one barrier a stage.
 //
 // A stage is two halves of 32 values.  While one half's products run, the wave reads the next half's fragments into the other
 // registers and, behind the barrier, starts the DMAs of the stage NST on (whose place every wave has read by then): the reads
 // and DMAs go between the products one at a time, since a wave issues in order and two or three instructions hide behind a
 // product of 16 clocks.
+template <int KIND, int BM, int BN, int WP, int WQ, int NST> struct TileLds {   // bytes of the stages
+    static constexpr int STAGES = NST * (Operand<KIND != NT, BN, WP * WQ>::BYTES + Operand<KIND == TN, BM, WP * WQ>::BYTES);
+};
+constexpr int LOOK = 512;   // TN: contraction rows looked up at a time
 template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
-__global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) void k_mm(const MMArgs a) {
+__device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0, int col, uint8_t *s_mem, int *s_pair, int *s_look) {
     constexpr int NW = WP * WQ, NTH = 64 * NW, FP = BN / WP / 16, FQ = BM / WQ / 16;
     constexpr bool WIDE = FP * FQ == 64;   // 256 sums a lane: in the accumulation registers
     using OP = Operand<KIND != NT, BN, NW>;
     using OQ = Operand<KIND == TN, BM, NW>;
     constexpr int NDMA = OP::N + OQ::N, STAGE = OP::BYTES + OQ::BYTES;
     constexpr int WN = BN / WP;                                  // columns a wave
-    constexpr int CH = 512;                                      // TN: contraction rows looked up at a time
-    __shared__ __attribute__((aligned(1024))) uint8_t s_mem[NST * STAGE];
-    __shared__ int s_pair[KIND == TN ? 1 : BM], s_look[KIND == TN ? 4 * CH : 1];
+    constexpr int CH = LOOK;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, wp = wave % WP, wq = wave / WP;
     constexpr int CN = DUAL ? BN / 2 : BN;   // output columns a tile
-    const int ncol = (a.N + CN - 1) / CN;
-    Group g;
-    int tile, col = 0;
-    if constexpr (KIND == TN) {
-        tile = place_tile<4>(blockIdx.x, (a.R + BM - 1) / BM, ncol, col);
-        g = find_expert<NTH>(a, blockIdx.y);
-    } else {
-        int gi;
-        if (BM == 64 && a.spread) {
-            if (!find_spread<NTH, BM>(a, ncol, g, tile, col)) return;
-        } else if (!find_item<NTH, BM>(a, [&](int items) { return place_tile<4>(blockIdx.x, items, ncol, col); }, [](int, int n) { return n; }, g, tile, gi)) return;
-    }
-    const int c0 = col * CN, r0 = tile * BM;
+    const int c0 = col * CN;
     const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);
     const int64_t ldp2 = a.ldp * 2, ldq2 = a.ldq * 2;
     OP P;
@@ -440,6 +430,30 @@ __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) v
     }
 }
 
+// A block's tile.  Groups end inside a tile: where 128 (64) rows or fewer are left of a group's 256 (128), a smaller tile of the
+// same columns takes them.
+template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
+__global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) void k_mm(const MMArgs a) {
+    constexpr int NTH = 64 * WP * WQ, CN = DUAL ? BN / 2 : BN;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_mem[TileLds<KIND, BM, BN, WP, WQ, NST>::STAGES];
+    __shared__ int s_pair[KIND == TN ? 1 : BM], s_look[KIND == TN ? 4 * LOOK : 1];
+    const int ncol = (a.N + CN - 1) / CN;
+    Group g;
+    int tile, col = 0;
+    if constexpr (KIND == TN) {
+        const int rows = (a.R + BM - 1) / BM, t = xcd_tile(blockIdx.x, (uint32_t) rows * (uint32_t) ncol);
+        if (t < 0) return;
+        band_tile<4>(t, rows, ncol, tile, col);
+        g = find_expert<NTH>(a, blockIdx.y);
+    } else if (!find_tile<NTH, BM>(a, ncol, BM == 64 && a.spread, g, tile, col)) return;
+    const int r0 = tile * BM, left = g.cnt - r0;
+    if constexpr (KIND != TN && BM >= 128) {
+        if (a.egrp && left <= BM / 4) return mm_tile<T, KIND, DUAL, BM / 4, BN, BM == 256 ? 4 : 2, BM == 256 ? 1 : 2, 3>(a, g, r0, col, s_mem, s_pair, s_look);
+        if (a.egrp && left <= BM / 2) return mm_tile<T, KIND, DUAL, BM / 2, BN, 2, 2, 2>(a, g, r0, col, s_mem, s_pair, s_look);
+    }
+    mm_tile<T, KIND, DUAL, BM, BN, WP, WQ, NST>(a, g, r0, col, s_mem, s_pair, s_look);
+}
+
 template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
 static int launch_tile(MMArgs a, hipStream_t s, const char *what) {
     const int64_t ncol = (a.N + (DUAL ? BN / 2 : BN) - 1) / (DUAL ? BN / 2 : BN);
@@ -458,19 +472,20 @@ static int launch_tile(MMArgs a, hipStream_t s, const char *what) {
 // when few tiles run, when 256 run, when all of `slots` run, and of its start and epilogue.  Measured on bf16 forward products:
 // 4096^3 (as many rounds of full slots as tiles ask), 256 tiles and fewer of 2048 .. 4096 contraction values.
 struct TileCost { int bm, bn, slots; float few, t256, full, ends; };
-constexpr TileCost T256x256{256, 256, 256, 1.37f, 2.07f, 2.07f, 7.0f}, T128x128{128, 128, 512, 0.66f, 0.88f, 1.19f, 3.0f},
-    T64x128{64, 128, 512, 0.345f, 0.40f, 0.708f, 2.0f}, T64x64{64, 64, 512, 0.26f, 0.272f, 0.5f, 1.5f},
-    T32x128{32, 128, 512, 0.286f, 0.30f, 0.574f, 1.5f}, T32x64{32, 64, 512, 0.20f, 0.22f, 0.334f, 1.2f};
+constexpr TileCost T256x256{256, 256, 256, 1.37f, 2.07f, 2.07f, 11.0f}, T128x128{128, 128, 512, 0.66f, 0.88f, 1.19f, 5.0f},
+    T64x128{64, 128, 512, 0.345f, 0.40f, 0.708f, 3.2f}, T64x64{64, 64, 512, 0.26f, 0.272f, 0.5f, 2.5f},
+    T32x128{32, 128, 512, 0.286f, 0.30f, 0.574f, 2.2f}, T32x64{32, 64, 512, 0.20f, 0.22f, 0.334f, 2.0f};
 
-// rounds of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, half a tile over
-// in each group that has more than half a tile.
+// rounds of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, a tile begun in
+// each (half a tile over; a fifth where smaller tiles take the group's end, and then no group costs less than 0.4 of a tile).
 inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual) {
     const int cn = dual ? t.bn / 2 : t.bn;
     const double ncol = (a.N + cn - 1) / cn, groups = a.egrp ? std::max(1, std::min({a.max_active, a.n_expert, a.n_pairs})) : 1;
     double rows = kind == TN ? (double) ((a.R + t.bm - 1) / t.bm) * (a.egrp ? a.n_local : 1)
                   : !a.egrp  ? (double) (((int64_t) a.R + t.bm - 1) / t.bm)
-                             : groups * std::max(1.0, a.n_pairs / groups / t.bm + 0.5);
+                             : groups * (t.bm >= 128 ? std::max(0.4, a.n_pairs / groups / t.bm + 0.22) : std::max(1.0, a.n_pairs / groups / t.bm + 0.5));
     const double stages = kind == TN ? (a.egrp ? a.n_pairs / groups : a.K) / BK + 1 : (double) (a.K + BK - 1) / BK * (kind == NN && a.P2 ? 2 : 1);
+    if (kind != TN && a.egrp && t.bm >= 128 && a.n_pairs <= 40 * groups) return 1e30f;   // the weights' bytes bound these: 64 rows
     const double tiles = rows * ncol, whole = std::floor(tiles / t.slots), left = tiles - whole * t.slots;
     double part = 0;
     if (left >= 1) {

@@ -60,6 +60,10 @@ def _call(fn, ref: torch.Tensor, stream, others, *args) -> None:
 def _mat(name: str, t: torch.Tensor, rows: Optional[int], cols: int, *dtypes, least: bool = False) -> int:
     """checks a row-major matrix and returns the elements between its rows (least: it may have more rows)"""
     shape = t.shape
+    if shape == (rows, cols) and (not dtypes or t.dtype in dtypes):   # the usual case
+        between, step = t.stride()
+        if step == 1:
+            return between if rows > 1 else cols
     if len(shape) != 2 or shape[1] != cols or (rows is not None and (shape[0] < rows if least else shape[0] != rows)):
         raise ValueError(f"{name} must be [{'*' if rows is None else rows}, {cols}], got {tuple(shape)}")
     if dtypes and t.dtype not in dtypes:
@@ -76,9 +80,10 @@ def _vec(name: str, t: Optional[torch.Tensor], n: int, dtype) -> None:
 
 
 def _act(act: str) -> int:
-    if act not in ACTS:
+    v = ACTS.get(act)
+    if v is None:
         raise ValueError(f"unknown activation {act!r}")
-    return ACTS[act]
+    return v
 
 
 # ------------------------------------------------------------------ linear layers
@@ -86,14 +91,16 @@ def _act(act: str) -> int:
 def linear(W, x, out, bias=None, act="none", resid=None, z=None, stream=None):
     """out = act(x W^T + bias) + resid for x [m, k], W [n, k]; out (and resid) of the operands' type or float32, bias
     float32, z the pre-activation kept for act_bwd.  resid may be out itself."""
-    ty, (n, k), m = _type16(W), W.shape, x.shape[0]
-    ldw, ldx = _mat("W", W, n, k), _mat("x", x, m, k, W.dtype)
-    ldo = _mat("out", out, m, n, W.dtype, torch.float32)
+    dt, (n, k), m = W.dtype, W.shape, x.shape[0]
+    ldw, ldx = _mat("W", W, n, k), _mat("x", x, m, k, dt)
+    ldo = _mat("out", out, m, n, dt, torch.float32)
     ldr = _mat("resid", resid, m, n, out.dtype) if resid is not None else 0
-    ldz = _mat("z", z, m, n, W.dtype) if z is not None else 0
-    _vec("bias", bias, n, torch.float32)
+    ldz = _mat("z", z, m, n, dt) if z is not None else 0
+    if bias is not None:
+        _vec("bias", bias, n, torch.float32)
     _call(lib().hy_linear, W, stream, (x, out, bias, resid, z),
-          ty, _p(W), ldw, n, k, _p(x), ldx, m, _p(bias), _act(act), _p(resid), ldr, _p(z), ldz, _p(out), _TYPE[out.dtype], ldo)
+          _type16(W), W.data_ptr(), ldw, n, k, x.data_ptr(), ldx, m, _p(bias), _act(act), _p(resid), ldr, _p(z), ldz, out.data_ptr(),
+          _TYPE[out.dtype], ldo)
 
 
 def linear_glu(Wg, Wu, x, h, clamp=0.0, g=None, u=None, stream=None):
@@ -208,7 +215,8 @@ def experts_from_gguf(g, il: int, device="cuda", clamp: float = 0.0) -> Moe16Dev
 
 def _groups(n_pairs, ids, order, order_n, egrp, max_active):
     if order is None:
-        _vec("ids", ids, n_pairs, torch.int32)
+        if ids is not None:
+            _vec("ids", ids, n_pairs, torch.int32)
         return
     _vec("order", order, n_pairs, torch.int32)
     _vec("order_n", order_n, 2, torch.int32)
@@ -216,6 +224,8 @@ def _groups(n_pairs, ids, order, order_n, egrp, max_active):
 
 
 def _pairs(name, t, rows, cols, *dtypes):
+    if t.shape == (rows, cols) and t.dtype in dtypes and t.is_contiguous():   # the usual case
+        return
     if _mat(name, t, rows, cols, *dtypes, least=True) != cols:
         raise ValueError(f"{name} must be contiguous")
 
@@ -288,16 +298,22 @@ def moe16_dw(m: Moe16Dev, a, ka, b, kb, n_pairs, order, order_n, egrp, max_activ
 
 def swiglu_bwd(g, u, dh, wts, dg, du, hw=None, dwts=None, clamp=0.0, order=None, order_n=None, stream=None):
     """From g, u [P, ff] and the unweighted dh: dg, du, hw = wts h and dwts[p] = sum dh h (the pairs of order, or all)."""
-    ty, (P, ff) = _type16(g), g.shape
-    for name, t in (("g", g), ("u", u), ("dh", dh), ("dg", dg), ("du", du), ("hw", hw)):
-        if t is not None:
-            _pairs(name, t, P, ff, g.dtype)
+    shape, dt = g.shape, g.dtype
+    for t in (g, u, dh, dg, du, hw):
+        if t is not None and not (t.shape == shape and t.dtype is dt and t.is_contiguous()):
+            raise ValueError(f"g, u, dh, dg, du and hw must be contiguous matrices of one shape and type, got {t.dtype} {tuple(t.shape)} beside "
+                             f"{dt} {tuple(shape)}")
+    if len(shape) != 2:
+        raise ValueError(f"g must be [pairs, ff], got {tuple(shape)}")
+    P, ff = shape
     _vec("wts", wts, P, torch.float32)
     _vec("dwts", dwts, P, torch.float32)
-    _vec("order", order, P, torch.int32)
-    _vec("order_n", order_n, 1, torch.int32)
+    if order is not None or order_n is not None:
+        _vec("order", order, P, torch.int32)
+        _vec("order_n", order_n, 1, torch.int32)
     _call(lib().hy_swiglu_bwd, g, stream, (u, dh, wts, dg, du, hw, dwts, order, order_n),
-          ty, _p(g), _p(u), _p(dh), _p(wts), P, ff, float(clamp), _p(order), _p(order_n), _p(dg), _p(du), _p(hw), _p(dwts))
+          _type16(g), g.data_ptr(), u.data_ptr(), dh.data_ptr(), _p(wts), P, ff, clamp, _p(order), _p(order_n), dg.data_ptr(), du.data_ptr(),
+          _p(hw), _p(dwts))
 
 
 # ------------------------------------------------------------------ one MoE layer
