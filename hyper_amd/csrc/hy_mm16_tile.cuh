@@ -301,7 +301,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
     static_assert(FIT >= 1 && FQ % JP == 0, "the epilogue's rows fit the stages");
     const uint32_t own = lds0 + (uint32_t) wave * JP * 16 * WN * 4;
     const int cl = c0 + wp * (CN / WP) + lane % LPR * 8;
-    const int64_t ob = KIND == TN ? (int64_t) blockIdx.y * a.ostride : 0;
+    const int64_t ob = KIND == TN ? (int64_t) g.le * a.ostride : 0;
 #pragma unroll
     for (int j0 = 0; j0 < FQ; j0 += JP) {
 #pragma unroll

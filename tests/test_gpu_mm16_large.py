@@ -1,0 +1,169 @@
+"""16-bit matrix products of the sizes that take the large tiles, against 64-bit products on the device.
+
+All on small integers: every sum is an integer below 2^24 (at most 9 * 4100 here), exact in any order of fp32 sums, so a float32
+output equals the formula's bit for bit and a 16-bit output is its nearest value."""
+import pytest
+import torch
+
+from hyper_amd import mm16
+from tests.helpers import gen
+from tests.test_gpu_mm16 import TYPES, Layer, empty, glu_err, ints, marked, put, same, within
+
+pytestmark = pytest.mark.gpu
+
+
+def mul(cuda, a, b):
+    """a b^T in 64 bits"""
+    return (a.to(cuda) @ b.to(cuda).t().contiguous()).cpu()
+
+
+# rows and columns that fill many 256 x 256, 128 x 128 and 64 x 128 tiles, none of them whole at the edges; contractions of one
+# value, less than a stage of 64, whole stages, and a remainder
+DENSE = [(4000, 4000, 520), (3900, 4040, 321), (4000, 4104, 520), (4100, 4096, 64), (4090, 3976, 1), (2040, 2056, 264), (1032, 2184, 72), (700, 2056, 136), (257, 8200, 200),
+         (64, 8200, 328), (40, 8200, 72), (20, 4104, 1032)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", DENSE)
+def test_linear(cuda, dtype, m, n, k):
+    g = gen(m + n + k)
+    kk = (k + 7) // 8 * 8                                        # whole 16-byte rows, the columns behind k full of NaN
+    W, x, b, r = ints(g, n, k), ints(g, m, k), ints(g, 1, n), ints(g, m, n)
+    Wd, xd = put(W, dtype, cuda, kk - k), put(x, dtype, cuda, kk - k)
+    want = mul(cuda, x, W)
+    for out_t in (dtype, torch.float32):
+        y, clean = empty(m, n, out_t, cuda, 8)
+        z, zclean = empty(m, n, dtype, cuda)
+        mm16.linear(Wd, xd, y, bias=b[0].float().to(cuda), act="relu", resid=put(r, out_t, cuda, 16), z=z)
+        same(z, want + b, "z")
+        same(y, (want + b).clamp_min(0) + r, "y")
+        clean(), zclean()
+        y, clean = empty(m, n, out_t, cuda)
+        mm16.linear(Wd, xd, y)
+        same(y, want, "y alone")
+        clean()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(4000, 2000, 520), (4000, 2056, 264), (2040, 1032, 136), (700, 1032, 72), (100, 4104, 264)])
+def test_linear_glu(cuda, dtype, m, n, k):
+    g = gen(m + n + k)
+    Wg, Wu, x = ints(g, n, k, lo=-1, hi=1), ints(g, n, k), ints(g, m, k, lo=-1, hi=1)
+    G, U = mul(cuda, x, Wg), mul(cuda, x, Wu)
+    outs = [empty(m, n, dtype, cuda) for _ in range(3)]
+    mm16.linear_glu(put(Wg, dtype, cuda), put(Wu, dtype, cuda), put(x, dtype, cuda, 8), outs[2][0], g=outs[0][0], u=outs[1][0])
+    same(outs[0][0], G, "g")
+    same(outs[1][0], U, "u")
+    want = G * torch.sigmoid(G) * U
+    within(outs[2][0], want, glu_err(want, U), "h")
+    for _, clean in outs:
+        clean()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(520, 4000, 4000), (4000, 520, 3960), (520, 4000, 4104), (64, 4104, 4096), (1, 4096, 3976), (264, 2040, 2056), (4100, 520, 1032), (4000, 1288, 264),
+                                   (4104, 264, 4096), (40, 1032, 8200), (1100, 136, 2056)])
+def test_linear_gradients(cuda, dtype, m, n, k):
+    """m rows of dz [m, n] and x [m, k]: dx contracts over n, dW and db over m"""
+    g = gen(m + n + k)
+    W, dz, x = ints(g, n, k), ints(g, m, n), ints(g, m, k)
+    Wd, dzd, xd = put(W, dtype, cuda), put(dz, dtype, cuda, 8), put(x, dtype, cuda, 16)
+    for out_t in (dtype, torch.float32):
+        dx, clean = empty(m, k, out_t, cuda, 8)
+        mm16.linear_dx(Wd, dzd, dx)
+        same(dx, mul(cuda, dz, W.t()), "dx")
+        clean()
+        dW, clean = empty(n, k, out_t, cuda)
+        db = torch.zeros(n, device=cuda)
+        want = mul(cuda, dz.t(), x.t())
+        mm16.linear_dw(dzd, xd, dW, db=db)
+        same(dW, want, "dW")
+        same(db, dz.sum(0), "db")
+        dW.fill_(5.0)
+        db.fill_(-2.0)
+        mm16.linear_dw(dzd, xd, dW, db=db, accumulate=True)
+        same(dW, want + 5, "dW accumulated")
+        same(db, dz.sum(0) - 2, "db accumulated")
+        clean()
+
+
+class LargeLayer(Layer):
+    """the same layer with its formulas evaluated on the device"""
+
+    def __init__(self, cuda, *a, **kw):
+        super().__init__(cuda, *a, **kw)
+        self.cuda = cuda
+
+    def fwd(self, W, rows):
+        out = torch.zeros(self.P, W.shape[1], dtype=torch.float64)
+        for e in range(self.nl):
+            p = (self.local & (self.le == e)).nonzero().view(-1)
+            if len(p):
+                out[p] = mul(self.cuda, rows[p], W[e])
+        return out
+
+    def dw(self, a, b):
+        out = torch.zeros(self.nl, a.shape[1], b.shape[1], dtype=torch.float64)
+        for e in range(self.nl):
+            p = (self.local & (self.le == e)).nonzero().view(-1)
+            if len(p):
+                out[e] = mul(self.cuda, a[p].t(), b[p].t())
+        return out
+
+
+# tokens, d, E, k, ff, routing: some 300 rows a group (ends of every length), long and empty groups, about 100, 60 and 20 a group;
+# groups that end in whole tiles of 256 rows and in every part of one, about 750 a group;
+# one group of more than 1024 pairs among short ones, gradients of six column tiles
+GROUPED = [(3000, 2056, 8, 2, 1032, "even"), (2300, 2056, 8, 2, 1032, "skew"), (2400, 520, 16, 2, 2056, "even"), (2300, 264, 8, 2, 1032, "skew"), (1200, 1160, 24, 2, 776, "even"), (500, 1160, 64, 8, 520, "even"),
+           (640, 776, 64, 2, 1288, "even"), (1300, 1288, 64, 1, 520, "skew"), (700, 264, 130, 4, 264, "even")]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,d,E,k,ff,kind", GROUPED)
+@pytest.mark.parametrize("missing", [False, True])
+def test_expert_products(cuda, dtype, T, d, E, k, ff, kind, missing):
+    L = LargeLayer(cuda, dtype, T, d, E, k, ff, kind, missing)
+    loc = L.local
+    xp = L.x[L.tok]
+    G, U = L.fwd(L.gate, xp), L.fwd(L.up, xp)
+    h, g, u = (marked(cuda, dtype, L.P, ff) for _ in range(3))
+    mm16.moe16_gate_up(L.dev, put(L.x, dtype, cuda, 8), k, L.P, h, **L.kw, g=g, u=u)
+    same(g[loc.to(cuda)], G[loc], "g")
+    same(u[loc.to(cuda)], U[loc], "u")
+    want = G * torch.sigmoid(G) * U
+    within(h[loc.to(cuda)], want[loc], glu_err(want[loc], U[loc]), "h")
+    assert (h[~loc.to(cuda)] == 77.0).all()
+    hrows = ints(L.g, L.P, ff)
+    want = L.fwd(L.down, hrows)
+    for out_t, w in ((dtype, L.wts), (torch.float32, None)):
+        y = marked(cuda, out_t, L.P, d)
+        mm16.moe16_down(L.dev, hrows.to(dtype).to(cuda), L.P, y, wts=None if w is None else w.float().to(cuda), **L.kw)
+        same(y[loc.to(cuda)], (want if w is None else want * w[:, None])[loc], f"y {out_t}")
+        assert (y[~loc.to(cuda)] == 77.0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,d,E,k,ff,kind", GROUPED)
+@pytest.mark.parametrize("missing", [False, True])
+def test_expert_gradients(cuda, dtype, T, d, E, k, ff, kind, missing):
+    L = LargeLayer(cuda, dtype, T, d, E, k, ff, kind, missing, seed=1)
+    loc = L.local
+    dy, dg, du, hw = ints(L.g, T, d), ints(L.g, L.P, ff), ints(L.g, L.P, ff), ints(L.g, L.P, ff)
+    on = lambda t: t.to(dtype).to(cuda)  # noqa: E731
+    dyd, dgd, dud, hwd, xd = put(dy, dtype, cuda, 8), on(dg), on(du), on(hw), on(L.x)
+    dh = marked(cuda, dtype, L.P, ff)
+    mm16.moe16_down_dx(L.dev, dyd, k, L.P, *L.grp, dh)
+    same(dh[loc.to(cuda)], L.fwd(L.down.transpose(1, 2), dy[L.tok])[loc], "dh")
+    dx = marked(cuda, torch.float32, L.P, d)
+    mm16.moe16_gate_up_dx(L.dev, dgd, dud, L.P, *L.grp, dx)
+    same(dx[loc.to(cuda)], (L.fwd(L.gate.transpose(1, 2), dg) + L.fwd(L.up.transpose(1, 2), du))[loc], "dx")
+    assert (dh[~loc.to(cuda)] == 77.0).all() and (dx[~loc.to(cuda)] == 77.0).all()
+    for name, a, ka, A, b, kb, B in (("gate", dgd, 1, dg, xd, k, L.x[L.tok]), ("down", dyd, k, dy[L.tok], hwd, 1, hw)):
+        want = L.dw(A, B)
+        for out_t in (dtype, torch.float32):
+            dW = marked(cuda, out_t, L.nl, *want.shape[1:])
+            mm16.moe16_dw(L.dev, a, ka, b, kb, L.P, *L.grp, dW)
+            same(dW, want, f"dW {name} {out_t}")
+            dW.fill_(3.0)
+            mm16.moe16_dw(L.dev, a, ka, b, kb, L.P, *L.grp, dW, accumulate=True)
+            same(dW, want + 3, f"dW {name} accumulated {out_t}")
