@@ -41,6 +41,8 @@ struct MMArgs {
     void *z, *g, *u, *out;
     int64_t ldr, ldz, ldo, ostride;   // ostride (TN): elements between the experts' gradients
     float *db;                        // TN: sums of Q's columns
+    float *part;                      // TN, parts > 1: the sums of each part of the contraction (`parts` of part_len rows), then of db
+    int parts, part_len;
     int act, out_f32, accumulate;
     float clamp;
     int bias16;                       // the bias starts on 16 bytes
@@ -341,6 +343,8 @@ int launch_mm(int kind, int type, bool dual, const MMArgs &a, hipStream_t s, con
 int launch_tiles_nt(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
 int launch_tiles_nn(int type, const MMArgs &a, hipStream_t s, const char *what);
 int launch_tiles_tn(int type, const MMArgs &a, hipStream_t s, const char *what);
+struct Parts { int n, len; };
+Parts dw_parts(int m, int n, int k);   // how the contraction of an n x k gradient of m rows is cut
 int launch_mv(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
 int launch_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
                    hipStream_t s);

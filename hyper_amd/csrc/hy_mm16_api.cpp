@@ -166,7 +166,11 @@ int hy_linear_dx(int type, const void *W, int64_t ldw, int n, int k, const void 
     return launch_mm(NN, type, false, a, s, what);
 }
 
-size_t hy_linear_dw_ws_bytes(int m, int n, int k) { return 0; }
+size_t hy_linear_dw_ws_bytes(int m, int n, int k) {
+    if (m <= 0 || n <= 0 || k <= 0 || m > HY_MM_MAX || n > HY_MM_MAX || k > HY_MM_MAX) return 0;
+    const Parts p = dw_parts(m, n, k);
+    return p.n > 1 ? (size_t) p.n * ((size_t) n * k + n) * 4 : 0;
+}
 int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t ldx, int m, int n, int k, void *dW, int out_type,
                  int64_t lddw, float *db, int accumulate, void *ws, size_t ws_bytes, hipStream_t s) {
     const char *what = "hy_linear_dw";
@@ -184,6 +188,10 @@ int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t 
     a.P = x; a.ldp = ldx; a.Q = dz; a.ldq = lddz; a.R = n; a.N = k; a.K = m;
     a.out = dW; a.ldo = lddw; a.out_f32 = out_type == HY_F32; a.db = db; a.accumulate = accumulate != 0;
     a.vec = vec16(dW, lddw, ob);
+    if (need) {
+        const Parts p = dw_parts(m, n, k);
+        a.part = (float *) ws; a.parts = p.n; a.part_len = p.len;
+    }
     return launch_mm(TN, type, false, a, s, what);
 }
 

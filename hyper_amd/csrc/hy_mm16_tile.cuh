@@ -120,7 +120,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
             P.p[i] = M + c * ldp2 + OP::krow(wave, lane, i) * 2;
         } else {
             const int c = c0 + at < a.N ? c0 + at : c0;
-            P.p[i] = Pb + c * 2 + (KIND == TN && a.order ? 0 : OP::krow(wave, lane, i) * ldp2);
+            P.p[i] = Pb + c * 2 + (KIND == TN && a.order ? 0 : (OP::krow(wave, lane, i) + (KIND == TN ? g.start : 0)) * ldp2);
         }
     }
 #pragma unroll
@@ -128,7 +128,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
         const int at = OQ::at(wave, lane, i);
         if constexpr (KIND == TN) {
             const int r = r0 + at < a.R ? r0 + at : r0;
-            Q.p[i] = (const char *) a.Q + r * 2 + (a.order ? 0 : OQ::krow(wave, lane, i) * ldq2);
+            Q.p[i] = (const char *) a.Q + r * 2 + (a.order ? 0 : (OQ::krow(wave, lane, i) + g.start) * ldq2);
         } else {
             const int p = max(s_pair[at], 0);
             Q.p[i] = (const char *) a.Q + div_k(p, a.kq, mq) * ldq2 + OQ::krow(wave, lane, i) * 2;
@@ -424,7 +424,10 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
 #pragma unroll
             for (int j = 0; j < FQ; ++j) {
                 const int row = r0 + wq * (BM / WQ) + j * 16 + lane;
-                if (row < a.R) a.db[row] = a.accumulate ? a.db[row] + dbs[j][0] : dbs[j][0];
+                if (row < a.R) {
+                    float *d = a.db + (a.parts > 1 ? (int64_t) g.le * a.R : 0) + row;
+                    *d = a.accumulate ? *d + dbs[j][0] : dbs[j][0];
+                }
             }
         }
     }
@@ -444,7 +447,10 @@ __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) v
         const int rows = (a.R + BM - 1) / BM, t = xcd_tile(blockIdx.x, (uint32_t) rows * (uint32_t) ncol);
         if (t < 0) return;
         band_tile<4>(t, rows, ncol, tile, col);
-        g = find_expert<NTH>(a, blockIdx.y);
+        if (a.parts > 1) {
+            const int start = (int) blockIdx.y * a.part_len;
+            g = Group{(int) blockIdx.y, start, min(a.part_len, a.K - start)};
+        } else g = find_expert<NTH>(a, blockIdx.y);
     } else if (!find_tile<NTH, BM>(a, ncol, BM == 64 && a.spread, g, tile, col)) return;
     const int r0 = tile * BM, left = g.cnt - r0;
     if constexpr (KIND != TN && BM >= 128) {
@@ -462,7 +468,7 @@ static int launch_tile(MMArgs a, hipStream_t s, const char *what) {
     const int64_t blocks = a.spread ? (ncol + 7) / 8 * 8 * items : ncol * items;   // an XCD has at most ncol / 8, rounded up, of a group's columns
     if (blocks <= 0) return HY_OK;
     if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
-    k_mm<T, KIND, DUAL, BM, BN, WP, WQ, NST><<<dim3((uint32_t) blocks, KIND == TN && a.egrp ? (uint32_t) a.n_local : 1u), 64 * WP * WQ, 0, s>>>(a);
+    k_mm<T, KIND, DUAL, BM, BN, WP, WQ, NST><<<dim3((uint32_t) blocks, KIND == TN ? (uint32_t) (a.parts > 1 ? a.parts : a.egrp ? a.n_local : 1) : 1u), 64 * WP * WQ, 0, s>>>(a);
     return check_launch(what);
 }
 
@@ -478,7 +484,7 @@ constexpr TileCost T256x256{256, 256, 256, 1.37f, 2.07f, 2.07f, 11.0f}, T128x128
 
 // rounds of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, a tile begun in
 // each (half a tile over; a fifth where smaller tiles take the group's end, and then no group costs less than 0.4 of a tile).
-inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual) {
+inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual, int parts = 1) {
     const int cn = dual ? t.bn / 2 : t.bn;
     const double ncol = (a.N + cn - 1) / cn, groups = a.egrp ? std::max(1, std::min({a.max_active, a.n_expert, a.n_pairs})) : 1;
     double rows = kind == TN ? (double) ((a.R + t.bm - 1) / t.bm) * (a.egrp ? a.n_local : 1)
@@ -486,7 +492,7 @@ inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual) 
                              : groups * (t.bm >= 128 ? std::max(0.4, a.n_pairs / groups / t.bm + 0.22) : std::max(1.0, a.n_pairs / groups / t.bm + 0.5));
     const double stages = kind == TN ? (a.egrp ? a.n_pairs / groups : a.K) / BK + 1 : (double) (a.K + BK - 1) / BK * (kind == NN && a.P2 ? 2 : 1);
     if (kind != TN && a.egrp && t.bm >= 128 && a.n_pairs <= 40 * groups) return 1e30f;   // the weights' bytes bound these: 64 rows
-    const double tiles = rows * ncol, whole = std::floor(tiles / t.slots), left = tiles - whole * t.slots;
+    const double tiles = rows * ncol * parts, whole = std::floor(tiles / t.slots), left = tiles - whole * t.slots;
     double part = 0;
     if (left >= 1) {
         const double st = left <= 256 ? t.few + (t.t256 - t.few) * left / 256 : t.t256 + (t.full - t.t256) * (left - 256) / std::max(1, t.slots - 256);

@@ -3,6 +3,9 @@
 
 namespace hy {
 
+// 64 x 128: 4096 rows of 2048 x 2048 (512 tiles) 66 us, 8192 rows of 2048 x 1024 (256 tiles) 62 us
+constexpr TileCost TILES[] = {T256x256, T128x128, {64, 128, 512, 0.36f, 0.46f, 0.97f, 3.2f}};
+
 // Experts' gradients of few rows each (256 pairs: four stages a 256 x 256 tile): alone, a tile's start (group, pairs, first rows)
 // and end take longer than its products.  Here a block goes through up to `nct` column tiles of one expert and row tile: the
 // group and the pairs' rows are looked up once, the stages of the tiles follow one another without a break, and a tile's sums go
@@ -230,10 +233,63 @@ template <typename T> static int launch_gradients(const MMArgs &a, hipStream_t s
     return check_launch(what);
 }
 
+// Gradients with fewer tiles than the card has CUs: the contraction is cut into parts, each a launch's worth of 128 x 128 tiles,
+// whose fp32 sums are joined in order (no atomics: the same result every time).  Microseconds uncut / of 2, 4, 8, 16 parts (bf16):
+// 8192 rows of 1024 x 1024 58 / 50, 36, 36, 50; of 512 x 512 54 / 46, 31, 22, 22; of 4096 x 1024 117 / 84, 93, 117, 187; 4096 rows of
+// 2048 x 2048 66 / 52, 63, 90; 2048 rows of 1000 x 1032 19 / 23, 23, 27; 65536 rows of 64 x 2048 433 / 359, 192, 108, 69.
+Parts dw_parts(int m, int n, int k) {
+    constexpr TileCost cut{128, 128, 512, 0.66f, 0.75f, 0.95f, 5.0f};   // (a stage of parts reads less)
+    MMArgs a{};
+    a.R = n; a.N = k; a.K = m;
+    float least = tile_cost(TILES[cheapest(TILES, a, TN, false)], a, TN, false);
+    Parts best{1, m};
+    for (int p = 2; p <= 32; p *= 2) {
+        const int len = (m / p / BK + 1) * BK, parts = len > 0 ? (m + len - 1) / len : 1;
+        const double sums = (double) n * k * parts;
+        if (parts < 2 || len < 4 * BK || sums > 1 << 26) break;   // (256 MB)
+        MMArgs b = a;
+        b.K = len;
+        const float c = tile_cost(cut, b, TN, false, parts) + 5.0f + (float) (sums * 8 / 5e6);   // the join's launch, and its bytes at 5 MB / us
+        if (c < least) { least = c; best = Parts{parts, len}; }
+    }
+    return best;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void k_join(const MMArgs a) {
+    const int64_t sums = (int64_t) a.R * a.N, pieces = sums / 4, all = pieces + (a.db ? a.R : 0);   // (N: a multiple of 8)
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t) gridDim.x * 256) {
+        if (i < pieces) {
+            union { f4 q; float v[4]; } s;
+            s.q = f4{};
+            for (int p = 0; p < a.parts; ++p) s.q += *(const f4 *) (a.part + p * sums + i * 4);
+            const int64_t row = i * 4 / a.N, at = row * a.ldo + (i * 4 - row * a.N);
+            if (a.accumulate) add_n<T, 4>(a.out, at, s.v, 4, a.out_f32, a.vec);
+            put_n<T, 4>(a.out, at, s.v, 4, a.out_f32, a.vec);
+        } else {
+            const int64_t r = i - pieces;
+            const float *d = a.part + a.parts * sums + r;
+            float s = 0.0f;
+            for (int p = 0; p < a.parts; ++p) s += d[(int64_t) p * a.R];
+            a.db[r] = a.accumulate ? a.db[r] + s : s;
+        }
+    }
+}
+
+template <typename T> static int launch_parts(const MMArgs &a, hipStream_t s, const char *what) {
+    MMArgs b = a;
+    b.out = a.part; b.ldo = a.N; b.ostride = (int64_t) a.R * a.N; b.out_f32 = 1; b.accumulate = 0; b.vec = 1;
+    if (a.db) b.db = a.part + a.parts * b.ostride;
+    const int rc = launch_tile<T, TN, false, 128, 128, 2, 2, 2>(b, s, what);
+    if (rc != HY_OK) return rc;
+    const int64_t items = b.ostride / 4 + (a.db ? a.R : 0);
+    k_join<T><<<(uint32_t) std::min<int64_t>((items + 255) / 256, 256 * 16), 256, 0, s>>>(a);
+    return check_launch(what);
+}
+
 template <typename T> static int tiles(const MMArgs &a, hipStream_t s, const char *what) {
-    constexpr TileCost t[] = {T256x256, T128x128, T64x128};
+    if (a.parts > 1) return launch_parts<T>(a, s, what);
     if (gradients(a)) return launch_gradients<T>(a, s, what);
-    switch (cheapest(t, a, TN, false)) {
+    switch (cheapest(TILES, a, TN, false)) {
     case 0: return launch_tile<T, TN, false, 256, 256, 2, 2, 2>(a, s, what);
     case 1: return launch_tile<T, TN, false, 128, 128, 2, 2, 2>(a, s, what);
     }

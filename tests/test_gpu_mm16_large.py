@@ -62,7 +62,8 @@ def test_linear_glu(cuda, dtype, m, n, k):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(520, 4000, 4000), (4000, 520, 3960), (520, 4000, 4104), (64, 4104, 4096), (1, 4096, 3976), (264, 2040, 2056), (4100, 520, 1032), (4000, 1288, 264),
-                                   (4104, 264, 4096), (40, 1032, 8200), (1100, 136, 2056)])
+                                   (4104, 264, 4096), (40, 1032, 8200), (1100, 136, 2056),
+                                   (8200, 136, 264), (4099, 520, 520), (2048, 1000, 1032), (16400, 8, 8)])
 def test_linear_gradients(cuda, dtype, m, n, k):
     """m rows of dz [m, n] and x [m, k]: dx contracts over n, dW and db over m"""
     g = gen(m + n + k)
@@ -75,13 +76,14 @@ def test_linear_gradients(cuda, dtype, m, n, k):
         clean()
         dW, clean = empty(n, k, out_t, cuda)
         db = torch.zeros(n, device=cuda)
+        ws = torch.full((mm16.linear_dw_ws_bytes(m, n, k),), 255, dtype=torch.uint8, device=cuda)   # NaN in fp32
         want = mul(cuda, dz.t(), x.t())
-        mm16.linear_dw(dzd, xd, dW, db=db)
+        mm16.linear_dw(dzd, xd, dW, db=db, ws=ws)
         same(dW, want, "dW")
         same(db, dz.sum(0), "db")
         dW.fill_(5.0)
         db.fill_(-2.0)
-        mm16.linear_dw(dzd, xd, dW, db=db, accumulate=True)
+        mm16.linear_dw(dzd, xd, dW, db=db, accumulate=True, ws=ws)
         same(dW, want + 5, "dW accumulated")
         same(db, dz.sum(0) - 2, "db accumulated")
         clean()
