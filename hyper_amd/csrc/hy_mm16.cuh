@@ -346,6 +346,8 @@ int launch_tiles_tn(int type, const MMArgs &a, hipStream_t s, const char *what);
 struct Parts { int n, len; };
 Parts dw_parts(int m, int n, int k);   // how the contraction of an n x k gradient of m rows is cut
 int launch_mv(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
+bool few_rows(const MMArgs &a);   // a plain product that launch_few takes
+int launch_few(int type, const MMArgs &a, hipStream_t s, const char *what);
 int launch_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, int64_t lddy, int m, int n, void *dz, int64_t lddz,
                    hipStream_t s);
 int launch_swiglu_bwd(int type, const void *g, const void *u, const void *dh, const float *wts, int n_pairs, int ff, float clamp,

@@ -116,7 +116,7 @@ int hy_linear(int type, const void *W, int64_t ldw, int n, int k, const void *x,
     a.out_f32 = out_type == HY_F32;
     a.bias16 = !misaligned(bias, 16);
     a.vec = vec16(out, ldo, ob) && vec16(resid, ldr, ob) && vec16(z, ldz, 2);
-    return m <= 4 ? launch_mv(type, false, a, s, what) : launch_mm(NT, type, false, a, s, what);
+    return few_rows(a) ? launch_few(type, a, s, what) : m <= 4 ? launch_mv(type, false, a, s, what) : launch_mm(NT, type, false, a, s, what);
 }
 
 int hy_linear_glu(int type, const void *Wg, const void *Wu, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, float clamp,

@@ -107,6 +107,64 @@ int launch_mv(int type, bool dual, const MMArgs &a, hipStream_t s, const char *w
     return type == HY_BF16 ? launch_mv_t<bf16>(dual, a, s, what) : launch_mv_t<f16>(dual, a, s, what);
 }
 
+// ------------------------------------------------------------------ a few rows
+
+static __device__ __attribute__((aligned(16))) const uint32_t g_zeros[4] = {0, 0, 0, 0};
+
+// x W^T of up to 16 rows: a block of eight waves for 16 columns, the waves taking 64 of every 512 values of the contraction, straight
+// to the registers of 16 x 16 x 32 products, four steps ahead; their sums meet in LDS.  Bound by the weights' bytes and, with them,
+// each block's reads of x from L2 (5 rows of 4096 x 4096: 9.5 us, 3.5 TB/s of weights; 16 rows: 11.2 us).
+template <typename T> __global__ __launch_bounds__(512) void k_few(const MMArgs a) {
+    constexpr int DEPTH = 4;
+    __shared__ f4 s_sum[8][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), c0 = (int) blockIdx.x * 16;
+    const int kl = wave * 64 + (lane >> 4) * 8;   // the lane's first value of a step's first half
+    // (columns and rows outside are never stored)
+    const T *w = (const T *) a.P + min(c0 + (lane & 15), a.N - 1) * a.ldp + kl, *x = (const T *) a.Q + min(lane & 15, a.R - 1) * a.ldq + kl;
+    f4 acc = {};
+    v8<T> fw[DEPTH][2], fx[DEPTH][2];
+    auto load = [&](int d, int k) {   // k: the step's first value (a multiple of 512)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool in = k + kl + h * 32 < a.K;   // (K is a multiple of 8, and at most 2^30)
+            fw[d][h] = *(const v8<T> *) (in ? w + k + h * 32 : (const T *) g_zeros);
+            fx[d][h] = *(const v8<T> *) (in ? x + k + h * 32 : (const T *) g_zeros);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(d, d * 512);
+    for (int k = 0; k < a.K; k += 512 * DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc = mfma16(fw[d][h], fx[d][h], acc);
+            load(d, k + (DEPTH + d) * 512);
+        }
+    }
+    s_sum[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    float v[4] = {};
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += s_sum[u][lane][e];
+    if ((lane & 15) < a.R) epi_store<T, 4>(a, 0, lane & 15, c0 + (lane >> 4) * 4, v, 1.0f);
+}
+
+// One block a CU.  Microseconds, k_mv or tiles against k_few: 2 rows of 4096 x 14336 29.2 / 30.4, of 7168 x 4096 14.7 / 16.9; 4 rows of
+// 4096 x 4096 12.2 / 9.5; 16 rows of 1024 x 2048, 4096 x 4096, 4096 x 14336 8.4 / 6.3, 14.5 / 11.2, 50 / 37, of 7168 x 4096 (448 blocks)
+// 19.9 / 21.6.  32 rows (two row fragments) 15.8 / 15.7; gated (two fragments of columns, half the blocks) 14.7 / 15.4.
+bool few_rows(const MMArgs &a) {
+    return a.R >= 3 && a.R <= 16 && a.N <= 16 * 256 && a.K % 8 == 0 && a.ldp % 8 == 0 && a.ldq % 8 == 0 && (((uintptr_t) a.P | (uintptr_t) a.Q) & 15) == 0;
+}
+int launch_few(int type, const MMArgs &a, hipStream_t s, const char *what) {
+    const uint32_t grid = (uint32_t) ((a.N + 15) / 16);
+    if (type == HY_BF16) k_few<bf16><<<grid, 512, 0, s>>>(a);
+    else k_few<f16><<<grid, 512, 0, s>>>(a);
+    return check_launch(what);
+}
+
 // ------------------------------------------------------------------ elementwise
 
 // dz = dy act'(z): eight values a thread where rows allow it (V = 8), else one

@@ -17,10 +17,11 @@ def mul(cuda, a, b):
     return (a.to(cuda) @ b.to(cuda).t().contiguous()).cpu()
 
 
+# (and few rows: blocks of 16 columns)
 # rows and columns that fill many 256 x 256, 128 x 128 and 64 x 128 tiles, none of them whole at the edges; contractions of one
 # value, less than a stage of 64, whole stages, and a remainder
 DENSE = [(4000, 4000, 520), (3900, 4040, 321), (4000, 4104, 520), (4100, 4096, 64), (4090, 3976, 1), (2040, 2056, 264), (1032, 2184, 72), (700, 2056, 136), (257, 8200, 200),
-         (64, 8200, 328), (40, 8200, 72), (20, 4104, 1032)]
+         (64, 8200, 328), (16, 4096, 4096), (3, 4088, 2056), (9, 24, 8200), (40, 8200, 72), (20, 4104, 1032)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
