@@ -46,7 +46,8 @@ struct MMArgs {
     int act, out_f32, accumulate;
     float clamp;
     int bias16;                       // the bias starts on 16 bytes
-    int spread;                       // grouped: find_spread's order of tiles
+    int spread;                       // grouped: find_tile's order of tiles
+    int split;                        // ungrouped 256 x 256: parts of the last round's tiles (1, 2 or 4)
     int vec;                          // out, resid, z, g and u can be moved in 16-byte pieces
 };
 
@@ -302,6 +303,17 @@ __device__ __forceinline__ int xcd_tile(uint32_t b, uint32_t T) {
     const uint32_t q = T >> 3, r = T & 7, x = b & 7;
     return (int) (x * q + min(x, r) + (b >> 3));
 }
+// The same where a block is alone on its CU and the tiles of an XCD's last, partial round (of 32) are shared out to S blocks each.
+__device__ __forceinline__ int split_tile(uint32_t b, uint32_t T, int S, int &part) {
+    const uint32_t q = T >> 3, r = T & 7, x = b & 7, n = q + (x < r), whole = n & ~31u, i = b >> 3;
+    const uint32_t at = i < whole ? i : whole + (i - whole) / S;
+    part = i < whole ? -1 : (int) ((i - whole) % S);
+    return at < n ? (int) (x * q + min(x, r) + at) : -1;
+}
+inline __host__ int split_parts(int64_t T) {   // what S may be: the parts fit the round on every XCD
+    const int q = (int) (T >> 3) & 31, most = T & 7 ? (q == 31 ? 31 : q + 1) : q;
+    return most == 0 || most > 16 ? 1 : most > 8 ? 2 : 4;
+}
 // tile t of rows x ncol tiles: bands of G row tiles go column by column, so that the blocks that run together read few row and
 // few column tiles
 template <int G> __device__ __forceinline__ void band_tile(int t, int rows, int ncol, int &tile, int &col) {
@@ -317,12 +329,15 @@ template <int G> __device__ __forceinline__ void band_tile(int t, int rows, int 
 // experts, 1000 tokens routed by Zipf(1.1): 860 against 785 us).
 __device__ __forceinline__ int spread_first(int i, int ncol, int x) { return (x - i * ncol) & 7; }   // XCD x's first column of group i
 __device__ __forceinline__ int spread_cols(int i, int ncol, int x) { const int c = spread_first(i, ncol, x); return c < ncol ? (ncol - 1 - c) / 8 + 1 : 0; }
-template <int NTH, int BM> __device__ __forceinline__ bool find_tile(const MMArgs &a, int ncol, bool spread, Group &g, int &tile, int &col) {
+template <int NTH, int BM> __device__ __forceinline__ bool find_tile(const MMArgs &a, int ncol, bool spread, Group &g, int &tile, int &col, int &part) {
     auto tiles = [](int rows) { return (int) (((uint32_t) rows + BM - 1) / BM); };
     const int x = blockIdx.x & 7;
     int gi, t;
+    part = -1;
     if (!a.egrp) {
-        t = xcd_tile(blockIdx.x, (uint32_t) tiles(a.R) * (uint32_t) ncol);
+        const uint32_t T = (uint32_t) tiles(a.R) * (uint32_t) ncol;
+        if (BM == 256 && a.split > 1) t = split_tile(blockIdx.x, T, a.split, part);
+        else t = xcd_tile(blockIdx.x, T);
         if (t < 0) return false;
         g = Group{0, 0, a.R};
         band_tile<4>(t, tiles(a.R), ncol, tile, col);

@@ -22,7 +22,8 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
         tile = blockIdx.x / ncol;
         col = blockIdx.x % ncol;
     } else {
-        if (!find_tile<256, 64>(a, ncol, false, g, tile, col)) return;
+        int part;
+        if (!find_tile<256, 64>(a, ncol, false, g, tile, col, part)) return;
     }
     const int c0 = col * BN, r0 = tile * 64;
     const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);

@@ -20,7 +20,7 @@ def mul(cuda, a, b):
 # (and few rows: blocks of 16 columns)
 # rows and columns that fill many 256 x 256, 128 x 128 and 64 x 128 tiles, none of them whole at the edges; contractions of one
 # value, less than a stage of 64, whole stages, and a remainder
-DENSE = [(4000, 4000, 520), (3900, 4040, 321), (4000, 4104, 520), (4100, 4096, 64), (4090, 3976, 1), (2040, 2056, 264), (1032, 2184, 72), (700, 2056, 136), (257, 8200, 200),
+DENSE = [(4000, 4000, 520), (4600, 4600, 328), (3900, 4040, 321), (4000, 4104, 520), (4100, 4096, 64), (4090, 3976, 1), (2040, 2056, 264), (1032, 2184, 72), (700, 2056, 136), (257, 8200, 200),
          (64, 8200, 328), (16, 4096, 4096), (3, 4088, 2056), (9, 24, 8200), (40, 8200, 72), (20, 4104, 1032)]
 
 
@@ -46,7 +46,7 @@ def test_linear(cuda, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,n,k", [(4000, 2000, 520), (4000, 2056, 264), (2040, 1032, 136), (700, 1032, 72), (100, 4104, 264)])
+@pytest.mark.parametrize("m,n,k", [(4000, 2000, 520), (4600, 2304, 328), (4000, 2056, 264), (2040, 1032, 136), (700, 1032, 72), (100, 4104, 264)])
 def test_linear_glu(cuda, dtype, m, n, k):
     g = gen(m + n + k)
     Wg, Wu, x = ints(g, n, k, lo=-1, hi=1), ints(g, n, k), ints(g, m, k, lo=-1, hi=1)
