@@ -47,7 +47,7 @@ struct MMArgs {
     float clamp;
     int bias16;                       // the bias starts on 16 bytes
     int spread;                       // grouped: find_tile's order of tiles
-    int split;                        // ungrouped 256 x 256: parts of the last round's tiles (1, 2 or 4)
+    int split;                        // ungrouped 256 x 256: parts of the tiles that are left for the last turn (1, 2 or 4)
     int vec;                          // out, resid, z, g and u can be moved in 16-byte pieces
 };
 
@@ -303,14 +303,14 @@ __device__ __forceinline__ int xcd_tile(uint32_t b, uint32_t T) {
     const uint32_t q = T >> 3, r = T & 7, x = b & 7;
     return (int) (x * q + min(x, r) + (b >> 3));
 }
-// The same where a block is alone on its CU and the tiles of an XCD's last, partial round (of 32) are shared out to S blocks each.
+// The same where a block is alone on its CU and the tiles of an XCD's last, partial turn (of 32) are shared out to S blocks each.
 __device__ __forceinline__ int split_tile(uint32_t b, uint32_t T, int S, int &part) {
     const uint32_t q = T >> 3, r = T & 7, x = b & 7, n = q + (x < r), whole = n & ~31u, i = b >> 3;
     const uint32_t at = i < whole ? i : whole + (i - whole) / S;
     part = i < whole ? -1 : (int) ((i - whole) % S);
     return at < n ? (int) (x * q + min(x, r) + at) : -1;
 }
-inline __host__ int split_parts(int64_t T) {   // what S may be: the parts fit the round on every XCD
+inline __host__ int split_parts(int64_t T) {   // what S may be: the parts fit the turn on every XCD
     const int q = (int) (T >> 3) & 31, most = T & 7 ? (q == 31 ? 31 : q + 1) : q;
     return most == 0 || most > 16 ? 1 : most > 8 ? 2 : 4;
 }
@@ -322,7 +322,7 @@ template <int G> __device__ __forceinline__ void band_tile(int t, int rows, int 
     tile = band * G + in % n;
 }
 // The block's tile of BM rows.  Ungrouped: bands of 4.  Grouped: the groups in order, bands of 8 that do not reach into the next
-// group, whose weights are others.  (Groups' ends dealt out behind all whole tiles, to fill the last round, read the weights
+// group, whose weights are others.  (Groups' ends dealt out behind all whole tiles, to fill the last turn, read the weights
 // once more: 64 experts of about 256 rows 160 against 149 us, 128 of about 256 rows 376 against 346.)
 // Grouped with few rows a group (spread): the time is the weights' bytes, of which every XCD should fetch as many.  Column tile c
 // of group i goes to XCD (i ncol + c) % 8 (tiles dealt out in order instead gave the XCDs of large groups fewer bytes: 288

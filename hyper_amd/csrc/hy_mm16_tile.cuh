@@ -434,7 +434,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
 }
 
 // A block's tile.  Groups (and matrices) end inside a tile: where half or a quarter of its rows are left, a smaller tile of the same
-// columns takes them; so it does where the last round's tiles are shared out (8192 x 4608 outputs of 4096 values, 576 tiles on 256
+// columns takes them; so it does where the tiles left for the CUs' last turn are shared out (8192 x 4608 outputs of 4096 values, 576 tiles on 256
 // CUs: 264 -> 236 us; 4100 x 4096: 155 -> 141).
 template <typename T, int KIND, bool DUAL, int BM, int BN, int WP, int WQ, int NST>
 __global__ __launch_bounds__(64 * WP * WQ, BM * BN / (WP * WQ) > 8192 ? 1 : 2) void k_mm(const MMArgs a) {
@@ -484,13 +484,13 @@ static int launch_tile(MMArgs a, hipStream_t s, const char *what) {
 
 // A tile's rows, columns, tiles that run at once (256 CUs times those that fit a CU), and its cost in microseconds: of one stage
 // when few tiles run, when 256 run, when all of `slots` run, and of its start and epilogue.  Measured on bf16 forward products:
-// 4096^3 (as many rounds of full slots as tiles ask), 256 tiles and fewer of 2048 .. 4096 contraction values.
+// 4096^3 (as many turns of full slots as tiles ask), 256 tiles and fewer of 2048 .. 4096 contraction values.
 struct TileCost { int bm, bn, slots; float few, t256, full, ends; };
 constexpr TileCost T256x256{256, 256, 256, 1.37f, 2.07f, 2.07f, 11.0f}, T128x128{128, 128, 512, 0.66f, 0.88f, 1.19f, 5.0f},
     T64x128{64, 128, 512, 0.345f, 0.40f, 0.708f, 3.2f}, T64x64{64, 64, 512, 0.26f, 0.272f, 0.5f, 2.5f},
     T32x128{32, 128, 512, 0.286f, 0.30f, 0.574f, 2.2f}, T32x64{32, 64, 512, 0.20f, 0.22f, 0.334f, 2.0f};
 
-// rounds of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, a tile begun in
+// turns of full slots, then what is left.  Grouped rows are a guess: the pairs spread evenly over the groups, a tile begun in
 // each (half a tile over; a fifth where smaller tiles take the group's end, and then no group costs less than 0.4 of a tile).
 inline float tile_cost(const TileCost &t, const MMArgs &a, int kind, bool dual, int parts = 1) {
     const int cn = dual ? t.bn / 2 : t.bn;

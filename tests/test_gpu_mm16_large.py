@@ -170,3 +170,75 @@ def test_expert_gradients(cuda, dtype, T, d, E, k, ff, kind, missing):
             dW.fill_(3.0)
             mm16.moe16_dw(L.dev, a, ka, b, kb, L.P, *L.grp, dW, accumulate=True)
             same(dW, want + 3, f"dW {name} accumulated {out_t}")
+
+
+def test_gradients_captured_and_repeated(cuda):
+    """experts' gradients and a cut contraction in one captured graph on a stream of its own, replayed on new inputs between eager
+    calls: every result is the formula's, the workspace's surroundings stay, and two runs are equal bit for bit"""
+    T, d, E, k, ff, m, n = 700, 264, 130, 4, 264, 8200, 136
+    L = LargeLayer(cuda, torch.bfloat16, T, d, E, k, ff)
+    need = mm16.linear_dw_ws_bytes(m, n, d)
+    assert need > 0
+    guard = torch.full((need + 64,), 77, dtype=torch.uint8, device=cuda)
+    ws = guard[:need]
+    dg, x = torch.empty(L.P, ff, dtype=torch.bfloat16, device=cuda), torch.empty(T, d, dtype=torch.bfloat16, device=cuda)
+    dz, xs = torch.empty(m, n, dtype=torch.bfloat16, device=cuda), torch.empty(m, d, dtype=torch.bfloat16, device=cuda)
+    dW, dE = torch.empty(n, d, device=cuda), torch.empty(L.nl, ff, d, device=cuda)
+    db = torch.empty(n, device=cuda)
+
+    def step(stream=None):
+        mm16.moe16_dw(L.dev, dg, 1, x, k, L.P, *L.grp, dE, stream=stream)
+        mm16.linear_dw(dz, xs, dW, db=db, ws=ws, stream=stream)
+
+    def fill(seed):
+        g = gen(seed)
+        vals = ints(g, L.P, ff), ints(g, T, d), ints(g, m, n), ints(g, m, d)
+        for t, v in zip((dg, x, dz, xs), vals):
+            t.copy_(v)
+        return L.dw(vals[0], vals[1][L.tok]), mul(cuda, vals[2].t(), vals[3].t()), vals[2].sum(0)
+
+    def check(want):
+        for t, w in zip((dE, dW, db), want):
+            same(t, w)
+            t.fill_(77.0)
+        assert (guard[need:] == 77).all()
+
+    want = fill(1)
+    step()
+    first = dE.clone(), dW.clone()
+    check(want)
+    step()
+    assert torch.equal(first[0], dE) and torch.equal(first[1], dW)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(side)
+    for seed in (2, 3, 4):
+        want = fill(seed)
+        torch.cuda.synchronize(cuda)
+        graph.replay()
+        torch.cuda.synchronize(cuda)
+        check(want)
+        step()                                                   # eager, on the current stream, between the replays
+        torch.cuda.synchronize(cuda)
+        check(want)
+
+
+@pytest.mark.parametrize("out_t", [torch.bfloat16, torch.float32])
+def test_gradients_bad_tables(cuda, out_t):
+    """pairs that are none and groups outside the pairs add nothing; every gradient is still written"""
+    L = LargeLayer(cuda, torch.bfloat16, 700, 264, 130, 4, 264, seed=2)
+    a, b = ints(L.g, L.P, L.ff), ints(L.g, L.P, L.d)
+    order, egrp = L.order.cpu(), L.egrp.cpu()
+    order_bad, egrp_bad = order.clone(), egrp.clone()
+    order_bad[0], order_bad[5], order_bad[6] = -1, L.P, 1 << 30
+    gone = {int(order[i]) for i in (0, 5, 6)}
+    e2, start2, cnt2 = (int(v) for v in egrp[6:9])
+    egrp_bad[8] = 1 << 30                                        # the third group: too long
+    gone |= {int(p) for p in order[start2:start2 + cnt2]}
+    keep = torch.ones(L.P, 1, dtype=torch.float64)
+    keep[list(gone)] = 0
+    dW = marked(cuda, out_t, L.nl, L.ff, L.d)
+    mm16.moe16_dw(L.dev, a.bfloat16().to(cuda), 1, b.bfloat16().to(cuda), 1, L.P, order_bad.to(cuda), L.order_n, egrp_bad.to(cuda), L.ma, dW)
+    same(dW, L.dw(a * keep, b))
