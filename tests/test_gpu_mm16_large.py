@@ -242,3 +242,62 @@ def test_gradients_bad_tables(cuda, out_t):
     dW = marked(cuda, out_t, L.nl, L.ff, L.d)
     mm16.moe16_dw(L.dev, a.bfloat16().to(cuda), 1, b.bfloat16().to(cuda), 1, L.P, order_bad.to(cuda), L.order_n, egrp_bad.to(cuda), L.ma, dW)
     same(dW, L.dw(a * keep, b))
+
+
+@pytest.mark.parametrize("pad,offset", [(3, 1), (8, 4), (1, 0)])
+def test_outputs_of_any_alignment(cuda, pad, offset):
+    """operands on 16 bytes, outputs and what is added to them anywhere: every kernel's last step one element at a time"""
+    dtype = torch.bfloat16
+    for m, n, k in ((1, 136, 264), (9, 136, 264), (40, 264, 136), (264, 520, 136), (1032, 2184, 72), (4000, 4000, 520), (8200, 136, 264)):
+        g = gen(m + n + k + pad)
+        W, x, dz, r = ints(g, n, k), ints(g, m, k), ints(g, m, n), ints(g, m, n)
+        Wd, xd, dzd = (put(t, dtype, cuda) for t in (W, x, dz))
+        b = ints(g, 1, n)[0]
+        bd = torch.empty(n + 1, device=cuda)[1:]
+        bd.copy_(b)
+        want = mul(cuda, x, W) + b
+        for out_t in (dtype, torch.float32):
+            y, clean = empty(m, n, out_t, cuda, pad, offset)
+            z, zclean = empty(m, n, dtype, cuda, pad, offset)
+            mm16.linear(Wd, xd, y, bias=bd, act="relu", resid=put(r, out_t, cuda, pad, offset), z=z)
+            same(z, want, "z")
+            same(y, want.clamp_min(0) + r, "y")
+            clean(), zclean()
+            dx, clean = empty(m, k, out_t, cuda, pad, offset)
+            mm16.linear_dx(Wd, dzd, dx)
+            same(dx, mul(cuda, dz, W.t()), "dx")
+            clean()
+            dW, clean = empty(n, k, out_t, cuda, pad, offset)
+            ws = torch.empty(mm16.linear_dw_ws_bytes(m, n, k), dtype=torch.uint8, device=cuda)
+            dW.fill_(-4.0)
+            mm16.linear_dw(dzd, xd, dW, accumulate=True, ws=ws)
+            same(dW, mul(cuda, dz.t(), x.t()) - 4, "dW")
+            clean()
+        h, clean = empty(m, n, dtype, cuda, pad, offset)
+        gk, gclean = empty(m, n, dtype, cuda, pad, offset)
+        u, uclean = empty(m, n, dtype, cuda, pad, offset)
+        mm16.linear_glu(Wd, Wd, xd, h, g=gk, u=u)
+        same(gk, want - b, "g")
+        same(u, want - b, "u")
+        clean(), gclean(), uclean()
+
+
+def test_expert_outputs_of_any_alignment(cuda):
+    """contiguous outputs that start one element off 16 bytes"""
+    dtype = torch.bfloat16
+    for T, d, E, k, ff in ((700, 264, 130, 4, 264), (37, 264, 20, 8, 136)):
+        L = LargeLayer(cuda, dtype, T, d, E, k, ff, seed=5)
+        off = lambda t, *s: torch.full((s[0] * s[1] * (s[2] if len(s) > 2 else 1) + 1,), 77.0, dtype=t, device=cuda)[1:].view(*s)  # noqa: E731
+        dy, dg, hw = ints(L.g, T, d), ints(L.g, L.P, ff), ints(L.g, L.P, ff)
+        h, g, u = (off(dtype, L.P, ff) for _ in range(3))
+        mm16.moe16_gate_up(L.dev, put(L.x, dtype, cuda), k, L.P, h, **L.kw, g=g, u=u)
+        same(g, L.fwd(L.gate, L.x[L.tok]), "g")
+        same(u, L.fwd(L.up, L.x[L.tok]), "u")
+        for out_t in (dtype, torch.float32):
+            y, dh, dW = off(out_t, L.P, d), off(out_t, L.P, ff), off(out_t, L.nl, ff, d)
+            mm16.moe16_down(L.dev, put(hw, dtype, cuda), L.P, y, **L.kw)
+            same(y, L.fwd(L.down, hw), "y")
+            mm16.moe16_down_dx(L.dev, put(dy, dtype, cuda), k, L.P, *L.grp, dh)
+            same(dh, L.fwd(L.down.transpose(1, 2), dy[L.tok]), "dh")
+            mm16.moe16_dw(L.dev, put(dg, dtype, cuda), 1, put(L.x, dtype, cuda), k, L.P, *L.grp, dW)
+            same(dW, L.dw(dg, L.x[L.tok]), "dW")
