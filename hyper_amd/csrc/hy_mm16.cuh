@@ -8,6 +8,7 @@
 // P is the matrix instruction's A operand and Q its B operand: lane l of a 16 x 16 product then holds columns
 // 4 (l / 16) .. + 3 of row l % 16, four neighbours of one output row, which it stores together.
 #pragma once
+#include "hy_div.h"
 #include "hy_internal.h"
 
 #include <algorithm>
@@ -34,7 +35,7 @@ struct MMArgs {
     // grouping: pairs order[start ..] of the egrp triples; operand row of pair p is p / kq (TN: also p / kp), output row p
     const int *order, *order_n, *egrp, *slot, *ids;
     int n_local, n_expert, n_pairs, max_active;
-    uint32_t kq, kp;
+    Divisor kq, kp;
     // epilogue: v = acc + bias; z = v; v = act(v) * wts[p] + resid (+ out).  Gated: h = SwiGLU(g, u), g and u on request
     const float *bias, *wts;
     const void *resid;
@@ -122,10 +123,6 @@ __device__ __forceinline__ float mm_act_grad(int act, float z) {
     }
     return 1.0f;
 }
-
-// p / k for 0 <= p < 2^31 and 1 <= k <= 64: M = ceil(2^40 / k) is at most 1 / k + 2^-40 too large, p times that error < 2^-9 < 1 / k
-__device__ __forceinline__ int div_k(int p, uint32_t k, uint64_t M) { return k == 1 ? p : (int) (((uint64_t) (uint32_t) p * M) >> 40); }
-__host__ __device__ __forceinline__ uint64_t div_magic(uint32_t k) { return ((1ull << 40) + k - 1) / k; }
 
 // W neighbours (4 or 8) of a T or fp32 matrix, the first n of them; vec: they can be moved in 16-byte pieces
 template <typename T, int W> __device__ __forceinline__ void put_n(void *base, int64_t at, const float *v, int n, bool f32, bool vec) {

@@ -26,12 +26,11 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
         if (!find_tile<256, 64>(a, ncol, false, g, tile, col, part)) return;
     }
     const int c0 = col * BN, r0 = tile * 64;
-    const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);
     if constexpr (KIND != TN) {
         if (tid < 64) {
             const int p = r0 + tid < g.cnt ? pair_of(a, g, r0 + tid) : -1;
             s_pair[tid] = p;
-            s_row[tid] = p < 0 ? -1 : div_k(p, a.kq, mq);
+            s_row[tid] = p < 0 ? -1 : div_k(p, a.kq);
         }
         __syncthreads();
     }
@@ -49,8 +48,8 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int r = r0 + (tid & 7) * 8 + i, c = c0 + (tid & 7) * 8 + i;
-                    qv[i] = p >= 0 && r < a.R ? Q[(int64_t) div_k(p, a.kq, mq) * a.ldq + r] : (T) 0.0f;
-                    pv[i] = p >= 0 && c < a.N ? P[(int64_t) div_k(p, a.kp, mp) * a.ldp + c] : (T) 0.0f;
+                    qv[i] = p >= 0 && r < a.R ? Q[(int64_t) div_k(p, a.kq) * a.ldq + r] : (T) 0.0f;
+                    pv[i] = p >= 0 && c < a.N ? P[(int64_t) div_k(p, a.kp) * a.ldp + c] : (T) 0.0f;
                     db[i] += (float) qv[i];
                 }
             } else {

@@ -29,7 +29,7 @@ static bool vec16(const void *p, int64_t ld, int bytes) { return !p || (ld % (16
 
 #define HY_TRY(e) do { const int rc_ = (e); if (rc_ != HY_OK) return rc_; } while (0)
 
-static MMArgs args() { MMArgs a{}; a.kq = a.kp = 1; return a; }
+static MMArgs args() { MMArgs a{}; a.kq = a.kp = divisor(1); return a; }
 
 // ------------------------------------------------------------------ experts
 
@@ -207,7 +207,7 @@ int hy_moe16_gate_up(const hy_moe_dev *m, const void *x, int64_t ldx, int k, con
     if (g && (misaligned(g, 2) || misaligned(u, 2))) { set_error("%s: g and u must be 2-byte aligned", what); return HY_EBAD_SHAPE; }
     if (n_pairs == 0) return HY_OK;
     MMArgs a = moe_args(m, n_pairs, ids, order, order_n, egrp, max_active);
-    a.P = m->gate; a.P2 = m->up; a.ldp = m->n; a.Q = x; a.ldq = ldx; a.kq = (uint32_t) k; a.N = m->ff; a.K = m->n; a.R = 1;
+    a.P = m->gate; a.P2 = m->up; a.ldp = m->n; a.Q = x; a.ldq = ldx; a.kq = divisor((uint32_t) k); a.N = m->ff; a.K = m->n; a.R = 1;
     a.g = g; a.u = u; a.out = h; a.ldo = m->ff; a.clamp = m->clamp;
     a.vec = vec16(h, m->ff, 2) && vec16(g, m->ff, 2) && vec16(u, m->ff, 2);
     return order ? launch_mm(NT, m->tg, true, a, s, what) : launch_mv(m->tg, true, a, s, what);
@@ -243,7 +243,7 @@ int hy_moe16_down_dx(const hy_moe_dev *m, const void *dy, int64_t lddy, int k, i
     HY_TRY(check_mat(what, "dh", dh, m->ff, n_pairs, m->ff, ob, true));
     if (n_pairs == 0) return HY_OK;
     MMArgs a = moe_args(m, n_pairs, nullptr, order, order_n, egrp, max_active);
-    a.P = m->down; a.ldp = m->ff; a.Q = dy; a.ldq = lddy; a.kq = (uint32_t) k; a.N = m->ff; a.K = m->n;
+    a.P = m->down; a.ldp = m->ff; a.Q = dy; a.ldq = lddy; a.kq = divisor((uint32_t) k); a.N = m->ff; a.K = m->n;
     a.out = dh; a.ldo = m->ff; a.out_f32 = out_type == HY_F32;
     a.vec = vec16(dh, m->ff, ob);
     return launch_mm(NN, m->td, false, a, s, what);
@@ -282,7 +282,7 @@ int hy_moe16_dw(const hy_moe_dev *m, int type, const void *a_, int64_t lda, int 
     HY_TRY(check_mat(what, "b", b, ldb, n_pairs, cols, 2, false));
     HY_TRY(check_mat(what, "dW", dW, cols, rows, cols, ob, true));
     MMArgs a = moe_args(m, n_pairs, nullptr, order, order_n, egrp, max_active);
-    a.P = b; a.ldp = ldb; a.kp = (uint32_t) kb; a.Q = a_; a.ldq = lda; a.kq = (uint32_t) ka; a.R = rows; a.N = cols;
+    a.P = b; a.ldp = ldb; a.kp = divisor((uint32_t) kb); a.Q = a_; a.ldq = lda; a.kq = divisor((uint32_t) ka); a.R = rows; a.N = cols;
     a.out = dW; a.ldo = cols; a.ostride = (int64_t) rows * cols; a.out_f32 = out_type == HY_F32; a.accumulate = accumulate != 0;
     a.vec = vec16(dW, cols, ob);
     return launch_mm(TN, type, false, a, s, what);

@@ -99,7 +99,6 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, wp = wave % WP, wq = wave / WP;
     constexpr int CN = DUAL ? BN / 2 : BN;   // output columns a tile
     const int c0 = col * CN;
-    const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);
     const int64_t ldp2 = a.ldp * 2, ldq2 = a.ldq * 2;
     OP P;
     OQ Q;
@@ -131,7 +130,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
             Q.p[i] = (const char *) a.Q + r * 2 + (a.order ? 0 : (OQ::krow(wave, lane, i) + g.start) * ldq2);
         } else {
             const int p = max(s_pair[at], 0);
-            Q.p[i] = (const char *) a.Q + div_k(p, a.kq, mq) * ldq2 + OQ::krow(wave, lane, i) * 2;
+            Q.p[i] = (const char *) a.Q + div_k(p, a.kq) * ldq2 + OQ::krow(wave, lane, i) * 2;
         }
     }
     const uint32_t lds0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds_addr(s_mem));
@@ -144,8 +143,8 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
             if (!a.order) return;
             for (int i = tid; i < CH; i += NTH) {
                 const int k = chunk * CH + i, p = k < K ? pair_of(a, g, k) : -1;
-                s_look[(chunk & 1) * CH + i] = p < 0 ? -1 : div_k(p, a.kp, mp);
-                s_look[(2 + (chunk & 1)) * CH + i] = p < 0 ? -1 : div_k(p, a.kq, mq);
+                s_look[(chunk & 1) * CH + i] = p < 0 ? -1 : div_k(p, a.kp);
+                s_look[(2 + (chunk & 1)) * CH + i] = p < 0 ? -1 : div_k(p, a.kq);
             }
         }
     };

@@ -115,11 +115,10 @@ template <typename T, bool F32> __global__ __launch_bounds__(256, 1) void k_grad
     const int nt = min(nct, ncol - col), nstage = max((K + BK - 1) / BK, 1);   // (no pairs: a stage of zeros)
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, wp = wave & 1, wq = wave >> 1;
-    const uint64_t mq = div_magic(a.kq), mp = div_magic(a.kp);
     for (int i = tid; i < nstage * BK; i += 256) {   // the pairs' rows; -1: none
         const int p = i < K ? pair_of(a, g, i) : -1;
-        s_look[i] = p < 0 ? -1 : div_k(p, a.kp, mp);
-        s_look[PAIRS + i] = p < 0 ? -1 : div_k(p, a.kq, mq);
+        s_look[i] = p < 0 ? -1 : div_k(p, a.kp);
+        s_look[PAIRS + i] = p < 0 ? -1 : div_k(p, a.kq);
     }
     const uint32_t lds0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds_addr(s_mem));
     const uint32_t pitch_p = (uint32_t) a.ldp * 2, pitch_q = (uint32_t) a.ldq * 2;

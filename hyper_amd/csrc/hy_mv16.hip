@@ -31,7 +31,7 @@ template <typename T, bool DUAL, int NR, bool AL> __global__ __launch_bounds__(2
         if ((uint32_t) e >= (uint32_t) a.n_expert) return;
         le = a.slot[e];
         if ((uint32_t) le >= (uint32_t) a.n_local) return;
-        row0 = div_k(p, a.kq, div_magic(a.kq));
+        row0 = div_k(p, a.kq);
         out0 = p;
         nr = 1;
     }
