@@ -99,8 +99,8 @@ __device__ __forceinline__ float mm_act(int act, float z) {
     case HY_ACT_GELU: {
         float c, e;
         mm_erfc(z, c, e);
-        const float h = 0.5f * z * c;
-        return z >= 0.0f ? z - h : h;
+        const float h = 0.5f * fminf(z, 14.0f) * c;   // 0 from 14 on, for +inf too; NaN takes the second way out
+        return z < 0.0f ? h : z - h;
     }
     case HY_ACT_GELU_TANH: return z * mm_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
     }

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from hyper_amd import mm16
+from tests.test_gpu_mm16 import TYPES, act64
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +52,38 @@ def test_more_than_2_24_tokens(cuda, d):
     dW2 = torch.empty(E, d, ff, device=cuda)
     mm16.moe16_dw(m, x, k, a, 1, P, *grp, dW2)
     assert torch.equal(dW2, want.transpose(1, 2)), "rows of tokens on the left"
+
+
+def ends(dtype):
+    """infinities, NaN and both signs of values from nothing to the type's largest"""
+    v = [float("inf"), float("nan"), 0.0, 1.0, 5.0, 13.875, 14.5, 30.0, 100.0, 3e4] + ([1e15, 1e20, 1e30, 3e38] if dtype == torch.bfloat16 else [])
+    return torch.tensor([s * t for t in v for s in (1.0, -1.0)]).to(dtype)
+
+
+def agrees(got, want, rel, tiny, what):
+    """equal where the formula is infinite or NaN, else within rel of it, or tiny (values whose exponentials leave the normal numbers)"""
+    rel = torch.as_tensor(rel, dtype=torch.float64).expand_as(want)
+    got = got.double().cpu()
+    wild = ~want.isfinite()
+    assert torch.equal(got[wild].nan_to_num(nan=7.0), want[wild].nan_to_num(nan=7.0)), (what, got, want)
+    off = (got[~wild] - want[~wild]).abs()
+    assert (off <= rel[~wild] * want[~wild].abs() + tiny).all(), (what, got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", list(mm16.ACTS))
+@pytest.mark.parametrize("m,k", [(1, 8), (5, 8), (5, 9), (40, 8), (300, 8), (40, 9)])   # each kernel that ends in an activation
+def test_activations_of_extreme_values(cuda, dtype, act, m, k):
+    """against the formula in 64 bits: it is +inf at +inf, and NaN where it is 0 times an infinity.  Bound: a few 2^-24 of
+    evaluation; gelu_tanh's exponent is the result of four roundings, each half a step of an exponent of at most 88, and an
+    absolute error of an exponent is a relative one of the value."""
+    z = ends(dtype)
+    n = z.numel()
+    W, x = torch.zeros(n, k, dtype=dtype), torch.zeros(m, k, dtype=dtype)
+    W[:, 0], x[:, 0] = z, 1.0
+    out = torch.empty(m, n, dtype=torch.float32, device=cuda)
+    mm16.linear(W.to(cuda), x.to(cuda), out, act=act)
+    rel = 16 * 2.0 ** -24
+    if act == "gelu_tanh":
+        rel = rel + 4 * 2.0 ** -24 * (1.6 * (z.double() + 0.044715 * z.double() ** 3)).abs().clamp_max(88).nan_to_num()
+    agrees(out, act64(act, z.double()).expand(m, n), rel, 1e-36, act)
