@@ -118,7 +118,8 @@ __device__ __forceinline__ float mm_act_grad(int act, float z) {
     }
     case HY_ACT_GELU_TANH: {   // z sigmoid(2 a): s + z s (1 - s) 2 a'
         const float s = mm_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
-        return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);
+        const float x = fminf(fmaxf(z, -16.0f), 16.0f);   // s (1 - s) is 0 from there on, while z^2 of large z is infinite
+        return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * x, x, 1.0f), s);
     }
     }
     return 1.0f;

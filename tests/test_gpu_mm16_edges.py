@@ -1,6 +1,8 @@
 """The 16-bit products at the ends of their ranges: many pairs, infinities and NaN, slot tables that change, empty calls.
 
 Products are on small integers, exact in any order of fp32 sums, as in test_gpu_mm16."""
+import math
+
 import pytest
 import torch
 
@@ -87,3 +89,34 @@ def test_activations_of_extreme_values(cuda, dtype, act, m, k):
     if act == "gelu_tanh":
         rel = rel + 4 * 2.0 ** -24 * (1.6 * (z.double() + 0.044715 * z.double() ** 3)).abs().clamp_max(88).nan_to_num()
     agrees(out, act64(act, z.double()).expand(m, n), rel, 1e-36, act)
+
+
+def act_grad64(name, z):
+    if name == "relu":
+        return torch.where(z.isnan(), z, (z > 0).double())
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return s + z * s * (1 - s)
+    if name == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if name == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        s = torch.sigmoid(2 * c * (z + 0.044715 * z ** 3))
+        return s + z * s * (1 - s) * 2 * c * (1 + 0.134145 * z * z)
+    return torch.ones_like(z)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", list(mm16.ACTS))
+@pytest.mark.parametrize("odd", [False, True])
+def test_activation_gradients_of_extreme_values(cuda, dtype, act, odd):
+    """1 and 0 far from zero, up to the type's largest value, whose square is no float; bounds as for the activations, and the
+    sum of two terms that the gradient is"""
+    z = ends(dtype)
+    z = torch.cat([z, z[:(1 if odd else 8 - z.numel() % 8)]])
+    out = torch.empty(1, z.numel(), dtype=dtype, device=cuda)
+    mm16.act_bwd(act, z[None].to(cuda), torch.ones_like(z)[None].to(cuda), out)
+    want, rel = act_grad64(act, z.double())[None], 32 * 2.0 ** -24 + torch.finfo(dtype).eps / 2
+    if act == "gelu_tanh":
+        rel = rel + 8 * 2.0 ** -24 * (1.6 * (z.double() + 0.044715 * z.double() ** 3)).abs().clamp_max(88).nan_to_num()[None]
+    agrees(out, want, rel, 1e-36 if dtype == torch.bfloat16 else 2.0 ** -25, act)
