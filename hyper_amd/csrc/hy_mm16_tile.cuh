@@ -350,10 +350,11 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
                                 put_n<T, 8>(a.u, row[u] * a.ldo + cl, w[u], 8, false, true);
                             }
                     }
+                    mm_limit<U * 8>(&v[0][0], &w[0][0], a.clamp);
 #pragma unroll
                     for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[u][e] = mm_swiglu(v[u][e], w[u][e], a.clamp);
+                        for (int e = 0; e < 8; ++e) v[u][e] = mm_swiglu(v[u][e], w[u][e]);
                 } else {
                     if (a.bias) {
                         const f4 *b = (const f4 *) (a.bias + cl);

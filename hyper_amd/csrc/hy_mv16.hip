@@ -69,7 +69,8 @@ template <typename T, bool DUAL, int NR, bool AL> __global__ __launch_bounds__(2
         if constexpr (DUAL) {
             const int64_t at = row * a.ldo + c0;
             if (a.g) { ((T *) a.g)[at] = (T) acc[0][r]; ((T *) a.u)[at] = (T) acc[1][r]; }
-            ((T *) a.out)[at] = (T) mm_swiglu(acc[0][r], acc[1][r], a.clamp);
+            mm_limit<1>(&acc[0][r], &acc[1][r], a.clamp);
+            ((T *) a.out)[at] = (T) mm_swiglu(acc[0][r], acc[1][r]);
         } else {
             const float wt = a.wts ? a.wts[row] : 1.0f;
 #pragma unroll
@@ -231,8 +232,8 @@ template <typename T, int V> __global__ __launch_bounds__(256) void k_swiglu_bwd
             if (L > 0.0f) {
                 gin = !(gg > L);
                 uin = !(uu > L || uu < -L);
-                gg = fminf(gg, L);
-                uu = fminf(fmaxf(uu, -L), L);
+                gg = gin ? gg : L;   // (NaN stays)
+                uu = uin ? uu : copysignf(L, uu);
             }
             const float s = mm_sigmoid(gg), silu = gg * s, h = silu * uu;
             sum = fmaf(d, h, sum);

@@ -316,8 +316,8 @@ int hy_block_ints(int type, const uint8_t *rows, size_t row_bytes, int nrows, co
    none): of out's type, may be out itself; z (NULL: none): the values before act, of `type`, for hy_act_bwd. */
 int hy_linear(int type, const void *W, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, const float *bias, int act,
               const void *resid, int64_t ldr, void *z, int64_t ldz, void *out, int out_type, int64_t ldo, hipStream_t s);
-/* Gated: g = x Wg^T, u = x Wu^T, h = silu(min(g, clamp)) * max(-clamp, min(u, clamp)) (clamp 0: no limits), a shared
-   expert's gate/up.  g and u (both or neither, row distance ldh) keep the products for hy_swiglu_bwd. */
+/* Gated: g = x Wg^T, u = x Wu^T, h = silu(min(g, clamp)) * max(-clamp, min(u, clamp)) (clamp 0: no limits; NaN
+   stays NaN), a shared expert's gate/up.  g and u (both or neither, row distance ldh) keep the products for hy_swiglu_bwd. */
 int hy_linear_glu(int type, const void *Wg, const void *Wu, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, float clamp,
                   void *g, void *u, void *h, int64_t ldh, hipStream_t s);
 /* dz = dy act'(z), [m][n].  dz may be dy or z. */

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from hyper_amd import mm16
-from tests.test_gpu_mm16 import TYPES, act64
+from tests.test_gpu_mm16 import TYPES, act64, same
 
 pytestmark = pytest.mark.gpu
 
@@ -64,12 +64,12 @@ def ends(dtype):
 
 def agrees(got, want, rel, tiny, what):
     """equal where the formula is infinite or NaN, else within rel of it, or tiny (values whose exponentials leave the normal numbers)"""
-    rel = torch.as_tensor(rel, dtype=torch.float64).expand_as(want)
+    rel, tiny = (torch.as_tensor(v, dtype=torch.float64).expand_as(want) for v in (rel, tiny))
     got = got.double().cpu()
     wild = ~want.isfinite()
     assert torch.equal(got[wild].nan_to_num(nan=7.0), want[wild].nan_to_num(nan=7.0)), (what, got, want)
     off = (got[~wild] - want[~wild]).abs()
-    assert (off <= rel[~wild] * want[~wild].abs() + tiny).all(), (what, got, want)
+    assert (off <= rel[~wild] * want[~wild].abs() + tiny[~wild]).all(), (what, got, want)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -120,3 +120,57 @@ def test_activation_gradients_of_extreme_values(cuda, dtype, act, odd):
     if act == "gelu_tanh":
         rel = rel + 8 * 2.0 ** -24 * (1.6 * (z.double() + 0.044715 * z.double() ** 3)).abs().clamp_max(88).nan_to_num()[None]
     agrees(out, want, rel, 1e-36 if dtype == torch.bfloat16 else 2.0 ** -25, act)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 8), (5, 8), (40, 8), (300, 8), (40, 9)])   # each kernel that ends in a gated product
+@pytest.mark.parametrize("clamp", [0.0, 7.0])
+def test_gated_products_of_extreme_values(cuda, dtype, m, k, clamp):
+    """every pair of a gate and an up value, against the formula in 64 bits: a limit stops infinities and keeps NaN.  Products
+    that 64 bits hold and the type does not are infinite; near its largest value only a rounding decides: those are left out, and
+    so is silu(-100), which is 0 in the kernels, times an infinity"""
+    z = ends(dtype)
+    g, u = z.repeat_interleave(z.numel()), z.repeat(z.numel())
+    n = g.numel()
+    Wg, Wu, x = torch.zeros(n, k, dtype=dtype), torch.zeros(n, k, dtype=dtype), torch.zeros(m, k, dtype=dtype)
+    Wg[:, 0], Wu[:, 0], x[:, 0] = g, u, 1.0
+    h, gd, ud = (torch.empty(m, n, dtype=dtype, device=cuda) for _ in range(3))
+    mm16.linear_glu(Wg.to(cuda), Wu.to(cuda), x.to(cuda), h, clamp=clamp, g=gd, u=ud)
+    same(gd, g.double().expand(m, n), "g")
+    same(ud, u.double().expand(m, n), "u")
+    a, b = g.double(), u.double()
+    if clamp:
+        a, b = a.clamp_max(clamp), b.clamp(-clamp, clamp)
+    want, top = a * torch.sigmoid(a) * b, torch.finfo(dtype).max
+    want = torch.where(want.abs() > 1.01 * top, want.sign() * float("inf"), want)
+    keep = ~(want.isfinite() & (want.abs() > 0.99 * top)) & ~((a < -87) & (a > -800) & b.isinf())
+    # below g = -87.33 silu is 0, at most 1.04e-36 off, and that times u
+    agrees(h[:, keep.to(cuda)], want[keep].expand(m, -1), 32 * 2.0 ** -24 + torch.finfo(dtype).eps / 2,
+           (1.04e-36 * b.abs() + (2.0 ** -134 if dtype == torch.bfloat16 else 2.0 ** -25)).nan_to_num(posinf=0)[keep].expand(m, -1), f"clamp {clamp}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ff", [64, 33])
+def test_gradients_of_nan_below_a_limit(cuda, dtype, ff):
+    """a NaN gate or up value shows in what depends on it and in its row's weight, and nowhere else; u = -2 lies beyond the limit
+    1.5, so its gradient is 0 whatever the gate is"""
+    P = 4
+    g, u, dh = (torch.full((P, ff), v, dtype=dtype, device=cuda) for v in (0.5, -2.0, 1.0))
+    w = torch.full((P,), 0.5, device=cuda)
+
+    def call():
+        o = [torch.empty(P, ff, dtype=dtype, device=cuda) for _ in range(3)] + [torch.empty(P, device=cuda)]
+        mm16.swiglu_bwd(g, u, dh, w, *o, clamp=1.5)
+        return o
+    u[1, 6] = 1.0
+    good = call()
+    assert all(t.isfinite().all() for t in good)
+    g[1, 5] = g[1, 6] = u[2, 7] = float("nan")
+    dg, du, hw, dw = call()
+    for t, bad in ((dg, [(1, 5), (1, 6), (2, 7)]), (du, [(1, 6)]), (hw, [(1, 5), (1, 6), (2, 7)])):
+        mark = torch.zeros(P, ff, dtype=torch.bool, device=cuda)
+        for at in bad:
+            mark[at] = True
+        assert torch.equal(t.isnan(), mark)
+    assert torch.equal(dw.isnan().cpu(), torch.tensor([False, True, True, False]))
+    assert torch.equal(dg[0], good[0][0]) and torch.equal(du[0], good[1][0]) and torch.equal(hw[3], good[2][3]) and torch.equal(dw[[0, 3]], good[3][[0, 3]])
