@@ -109,6 +109,7 @@ SIGNATURES = {
     "hy_linear_dw": (_I, [_I, _P, _L, _P, _L, _I, _I, _I, _P, _I, _L, _P, _I, _P, ctypes.c_size_t, _P]),
     "hy_moe16_gate_up": (_I, [_DEV, _P, _L, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P]),
     "hy_moe16_down": (_I, [_DEV, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "hy_moe16_reduce": (_I, [_DEV, _P, _P, _P, _I, _P, _I, _P, _P]),
     "hy_moe16_down_dx": (_I, [_DEV, _P, _L, _I, _I, _P, _P, _P, _I, _P, _I, _P]),
     "hy_moe16_gate_up_dx": (_I, [_DEV, _P, _P, _I, _P, _P, _P, _I, _P, _I, _P]),
     "hy_moe16_dw": (_I, [_DEV, _I, _P, _L, _I, _I, _P, _L, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P]),

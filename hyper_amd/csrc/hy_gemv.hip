@@ -207,15 +207,20 @@ int launch_down(const hy_moe_dev &m, const float *h, const int *ids, const float
 // out[t][r] = sg * shexp (if shexp) then + y of the token's pairs in ascending expert id (src/cpu_moe.cpp:863-874
 // order; the first pair is the start value when there is no shared expert); negative ids are skipped.  One block
 // per token: wave 0 ranks the token's pairs (rank = valid pairs with a smaller id, ties by position), then every
-// thread sums VW consecutive columns per pass (VW = 4: 16-byte loads when n and the rows allow it).
-template <int VW>
+// thread sums VW consecutive columns per pass (VW = 4: 16-byte loads when n and the rows allow it).  LOCAL: pairs whose
+// expert the slot table does not hold are left out too.
+struct SlotTable { const int *slot; int n_expert, n_local; };
+template <int VW, bool LOCAL>
 __global__ __launch_bounds__(256) void k_reduce(const float *__restrict__ shexp, const float *__restrict__ sg, const float *__restrict__ y,
-                                                int k, float *__restrict__ out, int n, const int *__restrict__ ids, int res) {
+                                                int k, float *__restrict__ out, int n, const int *__restrict__ ids, int res, SlotTable tab) {
     __shared__ int ord[64];
     __shared__ int s_cnt;
     const int t = blockIdx.x, tid = threadIdx.x;
     if (tid < 64) {
-        const int e = tid < k ? ids[(size_t) t * k + tid] : -1;
+        int e = tid < k ? ids[(size_t) t * k + tid] : -1;
+        if constexpr (LOCAL) {
+            if (e >= tab.n_expert || (e >= 0 && (uint32_t) tab.slot[e] >= (uint32_t) tab.n_local)) e = -1;
+        }
         int rank = 0;
         for (int i = 0; i < k; ++i) {
             const int o = __shfl(e, i);
@@ -265,12 +270,21 @@ __global__ __launch_bounds__(256) void k_reduce(const float *__restrict__ shexp,
         else out[(size_t) t * n + r] = acc[0];
     }
 }
-int launch_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int *ids, hipStream_t s, int res) {
+template <bool LOCAL>
+static int launch_reduce_t(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int *ids, hipStream_t s, int res,
+                           const SlotTable &tab, const char *what) {
     if (nt == 0) return HY_OK;
     const bool vec = n % 4 == 0 && ((uintptr_t) y & 15) == 0 && ((uintptr_t) out & 15) == 0 && ((uintptr_t) shexp & 15) == 0;
-    if (vec) hipLaunchKernelGGL(k_reduce<4>, dim3(nt), dim3(256), 0, s, shexp, sg, y, k, out, n, ids, res);
-    else hipLaunchKernelGGL(k_reduce<1>, dim3(nt), dim3(256), 0, s, shexp, sg, y, k, out, n, ids, res);
-    return check_launch("hy_moe_reduce");
+    if (vec) k_reduce<4, LOCAL><<<dim3(nt), dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
+    else k_reduce<1, LOCAL><<<dim3(nt), dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
+    return check_launch(what);
+}
+int launch_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int *ids, hipStream_t s, int res) {
+    return launch_reduce_t<false>(shexp, sg, y, k, out, n, nt, ids, s, res, SlotTable{}, "hy_moe_reduce");
+}
+int launch_reduce_local(const hy_moe_dev &m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int *ids,
+                        hipStream_t s) {
+    return launch_reduce_t<true>(shexp, sg, y, k, out, m.n, nt, ids, s, 0, SlotTable{m.slot, m.n_expert, m.n_local}, "hy_moe16_reduce");
 }
 
 // ---------------------------------------------------------------- fused decode down + combine

@@ -34,6 +34,8 @@ int launch_down_reduce(const hy_moe_dev &m, const float *h, const int *ids, cons
                        float *out, int nt, hipStream_t s, int res = 0);
 int launch_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int *ids, hipStream_t s,
                   int res = 0);
+int launch_reduce_local(const hy_moe_dev &m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int *ids,
+                        hipStream_t s);
 int launch_gemm_gate_up(const hy_moe_dev &m, const void *xq, int k, int n_pairs, const int *order, const int *order_n, const int *egrp,
                         int max_active, float *h, hipStream_t s);
 int launch_gemm_down(const hy_moe_dev &m, const void *hq, int n_pairs, const int *order, const int *order_n, const int *egrp, int max_active,

@@ -231,6 +231,18 @@ int hy_moe16_down(const hy_moe_dev *m, const void *h, const int32_t *ids, int n_
     return order ? launch_mm(NT, m->td, false, a, s, what) : launch_mv(m->td, false, a, s, what);
 }
 
+int hy_moe16_reduce(const hy_moe_dev *m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int32_t *ids,
+                    hipStream_t s) {
+    const char *what = "hy_moe16_reduce";
+    HY_TRY(check_dev16(what, m, false, false));
+    HY_TRY(check_k(what, k));
+    if (nt < 0 || nt > HY_MM_MAX / k) { set_error("%s: %d rows of %d pairs (up to 2^30 pairs)", what, nt, k); return nt < 0 ? HY_EINVAL : HY_EBAD_SHAPE; }
+    if (nt == 0) return HY_OK;
+    if (!y || !out || !ids) { set_error("%s: null y, out or ids", what); return HY_EINVAL; }
+    if (misaligned(shexp, 4) || misaligned(sg, 4) || misaligned(y, 4) || misaligned(out, 4) || misaligned(ids, 4)) { set_error("%s: arguments must be 4-byte aligned", what); return HY_EBAD_SHAPE; }
+    return launch_reduce_local(*m, shexp, sg, y, k, out, nt, ids, s);
+}
+
 int hy_moe16_down_dx(const hy_moe_dev *m, const void *dy, int64_t lddy, int k, int n_pairs, const int32_t *order, const int32_t *order_n,
                      const int32_t *egrp, int max_active, void *dh, int out_type, hipStream_t s) {
     const char *what = "hy_moe16_down_dx";

@@ -258,6 +258,18 @@ def moe16_down(m: Moe16Dev, h, n_pairs, y, wts=None, ids=None, order=None, order
           m.ref, _p(h), _p(ids), n_pairs, _p(order), _p(order_n), _p(egrp), max_active, _p(wts), _p(y), _TYPE[y.dtype])
 
 
+def moe16_reduce(m: Moe16Dev, shexp, sg, y, k, out, nt, ids, stream=None):
+    """out[t] = sg[t] shexp[t] + the float32 rows y of token t's pairs, in ascending expert order, pairs whose expert is not
+    local left out; shexp and sg may be None."""
+    _pairs("y", y, nt * k, m.n, torch.float32)
+    _pairs("out", out, nt, m.n, torch.float32)
+    if shexp is not None:
+        _pairs("shexp", shexp, nt, m.n, torch.float32)
+    _vec("sg", sg, nt, torch.float32)
+    _vec("ids", ids, nt * k, torch.int32)
+    _call(lib().hy_moe16_reduce, m.slot, stream, (shexp, sg, y, out, ids), m.ref, _p(shexp), _p(sg), _p(y), k, _p(out), nt, _p(ids))
+
+
 def moe16_down_dx(m: Moe16Dev, dy, k, n_pairs, order, order_n, egrp, max_active, dh, stream=None):
     """dh[p] = dy[p // k] down_e, not yet weighted."""
     if m.down is None:
@@ -322,8 +334,10 @@ class Moe16LayerRunner:
     """Workspace and call sequence for one MoE layer with 16-bit experts, as moe.MoeLayerRunner has it for quantized ones:
     router GEMV, softmax routing, then by ids (up to `decode_rows` rows) or grouped: gate/up, down, combine.
 
-    forward(x) takes [nt, d] float32 rows.  With keep=True it keeps what backward(dy) needs.  `shared`: an always-on expert
-    (a Moe16Dev with one matrix) added with weight 1."""
+    forward(x) takes [nt, d] float32 rows; pairs whose expert dev.slot does not hold at the time add nothing to the output.  With
+    keep=True it keeps what backward(dy) needs, the slot table among it; backward is for layers whose experts were all local
+    when the runner was made.  `shared`: an always-on expert (a Moe16Dev with one matrix) added with weight 1; backward leaves it
+    and the router out."""
 
     decode_rows = 2   # by ids every pair reads its expert's matrices; grouped, an expert's rows share them
 
@@ -344,14 +358,12 @@ class Moe16LayerRunner:
         new = lambda *s, dtype=self.dtype: torch.empty(*s, dtype=dtype, device=device)  # noqa: E731
         self.logits, self.ids, self.wts = new(T, self.E, dtype=torch.float32), new(P, dtype=torch.int32), new(P, dtype=torch.float32)
         self.order, self.order_n, self.egrp = new(P, dtype=torch.int32), torch.zeros(2, dtype=torch.int32, device=device), new(3 * self.E, dtype=torch.int32)
-        # rows of pairs whose expert is not local stay unwritten, and the combine adds every row: they are cleared where
-        # an expert is missing
-        self.all_local = bool((dev.slot >= 0).all()) and bool((dev.slot < dev.n_local).all())
+        self.all_local = bool((dev.slot >= 0).all()) and bool((dev.slot < dev.n_local).all())   # now; every call reads the table itself
         self.x16, self.h, self.y = new(T, self.d), new(P, self.ff), new(P, self.d, dtype=torch.float32)
         self.out = new(T, self.d, dtype=torch.float32)
         self.sh_y = new(T, self.d, dtype=torch.float32) if shared is not None else None
         self.sh_h = new(T, shared.ff) if shared is not None else None
-        self.g = self.u = None
+        self.g = self.u = self.kept_dev = None
         self.kept = 0
 
     def _rows(self, x):
@@ -385,16 +397,16 @@ class Moe16LayerRunner:
             if keep:
                 if self.g is None:
                     self.g, self.u = torch.empty_like(self.h), torch.empty_like(self.h)
+                    self.kept_dev = Moe16Dev(self.dev.gate, self.dev.up, self.dev.down, torch.empty_like(self.dev.slot), self.dev.clamp)
                 gu = dict(g=self.g, u=self.u)
-            if not self.all_local:
-                self.y[:P].zero_()
+                torch.add(self.dev.slot, 0, out=self.kept_dev.slot)   # (a kernel: no copy node in a captured graph)
             moe16_gate_up(self.dev, self.x16[:nt], k, P, self.h, **how, **gu, stream=stream)
             moe16_down(self.dev, self.h, P, self.y, wts=self.wts, **how, stream=stream)
             if self.shared is not None:
                 S = self.shared
                 linear_glu(S.gate[0], S.up[0], self.x16[:nt], self.sh_h[:nt], clamp=S.clamp, stream=stream)
                 linear(S.down[0], self.sh_h[:nt], self.sh_y[:nt], stream=stream)
-            moe.moe_reduce(self.sh_y, None, self.y, k, self.out, self.d, nt, self.ids, stream)
+            moe16_reduce(self.dev, self.sh_y, None, self.y, k, self.out, nt, self.ids, stream)
         self.kept = nt if keep else 0
         return self.out[:nt]
 
@@ -406,18 +418,19 @@ class Moe16LayerRunner:
             raise ValueError("backward follows forward(keep=True) of the same rows")
         if not self.all_local:
             raise ValueError("backward needs every expert local")
-        P, dev = nt * k, self.dev
+        P, dev = nt * k, self.kept_dev   # the slot table as forward found it
         grp = (self.order, self.order_n, self.egrp, min(self.E, P, 1024))
         new = lambda *s, dtype=self.dtype: torch.empty(*s, dtype=dtype, device=dy.device)  # noqa: E731
         with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dy.device)):
             dy16, dh, dg, du, hw = new(nt, self.d), new(P, self.ff), new(P, self.ff), new(P, self.ff), new(P, self.ff)
-            dwts, dxp, dx = new(nt, k, dtype=torch.float32), new(P, self.d, dtype=torch.float32), new(nt, self.d, dtype=torch.float32)
+            dwts, dxp, dx = torch.zeros(nt, k, device=dy.device), new(P, self.d, dtype=torch.float32), new(nt, self.d, dtype=torch.float32)
             W = {n: new(*t.shape, dtype=torch.float32) for n, t in (("gate", dev.gate), ("up", dev.up), ("down", dev.down))}
             rows16(dy, dy16)
             moe16_down_dx(dev, dy16, k, P, *grp, dh)
-            swiglu_bwd(self.g[:P], self.u[:P], dh, self.wts[:P], dg, du, hw, dwts.view(-1), clamp=dev.clamp)
+            swiglu_bwd(self.g[:P], self.u[:P], dh, self.wts[:P], dg, du, hw, dwts.view(-1), clamp=dev.clamp,
+                       order=self.order, order_n=self.order_n)
             moe16_gate_up_dx(dev, dg, du, P, *grp, dxp)
-            moe.moe_reduce(None, None, dxp, k, dx, self.d, nt, self.ids)
+            moe16_reduce(dev, None, None, dxp, k, dx, nt, self.ids)
             moe16_dw(dev, dg, 1, self.x16[:nt], k, P, *grp, W["gate"])
             moe16_dw(dev, du, 1, self.x16[:nt], k, P, *grp, W["up"])
             moe16_dw(dev, dy16, k, hw, 1, P, *grp, W["down"])

@@ -341,15 +341,19 @@ int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t 
    local are left as they were.
    gate_up: h[p] = SwiGLU(gate_e x[p / k], up_e x[p / k]) with the descriptor's clamp, g and u on request as in
    hy_linear_glu; h, g, u [n_pairs][ff].  down: y[p] = wts[p] (down_e h[p]) (wts NULL: 1), [n_pairs][n]; with out_type
-   HY_F32 hy_moe_reduce combines the rows. */
+   HY_F32 hy_moe_reduce combines the rows, or, where experts may not be local, hy_moe16_reduce. */
 int hy_moe16_gate_up(const hy_moe_dev *m, const void *x, int64_t ldx, int k, const int32_t *ids, int n_pairs, const int32_t *order,
                      const int32_t *order_n, const int32_t *egrp, int max_active, void *g, void *u, void *h, hipStream_t s);
 int hy_moe16_down(const hy_moe_dev *m, const void *h, const int32_t *ids, int n_pairs, const int32_t *order, const int32_t *order_n,
                   const int32_t *egrp, int max_active, const float *wts, void *y, int out_type, hipStream_t s);
+/* Combine: hy_moe_reduce of y [nt k][n] that leaves out the pairs whose expert is not local, whose rows nothing wrote
+   (out of a token without any: sg[t] * shexp[t], or zeros). */
+int hy_moe16_reduce(const hy_moe_dev *m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int32_t *ids,
+                    hipStream_t s);
 /* The backward pass of a layer y[t] = sum_j wts[p] down_e h[p], from dy [tokens][n]:
      hy_moe16_down_dx     dh[p] = dy[p / k] down_e (not yet weighted), [n_pairs][ff]
      hy_swiglu_bwd        from g, u, dh: dwts[p] = sum dh h,  hw = wts h,  dg, du of wts dh       (wts NULL: 1)
-     hy_moe16_gate_up_dx  dx[p] = dg[p] gate_e + du[p] up_e, [n_pairs][n]; hy_moe_reduce sums a token's pairs
+     hy_moe16_gate_up_dx  dx[p] = dg[p] gate_e + du[p] up_e, [n_pairs][n]; hy_moe_reduce (hy_moe16_reduce) sums a token's pairs
      hy_moe16_dw          dW[slot[e]] = sum over e's pairs of a[p / ka]^T b[p / kb], [n_local][rows][cols] (zeros for an
                           expert without pairs): gate from (dg, x), up from (du, x), down from (dy, hw)
    hy_swiglu_bwd takes all n_pairs rows, or with order and order_n the pairs listed there; hw and dwts may be NULL; dg, du

@@ -260,6 +260,10 @@ inline void moe16_down(const MoeDev &m, const void *h, const int *ids, int n_pai
                        int max_active, const float *wts, void *y, int out_type, hipStream_t s) {
     check(hy_moe16_down(&m, h, ids, n_pairs, order, order_n, egrp, max_active, wts, y, out_type, s));
 }
+inline void moe16_reduce(const MoeDev &m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int *ids,
+                         hipStream_t s) {
+    check(hy_moe16_reduce(&m, shexp, sg, y, k, out, nt, ids, s));
+}
 inline void moe16_down_dx(const MoeDev &m, const void *dy, int64_t lddy, int k, int n_pairs, const int *order, const int *order_n,
                           const int *egrp, int max_active, void *dh, int out_type, hipStream_t s) {
     check(hy_moe16_down_dx(&m, dy, lddy, k, n_pairs, order, order_n, egrp, max_active, dh, out_type, s));

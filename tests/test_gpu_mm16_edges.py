@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from hyper_amd import mm16
+from tests.helpers import gen
 from tests.test_gpu_mm16 import TYPES, act64, same
 
 pytestmark = pytest.mark.gpu
@@ -174,3 +175,102 @@ def test_gradients_of_nan_below_a_limit(cuda, dtype, ff):
         assert torch.equal(t.isnan(), mark)
     assert torch.equal(dw.isnan().cpu(), torch.tensor([False, True, True, False]))
     assert torch.equal(dg[0], good[0][0]) and torch.equal(du[0], good[1][0]) and torch.equal(hw[3], good[2][3]) and torch.equal(dw[[0, 3]], good[3][[0, 3]])
+
+
+# ------------------------------------------------------------------ slot tables
+
+@pytest.mark.parametrize("n", [64, 66, 33])   # rows of 16-byte pieces, and not
+@pytest.mark.parametrize("nt,k", [(1, 1), (3, 2), (40, 8), (5, 64)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_combine_of_local_pairs(cuda, n, nt, k, shared):
+    """integers, exact in any order; the rows of absent experts hold NaN"""
+    E = 70
+    g = gen(n + nt + k)
+    y = torch.randint(-9, 10, (nt * k, n), generator=g).float()
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(nt)]).reshape(-1).to(torch.int32)
+    slot = torch.randint(-1, 9, (E,), generator=g).to(torch.int32)
+    slot[slot == 8] = 1 << 20                                   # no matrix of the layer's 8
+    ids[::7] = torch.tensor([-1, E, 1 << 30, -(1 << 31)], dtype=torch.int32).repeat(nt * k)[:len(ids[::7])]
+    there = (ids >= 0) & (ids < E)
+    there &= (slot[ids.long().clamp(0, E - 1)] >= 0) & (slot[ids.long().clamp(0, E - 1)] < 8)
+    y[~there] = float("nan")
+    want = torch.where(there[:, None], y, torch.zeros(())).view(nt, k, n).sum(1)
+    b = torch.zeros(8, 8, n, dtype=torch.bfloat16, device=cuda)
+    m = mm16.Moe16Dev(b, b, None, slot.to(cuda))
+    sh = torch.randint(-9, 10, (nt, n), generator=g).float() if shared else None
+    sg = torch.full((nt,), 0.5) if shared else None
+    out = torch.full((nt + 1, n), 77.0, device=cuda)
+    mm16.moe16_reduce(m, sh.to(cuda) if shared else None, sg.to(cuda) if shared else None, y.to(cuda), k, out, nt, ids.to(cuda))
+    assert torch.equal(out[:nt].cpu(), want + (0.5 * sh if shared else 0)) and (out[nt] == 77.0).all()
+
+
+class _Runner:
+    """a layer whose experts can leave; its buffers are filled with NaN before each call"""
+
+    def __init__(self, cuda, nt, without=()):
+        g = gen(11)
+        r = lambda *s: (torch.randn(*s, generator=g) * 0.1).to(torch.bfloat16).to(cuda)  # noqa: E731
+        E, d, ff, k = 8, 64, 40, 2
+        self.gate, self.up, self.down = r(E, ff, d), r(E, ff, d), r(E, d, ff)
+        for e in without:
+            self.down[e] = 0
+        self.slot = torch.arange(E, dtype=torch.int32, device=cuda)
+        self.x, self.dy = torch.randn(nt, d, generator=g).to(cuda), torch.randn(nt, d, generator=g).to(cuda)
+        W_r = torch.randn(E, d, generator=g).to(cuda)
+        self.run = mm16.Moe16LayerRunner(mm16.Moe16Dev(self.gate, self.up, self.down, self.slot), W_r, k, nt)
+
+    def forward(self, **kw):
+        for t in (self.run.h, self.run.y, self.run.g, self.run.u):
+            if t is not None:
+                t.fill_(float("nan"))
+        return self.run.forward(self.x, **kw).clone()
+
+
+@pytest.mark.parametrize("nt", [1, 2, 20, 300])
+def test_runner_reads_the_slot_table_each_time(cuda, nt):
+    """an expert that leaves after the runner was made adds nothing: as one whose down matrix is zeros; the next call has it
+    again.  Eager and replayed."""
+    full, R = _Runner(cuda, nt), _Runner(cuda, nt)
+    want = full.forward()
+    gone = _Runner(cuda, nt, without=(2, 3, 5)).forward()
+    assert not torch.equal(want, gone) or nt < 20
+    assert torch.equal(R.forward(), want)
+    out_of = torch.tensor([0, 1, -1, 8, 4, 1 << 30, 6, 7], dtype=torch.int32, device=cuda)
+    back = torch.arange(8, dtype=torch.int32, device=cuda)
+    R.slot.copy_(out_of)
+    assert torch.equal(R.forward(), gone)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        out = R.run.forward(R.x)
+    for table, w in ((back, want), (out_of, gone), (back, want)):
+        R.slot.copy_(table)
+        R.run.y.fill_(float("nan"))
+        R.run.h.fill_(float("nan"))
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+        assert torch.equal(R.forward(), w)
+
+
+@pytest.mark.parametrize("nt", [1, 20, 300])
+def test_runner_backward_with_the_slot_table_of_its_forward(cuda, nt):
+    """experts that are away in forward have no part in the gradients and get zeros; tables that change between the two passes
+    change nothing.  Against experts whose down matrix is zeros, which only differ in that matrix's own gradient."""
+    R, Z = _Runner(cuda, nt), _Runner(cuda, nt, without=(2, 5))
+    Z.forward(keep=True)
+    want = Z.run.backward(Z.dy)
+    for e in (2, 5):
+        want["down"][e] = 0
+    R.forward(keep=True)
+    R.slot[2] = -1
+    R.slot[5] = 8
+    R.forward(keep=True)
+    for change in (None, (2, 2), (0, -1), (slice(None), -1)):
+        if change:
+            R.slot[change[0]] = change[1]
+        got = R.run.backward(R.dy)
+        for name, w in want.items():
+            assert torch.equal(got[name], w), (name, change)
