@@ -279,25 +279,44 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Gro
     gi = __builtin_amdgcn_readfirstlane(s_out[4]);
     return true;
 }
-// The pairs of local expert `le` (TN), found by the whole block; cnt 0 when it has none
+// The pairs of local matrix `le` (TN), found by the whole block; cnt 0 when it has none.  Start -1: the pairs of several groups
+// (experts that share a matrix) one after the other.
 template <int NTH> __device__ __forceinline__ Group find_expert(const MMArgs &a, int le) {
     if (!a.egrp) return Group{0, 0, a.K};
-    __shared__ int s_g[2];
-    if (threadIdx.x == 0) { s_g[0] = 0; s_g[1] = 0; }
+    __shared__ int s_n, s_start, s_cnt;
+    if (threadIdx.x == 0) { s_n = 0; s_start = 0; s_cnt = 0; }
     __syncthreads();
     const int ng = n_groups(a);
     for (int i = threadIdx.x; i < ng; i += NTH) {
         const Group g = load_group(a, i);
-        if (g.cnt && g.le == le) { s_g[0] = g.start; s_g[1] = g.cnt; }
+        if (g.cnt && g.le == le) {
+            atomicAdd(&s_n, 1);
+            atomicAdd(&s_cnt, g.cnt);
+            s_start = g.start;   // (used where one group writes it)
+        }
     }
     __syncthreads();
-    return Group{le, s_g[0], s_g[1]};
+    const int n = __builtin_amdgcn_readfirstlane(s_n), cnt = __builtin_amdgcn_readfirstlane(s_cnt);
+    return Group{le, n > 1 ? -1 : __builtin_amdgcn_readfirstlane(s_start), (int) min((uint32_t) cnt, (uint32_t) a.n_pairs)};
 }
 // pair (or plain row) number i of a group; -1 for an entry outside the pairs
 __device__ __forceinline__ int pair_of(const MMArgs &a, const Group &g, int i) {
     if (!a.order) return g.start + i;
     const int p = a.order[g.start + i];
     return (uint32_t) p < (uint32_t) a.n_pairs ? p : -1;
+}
+// the same of find_expert's group
+__device__ __forceinline__ int pair_of_expert(const MMArgs &a, const Group &g, int i) {
+    if (!a.order || g.start >= 0) return pair_of(a, g, i);
+    const int ng = n_groups(a);
+#pragma unroll 1
+    for (int j = 0; j < ng; ++j) {
+        const Group o = load_group(a, j);
+        if (!o.cnt || o.le != g.le) continue;
+        if (i < o.cnt) return pair_of(a, o, i);
+        i -= o.cnt;
+    }
+    return -1;
 }
 
 // Blocks b, b + 8, .. run on one XCD, whose L2 they share: XCD x gets the tiles from x / 8 of the T tiles on.  -1: no tile.

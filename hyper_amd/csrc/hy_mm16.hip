@@ -44,7 +44,7 @@ template <typename T, int KIND, bool DUAL> __global__ __launch_bounds__(256) voi
         for (int k0 = 0; k0 < K; k0 += BK) {
             T pv[8], qv[8];
             if constexpr (KIND == TN) {
-                const int kk = k0 + (tid >> 3), p = kk < K ? pair_of(a, g, kk) : -1;
+                const int kk = k0 + (tid >> 3), p = kk < K ? pair_of_expert(a, g, kk) : -1;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int r = r0 + (tid & 7) * 8 + i, c = c0 + (tid & 7) * 8 + i;

@@ -142,7 +142,7 @@ __device__ __forceinline__ void mm_tile(const MMArgs &a, const Group &g, int r0,
         if constexpr (KIND == TN) {
             if (!a.order) return;
             for (int i = tid; i < CH; i += NTH) {
-                const int k = chunk * CH + i, p = k < K ? pair_of(a, g, k) : -1;
+                const int k = chunk * CH + i, p = k < K ? pair_of_expert(a, g, k) : -1;
                 s_look[(chunk & 1) * CH + i] = p < 0 ? -1 : div_k(p, a.kp);
                 s_look[(2 + (chunk & 1)) * CH + i] = p < 0 ? -1 : div_k(p, a.kq);
             }

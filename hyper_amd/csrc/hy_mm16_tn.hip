@@ -116,7 +116,7 @@ template <typename T, bool F32> __global__ __launch_bounds__(256, 1) void k_grad
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, wp = wave & 1, wq = wave >> 1;
     for (int i = tid; i < nstage * BK; i += 256) {   // the pairs' rows; -1: none
-        const int p = i < K ? pair_of(a, g, i) : -1;
+        const int p = i < K ? pair_of_expert(a, g, i) : -1;
         s_look[i] = p < 0 ? -1 : div_k(p, a.kp);
         s_look[PAIRS + i] = p < 0 ? -1 : div_k(p, a.kq);
     }

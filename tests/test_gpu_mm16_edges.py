@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from hyper_amd import mm16
+from hyper_amd import mm16, moe
 from tests.helpers import gen
 from tests.test_gpu_mm16 import TYPES, act64, same
 
@@ -274,3 +274,39 @@ def test_runner_backward_with_the_slot_table_of_its_forward(cuda, nt):
         got = R.run.backward(R.dy)
         for name, w in want.items():
             assert torch.equal(got[name], w), (name, change)
+
+
+# T, d, E, experts that share a matrix, k, ff: the element-wise kernel, tiles by pairs, blocks that go through a group's tiles, long groups
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,d,E,same_as,k,ff", [(9, 33, 6, {4: 1}, 2, 17), (40, 72, 8, {5: 0, 6: 0, 7: 2}, 3, 40), (700, 136, 5, {3: 2}, 2, 264), (700, 264, 130, {7: 3, 129: 3, 64: 65}, 4, 264),
+                                                (2000, 264, 130, {e: 1 for e in range(2, 60)}, 4, 264), (3000, 72, 3, {1: 0, 2: 0}, 2, 40)])
+def test_weight_gradients_of_shared_matrices(cuda, dtype, T, d, E, same_as, k, ff):
+    """experts that share a local matrix: its gradient is the sum over the pairs of them all, the same every time"""
+    g = gen(T + E)
+    slot = torch.full((E,), -1, dtype=torch.int32)
+    nl = 0
+    for e in range(E):
+        if e not in same_as:
+            slot[e], nl = nl, nl + 1
+    for e, o in same_as.items():
+        slot[e] = slot[o]
+    P = T * k
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).reshape(-1).to(torch.int32)
+    r = lambda *s: torch.randint(-3, 4, s, generator=g).to(dtype)  # noqa: E731
+    a, b, w = r(P, ff), r(T, d), torch.zeros(nl, ff, d, dtype=dtype, device=cuda)
+    m = mm16.Moe16Dev(w, w, None, slot.to(cuda))
+    i32 = dict(dtype=torch.int32, device=cuda)
+    order, order_n, egrp = torch.zeros(P, **i32), torch.zeros(2, **i32), torch.zeros(3 * E, **i32)
+    moe.moe_order(m, ids.to(cuda), P, E, order, order_n, None, egrp)
+    le, tok = slot[ids.long()].long(), torch.arange(P) // k
+    want = torch.zeros(nl, ff, d, dtype=torch.float64)
+    for e in range(nl):
+        p = (le == e).nonzero().view(-1)
+        want[e] = a[p].double().t() @ b[tok[p]].double()
+    for out_t in (torch.float32, dtype):
+        dW = torch.full((nl, ff, d), 77.0, dtype=out_t, device=cuda)
+        mm16.moe16_dw(m, a.to(cuda), 1, b.to(cuda), k, P, order, order_n, egrp, min(E, P), dW)
+        same(dW, want, f"{out_t}")
+        again = torch.empty_like(dW)
+        mm16.moe16_dw(m, a.to(cuda), 1, b.to(cuda), k, P, order, order_n, egrp, min(E, P), again)
+        assert torch.equal(again, dW)
