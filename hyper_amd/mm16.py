@@ -296,7 +296,8 @@ def moe16_gate_up_dx(m: Moe16Dev, dg, du, n_pairs, order, order_n, egrp, max_act
 
 
 def moe16_dw(m: Moe16Dev, a, ka, b, kb, n_pairs, order, order_n, egrp, max_active, dW, accumulate=False, stream=None):
-    """dW[slot[e]] = sum over e's pairs of a[p // ka]^T b[p // kb], [n_local, rows, cols]; zeros for experts without pairs."""
+    """dW[slot[e]] = sum over e's pairs of a[p // ka]^T b[p // kb], [n_local, rows, cols]; zeros for a matrix without pairs,
+    the sum of them all where experts share one."""
     ty, rows, cols = _type16(a), a.shape[-1], b.shape[-1]
     lda = _mat("a", a, (n_pairs + ka - 1) // max(ka, 1), rows, least=True)
     ldb = _mat("b", b, (n_pairs + kb - 1) // max(kb, 1), cols, a.dtype, least=True)

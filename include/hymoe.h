@@ -354,8 +354,8 @@ int hy_moe16_reduce(const hy_moe_dev *m, const float *shexp, const float *sg, co
      hy_moe16_down_dx     dh[p] = dy[p / k] down_e (not yet weighted), [n_pairs][ff]
      hy_swiglu_bwd        from g, u, dh: dwts[p] = sum dh h,  hw = wts h,  dg, du of wts dh       (wts NULL: 1)
      hy_moe16_gate_up_dx  dx[p] = dg[p] gate_e + du[p] up_e, [n_pairs][n]; hy_moe_reduce (hy_moe16_reduce) sums a token's pairs
-     hy_moe16_dw          dW[slot[e]] = sum over e's pairs of a[p / ka]^T b[p / kb], [n_local][rows][cols] (zeros for an
-                          expert without pairs): gate from (dg, x), up from (du, x), down from (dy, hw)
+     hy_moe16_dw          dW[slot[e]] = sum over e's pairs of a[p / ka]^T b[p / kb], [n_local][rows][cols] (zeros for a
+                          matrix without pairs; experts that share one are summed): gate from (dg, x), up from (du, x), down from (dy, hw)
    hy_swiglu_bwd takes all n_pairs rows, or with order and order_n the pairs listed there; hw and dwts may be NULL; dg, du
    and hw may each be one of g, u, dh.  Where g (u) lies beyond the clamp its gradient is 0. */
 int hy_moe16_down_dx(const hy_moe_dev *m, const void *dy, int64_t lddy, int k, int n_pairs, const int32_t *order, const int32_t *order_n,
