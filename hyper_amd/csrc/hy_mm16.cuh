@@ -282,7 +282,7 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Gro
 // The pairs of local matrix `le` (TN), found by the whole block; cnt 0 when it has none.  Start -1: the pairs of several groups
 // (experts that share a matrix) one after the other.
 template <int NTH> __device__ __forceinline__ Group find_expert(const MMArgs &a, int le) {
-    if (!a.egrp) return Group{0, 0, a.K};
+    if (!a.egrp) return Group{le, 0, a.K};   // (experts without any pairs: K = 0)
     __shared__ int s_n, s_start, s_cnt;
     if (threadIdx.x == 0) { s_n = 0; s_start = 0; s_cnt = 0; }
     __syncthreads();

@@ -150,7 +150,7 @@ template <typename T> static int launch_any(int kind, bool dual, const MMArgs &a
     const int64_t blocks = ncol * items;
     if (blocks <= 0) return HY_OK;
     if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
-    const dim3 grid((uint32_t) blocks, kind == TN && a.egrp ? (uint32_t) a.n_local : 1u);
+    const dim3 grid((uint32_t) blocks, kind == TN ? (uint32_t) std::max(1, a.n_local) : 1u);
     if (kind == NT) {
         if (dual) k_mm_any<T, NT, true><<<grid, 256, 0, s>>>(a);
         else k_mm_any<T, NT, false><<<grid, 256, 0, s>>>(a);

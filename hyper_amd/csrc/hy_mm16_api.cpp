@@ -58,10 +58,11 @@ static int check_k(const char *what, int k) {
     if (k < 1 || k > 64) { set_error("%s: k = %d pairs a row (1 .. 64)", what, k); return HY_EBAD_SHAPE; }
     return HY_OK;
 }
-// the pairs' grouping: order, order_n and egrp of hy_moe_order
+// the pairs' grouping: order, order_n and egrp of hy_moe_order (without pairs nothing reads it: empty arrays have no address)
 static int check_groups(const char *what, int n_pairs, const int32_t *order, const int32_t *order_n, const int32_t *egrp, int max_active) {
     if (n_pairs < 0) { set_error("%s: %d pairs", what, n_pairs); return HY_EINVAL; }
     if (n_pairs > HY_MM_MAX) { set_error("%s: %d pairs (up to 2^30)", what, n_pairs); return HY_EBAD_SHAPE; }
+    if (n_pairs == 0) return HY_OK;
     if (!order || !order_n || !egrp) { set_error("%s: order, order_n and egrp are needed", what); return HY_EINVAL; }
     if (misaligned(order, 4) || misaligned(order_n, 4) || misaligned(egrp, 4)) { set_error("%s: order, order_n and egrp must be 4-byte aligned", what); return HY_EBAD_SHAPE; }
     if (max_active < 1 || max_active > 1024) { set_error("%s: max_active %d (1 .. 1024)", what, max_active); return HY_EBAD_SHAPE; }
@@ -72,6 +73,7 @@ static int check_pairs(const char *what, int n_pairs, const int32_t *ids, const 
                        int max_active) {
     if (order) return check_groups(what, n_pairs, order, order_n, egrp, max_active);
     if (n_pairs < 0) { set_error("%s: %d pairs", what, n_pairs); return HY_EINVAL; }
+    if (n_pairs == 0) return HY_OK;
     if (!ids) { set_error("%s: ids or order is needed", what); return HY_EINVAL; }
     if (misaligned(ids, 4)) { set_error("%s: ids must be 4-byte aligned", what); return HY_EBAD_SHAPE; }
     if (n_pairs > 65535) { set_error("%s: %d pairs by ids (up to 65535: group them with hy_moe_order)", what, n_pairs); return HY_EBAD_SHAPE; }
@@ -85,6 +87,7 @@ static MMArgs moe_args(const hy_moe_dev *m, int n_pairs, const int32_t *ids, con
     a.n_expert = m->n_expert;
     a.n_pairs = n_pairs;
     a.pstride = (int64_t) m->ff * m->n;
+    if (n_pairs == 0) return a;   // (gradients of no pairs: zeros)
     if (order) { a.order = order; a.order_n = order_n; a.egrp = egrp; a.max_active = max_active; }
     else a.ids = ids;
     return a;

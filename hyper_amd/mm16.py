@@ -219,8 +219,8 @@ def _groups(n_pairs, ids, order, order_n, egrp, max_active):
             _vec("ids", ids, n_pairs, torch.int32)
         return
     _vec("order", order, n_pairs, torch.int32)
-    _vec("order_n", order_n, 2, torch.int32)
-    _vec("egrp", egrp, 3 * max_active, torch.int32)
+    _vec("order_n", order_n, 2 if n_pairs else 0, torch.int32)   # (no pairs: nothing reads them)
+    _vec("egrp", egrp, 3 * max_active if n_pairs else 0, torch.int32)
 
 
 def _pairs(name, t, rows, cols, *dtypes):

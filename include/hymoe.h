@@ -337,8 +337,8 @@ int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t 
    [n_local][ff][n] and down [n_local][n][ff], gate_bytes = down_bytes = 2 ff n, ff and n of any size (hy_upload_experts
    copies them from GGUF rows as they are).  hy_moe_order takes the same descriptor.  Pairs p = t k + j: either grouped by
    order, order_n, egrp of hy_moe_order (max_active >= order_n[1], at most 1024), or, with order NULL, each by its expert
-   ids[p] (single tokens: every pair reads its expert's matrices; up to 65535 pairs).  Rows of pairs whose expert is not
-   local are left as they were.
+   ids[p] (single tokens: every pair reads its expert's matrices; up to 65535 pairs).  With n_pairs 0 these arrays may be NULL.  Rows
+   of pairs whose expert is not local are left as they were.
    gate_up: h[p] = SwiGLU(gate_e x[p / k], up_e x[p / k]) with the descriptor's clamp, g and u on request as in
    hy_linear_glu; h, g, u [n_pairs][ff].  down: y[p] = wts[p] (down_e h[p]) (wts NULL: 1), [n_pairs][n]; with out_type
    HY_F32 hy_moe_reduce combines the rows, or, where experts may not be local, hy_moe16_reduce. */

@@ -310,3 +310,32 @@ def test_weight_gradients_of_shared_matrices(cuda, dtype, T, d, E, same_as, k, f
         again = torch.empty_like(dW)
         mm16.moe16_dw(m, a.to(cuda), 1, b.to(cuda), k, P, order, order_n, egrp, min(E, P), again)
         assert torch.equal(again, dW)
+
+
+# ------------------------------------------------------------------ empty calls
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,d,ff", [(3, 33, 17), (3, 64, 40), (130, 264, 264), (5, 520, 520)])
+def test_no_pairs(cuda, dtype, E, d, ff):
+    """empty tensors, a grouping of no entries: outputs of no rows, and gradients of zeros for every expert"""
+    e = lambda *s, dt=dtype: torch.empty(*s, dtype=dt, device=cuda)  # noqa: E731
+    w = torch.zeros(E, ff, d, dtype=dtype, device=cuda)
+    m = mm16.Moe16Dev(w, w, w.view(E, d, ff), torch.arange(E, dtype=torch.int32, device=cuda))
+    none = e(0, dt=torch.int32)
+    for grp in ((none, none, none, 0), (none, torch.zeros(2, dtype=torch.int32, device=cuda), torch.zeros(3 * E, dtype=torch.int32, device=cuda), E)):
+        kw = dict(order=grp[0], order_n=grp[1], egrp=grp[2], max_active=grp[3])
+        mm16.moe16_gate_up(m, e(0, d), 2, 0, e(0, ff), **kw)
+        mm16.moe16_gate_up(m, e(0, d), 2, 0, e(0, ff), ids=none)
+        mm16.moe16_down(m, e(0, ff), 0, e(0, d), **kw)
+        mm16.moe16_down(m, e(0, ff), 0, e(0, d), ids=none)
+        mm16.moe16_down_dx(m, e(0, d), 2, 0, *grp, e(0, ff))
+        mm16.moe16_gate_up_dx(m, e(0, ff), e(0, ff), 0, *grp, e(0, d))
+        mm16.swiglu_bwd(e(0, ff), e(0, ff), e(0, ff), None, e(0, ff), e(0, ff), e(0, ff), e(0, dt=torch.float32))
+        mm16.moe16_reduce(m, None, None, e(0, d, dt=torch.float32), 2, e(0, d, dt=torch.float32), 0, none)
+        for out_t in (dtype, torch.float32):
+            buf = torch.full((E * ff * d + 8,), 5.0, dtype=out_t, device=cuda)
+            dW = buf[:E * ff * d].view(E, ff, d)
+            mm16.moe16_dw(m, e(0, ff), 1, e(0, d), 2, 0, *grp, dW, accumulate=True)
+            assert (buf == 5.0).all()
+            mm16.moe16_dw(m, e(0, ff), 1, e(0, d), 2, 0, *grp, dW)
+            assert (dW == 0).all() and (buf[E * ff * d:] == 5.0).all()
