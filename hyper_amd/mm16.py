@@ -365,7 +365,7 @@ class Moe16LayerRunner:
         self.sh_y = new(T, self.d, dtype=torch.float32) if shared is not None else None
         self.sh_h = new(T, shared.ff) if shared is not None else None
         self.g = self.u = self.kept_dev = None
-        self.kept = 0
+        self.kept = None   # rows of the last forward(keep=True); None: there was another one since, or none
 
     def _rows(self, x):
         if x.dim() != 2 or x.shape[1] != self.d or x.dtype != torch.float32 or x.device != self.W_r.device:
@@ -384,21 +384,22 @@ class Moe16LayerRunner:
         """The layer's output [nt, d] (a view of the runner's buffer) for nt rows; keep=True: also what backward needs."""
         nt, k = self._rows(x), self.k
         P = nt * k
-        self.kept = 0
-        if nt == 0:
-            return self.out[:0]
+        self.kept = None
         device = self.W_r.device
         stream = stream if stream is not None else torch.cuda.current_stream(device)
         with torch.cuda.stream(stream):
+            if keep and self.g is None:
+                self.g, self.u = torch.empty_like(self.h), torch.empty_like(self.h)
+                self.kept_dev = Moe16Dev(self.dev.gate, self.dev.up, self.dev.down, torch.empty_like(self.dev.slot), self.dev.clamp)
+            if nt == 0:
+                self.kept = 0 if keep else None
+                return self.out[:0]
             moe.gemv_f32(self.W_r, self.E, self.d, x, x.stride(0), self.logits, self.E, nt, stream)
             moe.moe_route(self.logits, self.E, self.E, k, self.ids, self.wts, None, nt, stream)
             rows16(x, self.x16[:nt], stream)
             how = dict(ids=self.ids) if nt <= self.decode_rows and not keep else self._group(nt, stream)
             gu = {}
             if keep:
-                if self.g is None:
-                    self.g, self.u = torch.empty_like(self.h), torch.empty_like(self.h)
-                    self.kept_dev = Moe16Dev(self.dev.gate, self.dev.up, self.dev.down, torch.empty_like(self.dev.slot), self.dev.clamp)
                 gu = dict(g=self.g, u=self.u)
                 torch.add(self.dev.slot, 0, out=self.kept_dev.slot)   # (a kernel: no copy node in a captured graph)
             moe16_gate_up(self.dev, self.x16[:nt], k, P, self.h, **how, **gu, stream=stream)
@@ -408,14 +409,14 @@ class Moe16LayerRunner:
                 linear_glu(S.gate[0], S.up[0], self.x16[:nt], self.sh_h[:nt], clamp=S.clamp, stream=stream)
                 linear(S.down[0], self.sh_h[:nt], self.sh_y[:nt], stream=stream)
             moe16_reduce(self.dev, self.sh_y, None, self.y, k, self.out, nt, self.ids, stream)
-        self.kept = nt if keep else 0
+        self.kept = nt if keep else None
         return self.out[:nt]
 
     def backward(self, dy: torch.Tensor, stream=None) -> dict:
         """Gradients of the routed experts for the last forward(keep=True): dy [nt, d] float32 -> {"dx": [nt, d] float32 (the
         experts' part), "dwts": [nt, k] (of the routing weights), "gate", "up", "down": float32}."""
         nt, k = self._rows(dy), self.k
-        if not self.kept or nt != self.kept:
+        if nt != self.kept:
             raise ValueError("backward follows forward(keep=True) of the same rows")
         if not self.all_local:
             raise ValueError("backward needs every expert local")

@@ -339,3 +339,28 @@ def test_no_pairs(cuda, dtype, E, d, ff):
             assert (buf == 5.0).all()
             mm16.moe16_dw(m, e(0, ff), 1, e(0, d), 2, 0, *grp, dW)
             assert (dW == 0).all() and (buf[E * ff * d:] == 5.0).all()
+
+
+def test_runner_without_rows(cuda):
+    """a step of no rows has gradients: zeros.  They belong to the last forward, which kept something or not"""
+    R = _Runner(cuda, 20)
+    with pytest.raises(ValueError, match="follows"):
+        R.run.backward(R.dy[:0])
+    for before in (False, True):
+        if before:
+            R.forward(keep=True)
+        assert R.run.forward(R.x[:0], keep=True).shape == (0, 64)
+        got = R.run.backward(R.dy[:0])
+        assert got["dx"].shape == (0, 64) and got["dwts"].shape == (0, 2)
+        for name, t in (("gate", R.gate), ("up", R.up), ("down", R.down)):
+            assert got[name].shape == t.shape and (got[name] == 0).all()
+        with pytest.raises(ValueError, match="follows"):
+            R.run.backward(R.dy)
+        R.run.forward(R.x[:0])
+        with pytest.raises(ValueError, match="follows"):
+            R.run.backward(R.dy[:0])
+    R.forward(keep=True)
+    first = R.run.backward(R.dy)
+    R.forward(keep=True)
+    again = R.run.backward(R.dy)
+    assert all(torch.equal(first[n], again[n]) for n in first)
