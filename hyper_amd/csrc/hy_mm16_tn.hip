@@ -240,6 +240,7 @@ Parts dw_parts(int m, int n, int k) {
     constexpr TileCost cut{128, 128, 512, 0.66f, 0.75f, 0.95f, 5.0f};   // (a stage of parts reads less)
     MMArgs a{};
     a.R = n; a.N = k; a.K = m;
+    if (n % 8 || k % 8) return Parts{1, m};   // rows that are not whole 16-byte pieces: k_mm_any, which goes through them uncut
     float least = tile_cost(TILES[cheapest(TILES, a, TN, false)], a, TN, false);
     Parts best{1, m};
     for (int p = 2; p <= 32; p *= 2) {

@@ -327,8 +327,8 @@ int hy_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy, in
 int hy_linear_dx(int type, const void *W, int64_t ldw, int n, int k, const void *dz, int64_t lddz, int m, const void *resid, int64_t ldr,
                  void *dx, int out_type, int64_t lddx, hipStream_t s);
 /* dW = dz^T x [n][k] and db[r] = sum of dz[i][r] (NULL: none), added to what is there with accumulate != 0.  m = 0 gives
-   zeros.  ws: at least hy_linear_dw_ws_bytes(m, n, k) bytes (which may be 0), 16-byte aligned, for calls on one stream;
-   nothing in it is kept between calls. */
+   zeros.  ws: at least hy_linear_dw_ws_bytes(m, n, k) bytes (which may be 0, and is 0 where n or k is no multiple of 8), 16-byte
+   aligned, for calls on one stream; nothing in it is kept between calls. */
 size_t hy_linear_dw_ws_bytes(int m, int n, int k);
 int hy_linear_dw(int type, const void *dz, int64_t lddz, const void *x, int64_t ldx, int m, int n, int k, void *dW, int out_type,
                  int64_t lddw, float *db, int accumulate, void *ws, size_t ws_bytes, hipStream_t s);
