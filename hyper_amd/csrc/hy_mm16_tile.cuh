@@ -8,9 +8,9 @@
 namespace hy {
 
 // 16 bytes a lane from per-lane addresses to 1 KB of LDS at `lds` (lane l's bytes at lds + 16 l), in flight when it returns.
-// M0 holds the LDS address; the compiler uses M0 only within sequences of its own, which set it themselves.
+// M0 holds the LDS address (named as overwritten, so that the compiler keeps nothing of its own there).
 __device__ __forceinline__ void dma16(const char *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 template <typename V> __device__ __forceinline__ V lds_get(uint32_t addr) { return *(const __attribute__((address_space(3))) V *) (uintptr_t) addr; }
 // what the wave's lanes wrote to LDS before is what its lanes read behind (LDS operations of a wave keep their order; this
