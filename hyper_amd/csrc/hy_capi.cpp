@@ -325,11 +325,13 @@ int hy_moe_gemm_down(const hy_moe_dev *m, const void *hq, int n_pairs, const int
 
 int hy_moe_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int32_t *ids, hipStream_t s) {
     if (!y || !out || !ids || k <= 0 || k > 64 || n <= 0 || nt < 0) { set_error("hy_moe_reduce: bad argument"); return HY_EINVAL; }
+    if (nt >= 1 << 24) { set_error("hy_moe_reduce: %d tokens (a launch of 256 threads each takes less than 2^24)", nt); return HY_EBAD_SHAPE; }
     return launch_reduce(shexp, sg, y, k, out, n, nt, ids, s);
 }
 int hy_moe_reduce_residual(const float *shexp, const float *sg, const float *y, int k, float *resid, int n, int nt, const int32_t *ids,
                            hipStream_t s) {
     if (!y || !resid || !ids || k <= 0 || k > 64 || n <= 0 || nt < 0) { set_error("hy_moe_reduce_residual: bad argument"); return HY_EINVAL; }
+    if (nt >= 1 << 24) { set_error("hy_moe_reduce_residual: %d tokens (a launch of 256 threads each takes less than 2^24)", nt); return HY_EBAD_SHAPE; }
     return launch_reduce(shexp, sg, y, k, resid, n, nt, ids, s, 1);
 }
 

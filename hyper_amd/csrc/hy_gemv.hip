@@ -209,13 +209,14 @@ int launch_down(const hy_moe_dev &m, const float *h, const int *ids, const float
 // per token: wave 0 ranks the token's pairs (rank = valid pairs with a smaller id, ties by position), then every
 // thread sums VW consecutive columns per pass (VW = 4: 16-byte loads when n and the rows allow it).  LOCAL: pairs whose
 // expert the slot table does not hold are left out too.
-struct SlotTable { const int *slot; int n_expert, n_local; };
+struct SlotTable { const int *slot; int n_expert, n_local, nt; };   // (nt: the tokens, where the grid has rows of them)
 template <int VW, bool LOCAL>
 __global__ __launch_bounds__(256) void k_reduce(const float *__restrict__ shexp, const float *__restrict__ sg, const float *__restrict__ y,
                                                 int k, float *__restrict__ out, int n, const int *__restrict__ ids, int res, SlotTable tab) {
     __shared__ int ord[64];
     __shared__ int s_cnt;
-    const int t = blockIdx.x, tid = threadIdx.x;
+    const int t = LOCAL ? (int) (blockIdx.y * gridDim.x + blockIdx.x) : (int) blockIdx.x, tid = threadIdx.x;
+    if (LOCAL && t >= tab.nt) return;
     if (tid < 64) {
         int e = tid < k ? ids[(size_t) t * k + tid] : -1;
         if constexpr (LOCAL) {
@@ -275,8 +276,9 @@ static int launch_reduce_t(const float *shexp, const float *sg, const float *y, 
                            const SlotTable &tab, const char *what) {
     if (nt == 0) return HY_OK;
     const bool vec = n % 4 == 0 && ((uintptr_t) y & 15) == 0 && ((uintptr_t) out & 15) == 0 && ((uintptr_t) shexp & 15) == 0;
-    if (vec) k_reduce<4, LOCAL><<<dim3(nt), dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
-    else k_reduce<1, LOCAL><<<dim3(nt), dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
+    const dim3 grid(LOCAL ? std::min(nt, 1 << 22) : nt, LOCAL ? (nt + (1 << 22) - 1) >> 22 : 1);   // (a launch counts its threads in each direction in 32 bits)
+    if (vec) k_reduce<4, LOCAL><<<grid, dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
+    else k_reduce<1, LOCAL><<<grid, dim3(256), 0, s>>>(shexp, sg, y, k, out, n, ids, res, tab);
     return check_launch(what);
 }
 int launch_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int *ids, hipStream_t s, int res) {
@@ -284,7 +286,7 @@ int launch_reduce(const float *shexp, const float *sg, const float *y, int k, fl
 }
 int launch_reduce_local(const hy_moe_dev &m, const float *shexp, const float *sg, const float *y, int k, float *out, int nt, const int *ids,
                         hipStream_t s) {
-    return launch_reduce_t<true>(shexp, sg, y, k, out, m.n, nt, ids, s, 0, SlotTable{m.slot, m.n_expert, m.n_local}, "hy_moe16_reduce");
+    return launch_reduce_t<true>(shexp, sg, y, k, out, m.n, nt, ids, s, 0, SlotTable{m.slot, m.n_expert, m.n_local, nt}, "hy_moe16_reduce");
 }
 
 // ---------------------------------------------------------------- fused decode down + combine

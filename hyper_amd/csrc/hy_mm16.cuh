@@ -375,6 +375,13 @@ template <int NTH, int BM> __device__ __forceinline__ bool find_tile(const MMArg
     return true;
 }
 
+// A launch of 2^32 threads or more runs those that 32 bits count and reports nothing: such grids (of blocks of 256) are refused.
+inline __host__ int check_blocks(const char *what, int64_t blocks) {
+    if (blocks < 1 << 24) return HY_OK;
+    set_error("%s: %lld tiles of the output (a call takes less than 2^24)", what, (long long) blocks);
+    return HY_EBAD_SHAPE;
+}
+
 // launchers (type: HY_F16 / HY_BF16)
 int launch_mm(int kind, int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);
 int launch_tiles_nt(int type, bool dual, const MMArgs &a, hipStream_t s, const char *what);

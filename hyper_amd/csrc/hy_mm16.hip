@@ -149,7 +149,7 @@ template <typename T> static int launch_any(int kind, bool dual, const MMArgs &a
     const int64_t items = kind == TN || !a.egrp ? (a.R + 63) / 64 : (a.n_pairs + 63) / 64 + a.max_active;
     const int64_t blocks = ncol * items;
     if (blocks <= 0) return HY_OK;
-    if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
+    if (const int rc = check_blocks(what, blocks)) return rc;
     const dim3 grid((uint32_t) blocks, kind == TN ? (uint32_t) std::max(1, a.n_local) : 1u);
     if (kind == NT) {
         if (dual) k_mm_any<T, NT, true><<<grid, 256, 0, s>>>(a);

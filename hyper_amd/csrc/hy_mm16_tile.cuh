@@ -476,7 +476,7 @@ static int launch_tile(MMArgs a, hipStream_t s, const char *what) {
     const int64_t per = (ncol * items + 7) / 8;   // tiles of an XCD
     const int64_t blocks = a.split > 1 ? 8 * ((per & ~31ll) + (per & 31) * a.split) : a.spread ? (ncol + 7) / 8 * 8 * items : ncol * items;   // an XCD has at most ncol / 8, rounded up, of a group's columns
     if (blocks <= 0) return HY_OK;
-    if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
+    if (const int rc = check_blocks(what, blocks)) return rc;
     k_mm<T, KIND, DUAL, BM, BN, WP, WQ, NST><<<dim3((uint32_t) blocks, KIND == TN ? (uint32_t) (a.parts > 1 ? a.parts : std::max(1, a.n_local)) : 1u), 64 * WP * WQ, 0, s>>>(a);
     return check_launch(what);
 }

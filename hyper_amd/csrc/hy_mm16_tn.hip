@@ -226,7 +226,7 @@ template <typename T> static int launch_gradients(const MMArgs &a, hipStream_t s
     const int64_t blocks = a.n_local * rows * ncol;
     // (8 tiles a block: as fast where the pairs are even, 330 for 187 us where they are spread as 1 / rank^1.1; 2 tiles: 172 for 152)
     const int nct = (int) std::min<int64_t>(std::clamp<int64_t>(blocks / 256, 1, 4), ncol);
-    if (blocks > 0x7fffffffll) { set_error("%s: %lld tiles", what, (long long) blocks); return HY_EBAD_SHAPE; }
+    if (const int rc = check_blocks(what, blocks)) return rc;
     if (a.out_f32) k_gradients<T, true><<<(uint32_t) blocks, 256, 0, s>>>(a, nct);
     else k_gradients<T, false><<<(uint32_t) blocks, 256, 0, s>>>(a, nct);
     return check_launch(what);

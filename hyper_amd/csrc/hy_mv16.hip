@@ -23,8 +23,9 @@ template <typename T, bool AL> __device__ __forceinline__ v8<T> ld8(const T *row
 template <typename T, bool DUAL, int NR, bool AL> __global__ __launch_bounds__(256) void k_mv(const MMArgs a) {
     constexpr int CW = DUAL ? 1 : 2;
     const int lane = threadIdx.x & 63;
-    const int c0 = ((int) blockIdx.x * 4 + (int) (threadIdx.x >> 6)) * CW;
-    if (c0 >= a.N) return;
+    const int64_t col = ((int64_t) blockIdx.z * gridDim.x + blockIdx.x) * (4 * CW) + (threadIdx.x >> 6) * CW;
+    if (col >= a.N) return;
+    const int c0 = (int) col;
     int le = 0, row0 = 0, out0 = 0, nr = a.R;
     if (a.ids) {
         const int p = blockIdx.y, e = a.ids[p];
@@ -90,6 +91,8 @@ template <typename T, bool DUAL, int NR, bool AL> __global__ __launch_bounds__(2
     }
 }
 
+constexpr uint32_t MAX_ROW = 1 << 22;   // blocks in a row of the grid (a launch counts its threads in each direction in 32 bits)
+
 template <typename T, bool DUAL, bool AL> static void mv_rows(const MMArgs &a, dim3 grid, hipStream_t s) {
     const int nr = a.ids ? 1 : a.R;
     if (nr == 1) k_mv<T, DUAL, 1, AL><<<grid, 256, 0, s>>>(a);
@@ -99,7 +102,8 @@ template <typename T, bool DUAL, bool AL> static void mv_rows(const MMArgs &a, d
 template <typename T> static int launch_mv_t(bool dual, const MMArgs &a, hipStream_t s, const char *what) {
     const bool al = a.K % 8 == 0 && a.ldp % 8 == 0 && a.ldq % 8 == 0 && a.pstride % 8 == 0 &&
                     (((uintptr_t) a.P | (uintptr_t) a.P2 | (uintptr_t) a.Q) & 15) == 0;
-    const dim3 grid((uint32_t) (dual ? (a.N + 3) / 4 : (a.N + 7) / 8), a.ids ? (uint32_t) a.n_pairs : 1u);
+    const uint32_t blocks = (uint32_t) (dual ? (a.N + 3) / 4 : (a.N + 7) / 8), rows = (blocks + MAX_ROW - 1) / MAX_ROW;
+    const dim3 grid(std::min(blocks, MAX_ROW), a.ids ? (uint32_t) a.n_pairs : 1u, rows);
     if (dual) { if (al) mv_rows<T, true, true>(a, grid, s); else mv_rows<T, true, false>(a, grid, s); }
     else { if (al) mv_rows<T, false, true>(a, grid, s); else mv_rows<T, false, false>(a, grid, s); }
     return check_launch(what);
@@ -207,7 +211,7 @@ int launch_act_bwd(int type, int act, const void *z, int64_t ldz, const void *dy
 template <typename T, int V> __global__ __launch_bounds__(256) void k_swiglu_bwd(const T *g, const T *u, const T *dh, const float *wts,
                                                                                int n_pairs, int ff, float L, const int *order,
                                                                                const int *order_n, T *dg, T *du, T *hw, float *dwts) {
-    const int lane = threadIdx.x & 63, i = (int) blockIdx.x * 4 + (int) (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, i = (int) (blockIdx.y * gridDim.x + blockIdx.x) * 4 + (int) (threadIdx.x >> 6);
     int p = i;
     if (order) {
         if (i >= min(order_n[0], n_pairs)) return;
@@ -259,7 +263,8 @@ template <typename T> static int launch_swiglu_bwd_t(const void *g, const void *
                                                      float clamp, const int *order, const int *order_n, void *dg, void *du, void *hw,
                                                      float *dwts, hipStream_t s) {
     const bool v = ff % 8 == 0 && (((uintptr_t) g | (uintptr_t) u | (uintptr_t) dh | (uintptr_t) dg | (uintptr_t) du | (uintptr_t) hw) & 15) == 0;
-    const uint32_t grid = (uint32_t) ((n_pairs + 3) / 4);
+    const uint32_t blocks = (uint32_t) ((n_pairs + 3) / 4);
+    const dim3 grid(std::min(blocks, MAX_ROW), (blocks + MAX_ROW - 1) / MAX_ROW);
     if (v) k_swiglu_bwd<T, 8><<<grid, 256, 0, s>>>((const T *) g, (const T *) u, (const T *) dh, wts, n_pairs, ff, clamp, order, order_n, (T *) dg, (T *) du, (T *) hw, dwts);
     else k_swiglu_bwd<T, 1><<<grid, 256, 0, s>>>((const T *) g, (const T *) u, (const T *) dh, wts, n_pairs, ff, clamp, order, order_n, (T *) dg, (T *) du, (T *) hw, dwts);
     return check_launch("hy_swiglu_bwd");

@@ -350,6 +350,8 @@ class Moe16LayerRunner:
             raise ValueError(f"W_r must be a contiguous fp32 or bf16 [{dev.slot.numel()}, {dev.n}] matrix, got {W_r.dtype} {tuple(W_r.shape)}")
         if dev.n % 4:
             raise ValueError("the router takes d_model in multiples of 4")
+        if max_rows >= 1 << 23 or -(-dev.slot.numel() // 16) * -(-max_rows // 8) >= 1 << 24:   # (a launch counts its threads in 32 bits)
+            raise ValueError(f"max_rows {max_rows} with {dev.slot.numel()} experts: more than the router takes in one launch")
         if shared is not None and (shared.gate is None or shared.down is None or shared.n != dev.n or shared.gate.dtype != dev.gate.dtype
                                    or shared.down.dtype != dev.gate.dtype):
             raise ValueError("the shared expert must have the experts' d_model and type")

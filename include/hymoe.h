@@ -301,7 +301,8 @@ int hy_block_ints(int type, const uint8_t *rows, size_t row_bytes, int nrows, co
    the nearest even value of the output's type (out_type: `type` or HY_F32).  Matrices are row-major; ld* is the number of
    elements between the rows (an input may repeat rows with 0).  Any size and any alignment to the values' own size is
    taken; rows of multiples of 8 values that start on 16 bytes are fastest.  Results do not depend on anything but the
-   arguments (no atomics).  Sizes up to HY_MM_MAX. */
+   arguments (no atomics).  Sizes up to HY_MM_MAX; products of more than four rows
+   whose output has 2^24 or more tiles (of 32 x 32 values or more each) are refused (HY_EBAD_SHAPE). */
 #define HY_F32 0
 #define HY_F16 1
 #define HY_BF16 30
