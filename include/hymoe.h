@@ -118,7 +118,8 @@ size_t hy_q8_row_bytes(int vtype, int n);
 
 /* Upload the experts with slot_host[e] >= 0 to their slots (replaces upload_experts, src/experts.h:50 /
    src/experts.cu:56-74), re-laid from GGUF rows into the tiled order above (ff and n multiples of 256, gb / db the
-   matrices' GGUF sizes).  Allocates gate/up/down and the slot table with hipMalloc; hy_free_experts releases. */
+   matrices' GGUF sizes); F16 and BF16 matrices of any size as plain rows, for the 16-bit products below.
+   Allocates gate/up/down and the slot table with hipMalloc; hy_free_experts releases. */
 int hy_upload_experts(const hy_expert_tensors *t, const int32_t *slot_host, int32_t ff, int32_t n, float clamp, hy_moe_dev *out);
 int hy_free_experts(hy_moe_dev *m);
 
@@ -192,8 +193,8 @@ int hy_moe_gemm_down(const hy_moe_dev *m, const void *hq, int n_pairs, const int
                      int max_active, const float *wts, float *y, hipStream_t s);
 
 /* Combine: out[t][r] = sg[t] * shexp[t][r] (when shexp; sg NULL: 1) + the pairs' y[t*k + j][r] added in ascending
-   expert-id order (without shexp the first pair is the start value); ids with a negative expert are skipped
-   (replaces moe_reduce, src/kernels4.cuh:88-91 / src/kernels4.cu:1182-1206, single device, no CPU owner). */
+   expert-id order (without shexp the first pair is the start value); ids with a negative expert are skipped;
+   nt < 2^24 (replaces moe_reduce, src/kernels4.cuh:88-91 / src/kernels4.cu:1182-1206, single device, no CPU owner). */
 int hy_moe_reduce(const float *shexp, const float *sg, const float *y, int k, float *out, int n, int nt, const int32_t *ids,
                   hipStream_t s);
 /* The combine written straight into the residual (the next row after moe_reduce, src/kernels4.cu:1182-1206: on one GPU
