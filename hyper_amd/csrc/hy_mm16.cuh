@@ -242,6 +242,8 @@ __device__ __forceinline__ int n_groups(const MMArgs &a) { return max(0, min(a.o
 // The group of this block's work item, found by the whole block of NTH threads: count(i, rows) is the number of items of group i;
 // every thread counts those of its few groups and a scan over the block places them.  place(total) says which of the `total`
 // items is the block's (below 0: none; the result is false then); `item` becomes its number within the group, gi the group's.
+// A group has fewer than 2^24 items (check_blocks).  Groups that overlap, as no hy_moe_order makes them, may have 2^34 in all: the
+// scan stops at 2^30, whose last 2^26 no block is placed at, so that at most one thread finds itself named.
 template <int NTH, typename C, typename F>
 __device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Group &g, int &item, int &gi) {
     constexpr int PER = 1024 / NTH;
@@ -258,14 +260,16 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Gro
         nt[j] = count(i, gs[j].cnt);
         sum += nt[j];
     }
+    auto plus = [](int a, int b) { return (int) min((uint32_t) a + (uint32_t) b, 1u << 30); };
     int inc = sum;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(inc, o); if (lane >= o) inc += v; }
+    for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(inc, o); if (lane >= o) inc = plus(inc, v); }
     if (lane == 63) s_w[tid >> 6] = inc;
+    if (tid == 0) s_out[2] = 0;
     __syncthreads();
     int pre = inc - sum, all = 0;
 #pragma unroll
-    for (int w = 0; w < NTH / 64; ++w) { if (w < (tid >> 6)) pre += s_w[w]; all += s_w[w]; }
+    for (int w = 0; w < NTH / 64; ++w) { if (w < (tid >> 6)) pre = plus(pre, s_w[w]); all = plus(all, s_w[w]); }
     const int it = place(all);
     if (it < 0) return false;
 #pragma unroll
@@ -275,6 +279,7 @@ __device__ __forceinline__ bool find_item(const MMArgs &a, C count, F place, Gro
     }
     __syncthreads();
     g = Group{__builtin_amdgcn_readfirstlane(s_out[0]), __builtin_amdgcn_readfirstlane(s_out[1]), __builtin_amdgcn_readfirstlane(s_out[2])};
+    if (!g.cnt) return false;
     item = __builtin_amdgcn_readfirstlane(s_out[3]);
     gi = __builtin_amdgcn_readfirstlane(s_out[4]);
     return true;

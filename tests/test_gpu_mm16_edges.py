@@ -364,3 +364,25 @@ def test_runner_without_rows(cuda):
     R.forward(keep=True)
     again = R.run.backward(R.dy)
     assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+def test_overlapping_groups(cuda):
+    """1024 groups that each claim all of 2^22 pairs, as no grouping makes them: more tiles than the scan over the groups counts.
+    Every block still takes a tile of one of them: with the same weights for all experts, the formula or what was there."""
+    T, k, E, d, ff = 1 << 16, 64, 1024, 7, 544
+    P = T * k
+    g = torch.Generator(device=cuda)
+    g.manual_seed(5)
+    W = [dints(g, cuda, 1, ff, d).repeat(E, 1, 1) for _ in range(2)]
+    x = dints(g, cuda, T, d)
+    m = mm16.Moe16Dev(W[0], W[1], None, torch.arange(E, dtype=torch.int32, device=cuda))
+    order = torch.arange(P, dtype=torch.int32, device=cuda)
+    egrp = torch.stack([torch.arange(E), torch.zeros(E, dtype=torch.long), torch.full((E,), P)], 1).reshape(-1).to(torch.int32).to(cuda)
+    buf = torch.full(((P + 2) * ff,), 77.0, dtype=torch.bfloat16, device=cuda)
+    h = buf[ff:-ff].view(P, ff)
+    mm16.moe16_gate_up(m, x, k, P, h, order=order, order_n=torch.tensor([P, E], dtype=torch.int32, device=cuda), egrp=egrp, max_active=E)
+    want = torch.empty(T, ff, dtype=torch.bfloat16, device=cuda)
+    mm16.linear_glu(W[0][0], W[1][0], x, want)
+    wrong = int(((h.view(T, k, ff) != want[:, None]) & (h.view(T, k, ff) != 77.0)).sum())
+    around = int((buf[:ff] != 77.0).sum()) + int((buf[-ff:] != 77.0).sum())
+    assert wrong == 0 and around == 0 and bool((h[0] != 77.0).any())
