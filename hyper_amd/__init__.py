@@ -115,6 +115,13 @@ SIGNATURES = {
     "hy_moe16_dw": (_I, [_DEV, _I, _P, _L, _I, _I, _P, _L, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P]),
     "hy_swiglu_bwd": (_I, [_I, _P, _P, _P, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P]),
     "hy_rows16": (_I, [_I, _P, _L, _I, _I, _P, _L, _P]),
+    "hy_norm": (_I, [_I, _I, _P, _L, _P, _L, _P, _L, _P, _P, _F, _I, _I, _P, _I, _L, _P, _L, _P, _P, _P]),
+    "hy_norm_bwd_ws_bytes": (ctypes.c_size_t, [_I, _I]),
+    "hy_norm_bwd": (_I, [_I, _I, _P, _L, _I, _P, _L, _P, _P, _P, _P, _L, _I, _I, _P, _L, _P, _P, _I, _P, ctypes.c_size_t, _P]),
+    "hy_moe_route_groups": (_I, [_P, _L, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _P]),
+    "hy_moe_route_groups_bwd": (_I, [_P, _L, _I, _I, _P, _I, _I, _F, _P, _P, _I, _L, _I, _P]),
+    "hy_lora_ws_bytes": (ctypes.c_size_t, [_I, _I, _I]),
+    "hy_lora": (_I, [_I, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _L, _P, _I, _L, _P, ctypes.c_size_t, _P]),
     "hy_dequant_row": (_I, [_I, _P, _I, _P, _P]),
     "hy_block_ints": (_I, [_I, _P, ctypes.c_size_t, _I, _P, _I, _P, _P, _P]),
 }

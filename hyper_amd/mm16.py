@@ -329,6 +329,141 @@ def swiglu_bwd(g, u, dh, wts, dg, du, hw=None, dwts=None, clamp=0.0, order=None,
           _p(hw), _p(dwts))
 
 
+# ------------------------------------------------------------------ norms
+
+NORMS = {"layer": 0, "rms": 1}
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _any(name: str, t: torch.Tensor) -> int:
+    v = _TYPE.get(t.dtype)
+    if v is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return v
+
+
+def _named(table, what: str, name: str) -> int:
+    v = table.get(name)
+    if v is None:
+        raise ValueError(f"unknown {what} {name!r}")
+    return v
+
+
+def norm(x, w, out=None, b=None, eps=1e-5, kind="layer", add=None, total=None, out32=None, mean=None, rstd=None, stream=None):
+    """out = (s - mean(s)) rstd w + b for the rows s = x + add, rstd = 1 / sqrt(mean((s - mean)^2) + eps); kind "rms": without the
+    mean.  x, add, total [m, n] of one type; total receives s (rounded to that type, which is what is normed) and may be x or add.  out: any
+    of the types, out32: the same in float32; w, b: n float32 values; mean, rstd: m float32 values kept for norm_bwd."""
+    ki, xt, (m, n) = _named(NORMS, "norm", kind), _any("x", x), x.shape
+    ldx = _mat("x", x, m, n)
+    lda = _mat("add", add, m, n, x.dtype) if add is not None else 0
+    ldt = _mat("total", total, m, n, x.dtype) if total is not None else 0
+    ldo, ot = (_mat("out", out, m, n), _any("out", out)) if out is not None else (0, HY_F32)
+    ldo32 = _mat("out32", out32, m, n, torch.float32) if out32 is not None else 0
+    if w is None:
+        raise ValueError("w is needed")
+    _vec("w", w, n, torch.float32)
+    _vec("b", b, n, torch.float32)
+    _vec("mean", mean, m, torch.float32)
+    _vec("rstd", rstd, m, torch.float32)
+    _call(lib().hy_norm, x, stream, (w, out, b, add, total, out32, mean, rstd),
+          ki, xt, _p(x), ldx, _p(add), lda, _p(total), ldt, _p(w), _p(b), eps, m, n, _p(out), ot, ldo, _p(out32), ldo32, _p(mean), _p(rstd))
+
+
+def norm_bwd_ws_bytes(m: int, n: int) -> int:
+    """bytes of norm_bwd's workspace (0: none needed)"""
+    return lib().hy_norm_bwd_ws_bytes(m, n)
+
+
+def norm_bwd(x, dy, w, rstd, dx, mean=None, kind="layer", resid=None, dw=None, db=None, accumulate=False, ws=None, stream=None):
+    """Gradients of norm from dy, the normed rows x (norm's total, where something was added) and their statistics: dx (+ resid, the
+    gradient that passes by on the residual stream; both of x's type), dw and db (float32), added to what is there with `accumulate`.
+    ws: a uint8 tensor of norm_bwd_ws_bytes(m, n) bytes, free again once the call's work on the stream is done."""
+    ki, xt, yt, (m, n) = _named(NORMS, "norm", kind), _any("x", x), _any("dy", dy), x.shape
+    ldx, ldy = _mat("x", x, m, n), _mat("dy", dy, m, n)
+    ldr = _mat("resid", resid, m, n, x.dtype) if resid is not None else 0
+    ldd = _mat("dx", dx, m, n, x.dtype)
+    if w is None or rstd is None or (mean is None and ki == 0):
+        raise ValueError("w, rstd and a layer norm's mean are needed")
+    _vec("w", w, n, torch.float32)
+    _vec("mean", mean, m, torch.float32)
+    _vec("rstd", rstd, m, torch.float32)
+    _vec("dw", dw, n, torch.float32)
+    _vec("db", db, n, torch.float32)
+    _vec("ws", ws, 0, torch.uint8)
+    _call(lib().hy_norm_bwd, x, stream, (dy, w, rstd, dx, mean, resid, dw, db, ws),
+          ki, xt, _p(x), ldx, yt, _p(dy), ldy, _p(w), _p(mean), _p(rstd), _p(resid), ldr, m, n, _p(dx), ldd, _p(dw), _p(db), int(bool(accumulate)),
+          _p(ws), 0 if ws is None else ws.numel())
+
+
+# ------------------------------------------------------------------ routing with groups
+
+def _rows_of(name, t, nt, k, dtype):
+    if t.shape != (nt, k) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous [{nt}, {k}] {dtype}, got {t.dtype} {tuple(t.shape)}")
+
+
+def route_groups(logits, ids, wts, score="softmax", bias=None, n_group=1, top_group=1, group_best=1, renorm=True, scale=1.0, stream=None):
+    """ids, wts [nt, k] from the float32 logits [nt, E]: scores by softmax or sigmoid, c = score + bias, the top_group of n_group equal
+    runs of experts by the sum of their group_best largest c, in them the k experts with the largest c (ties to the lower index);
+    weights score * scale, with `renorm` over their sum.  Experts with a logit of -inf, and those whose c is NaN or -inf, are never
+    chosen; places that are left get id -1 and weight 0, which the calls for experts skip."""
+    sc, (nt, E), k = _named(SCORES, "score", score), logits.shape, ids.shape[-1]
+    ls = _mat("logits", logits, nt, E, torch.float32)
+    _vec("bias", bias, E, torch.float32)
+    _rows_of("ids", ids, nt, k, torch.int32)
+    _rows_of("wts", wts, nt, k, torch.float32)
+    _call(lib().hy_moe_route_groups, logits, stream, (ids, wts, bias),
+          _p(logits), ls, E, _p(bias), sc, n_group, top_group, group_best, k, int(bool(renorm)), scale, _p(ids), _p(wts), nt)
+
+
+def route_groups_bwd(logits, ids, dwts, dlogits, score="softmax", renorm=True, scale=1.0, stream=None):
+    """dlogits [nt, E] (float32 or a 16-bit type) of route_groups' weights from their gradient dwts [nt, k]; the choice and the bias have none."""
+    sc, (nt, E), k = _named(SCORES, "score", score), logits.shape, ids.shape[-1]
+    ls = _mat("logits", logits, nt, E, torch.float32)
+    ldd, ty = _mat("dlogits", dlogits, nt, E), _any("dlogits", dlogits)
+    _rows_of("ids", ids, nt, k, torch.int32)
+    _rows_of("dwts", dwts, nt, k, torch.float32)
+    _call(lib().hy_moe_route_groups_bwd, logits, stream, (ids, dwts, dlogits),
+          _p(logits), ls, E, sc, _p(ids), k, int(bool(renorm)), scale, _p(dwts), _p(dlogits), ty, ldd, nt)
+
+
+# ------------------------------------------------------------------ low-rank adapters
+
+class Lora16:
+    """Adapters beside one projection: A [adapters, r, k], B [adapters, n, r] of one 16-bit type, contiguous (lower ranks padded
+    with zeros), and their scales (float32, None: 1).  Keeps the tensors alive."""
+
+    def __init__(self, A, B, scale: Optional[torch.Tensor] = None):
+        if A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
+            raise ValueError(f"A must be [adapters, r, k] and B [adapters, n, r], got {tuple(A.shape)} and {tuple(B.shape)}")
+        if A.dtype != B.dtype or not A.is_contiguous() or not B.is_contiguous():
+            raise ValueError("A and B must be contiguous and of one type")
+        if A.device != B.device or (scale is not None and scale.device != A.device):
+            raise ValueError("A, B and scale must be on one device")
+        self.type, (self.n_local, self.r, self.k), self.n = _type16(A), A.shape, B.shape[1]
+        _vec("scale", scale, self.n_local, torch.float32)
+        self.A, self.B, self.scale = A, B, scale
+
+
+def lora_ws_bytes(L: Lora16, m: int) -> int:
+    """bytes of lora's workspace for m rows"""
+    return lib().hy_lora_ws_bytes(m, L.r, L.k)
+
+
+def lora(L: Lora16, x, ids, out, resid=None, ws=None, stream=None):
+    """out[t] = resid[t] + scale_a B_a (A_a x[t]) with a = ids[t] (int32; outside the adapters: resid[t] alone, zeros without resid).
+    out and resid [m, n] of the adapters' type or float32; resid may be out, e.g. the output of linear.  ws: a uint8 tensor of
+    lora_ws_bytes(L, m) bytes, free again once the call's work on the stream is done."""
+    m, dt = x.shape[0], L.A.dtype
+    ldx, ldo = _mat("x", x, m, L.k, dt), _mat("out", out, m, L.n, dt, torch.float32)
+    ldr = _mat("resid", resid, m, L.n, out.dtype) if resid is not None else 0
+    _vec("ids", ids, m, torch.int32)
+    _vec("ws", ws, 0, torch.uint8)
+    _call(lib().hy_lora, L.A, stream, (x, ids, out, resid, ws),
+          L.type, _p(L.A), _p(L.B), _p(L.scale), L.n_local, L.r, L.k, L.n, _p(x), ldx, m, _p(ids), _p(resid), ldr, _p(out), _TYPE[out.dtype], ldo,
+          _p(ws), 0 if ws is None else ws.numel())
+
+
 # ------------------------------------------------------------------ one MoE layer
 
 class Moe16LayerRunner:

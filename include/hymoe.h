@@ -372,6 +372,57 @@ int hy_swiglu_bwd(int type, const void *g, const void *u, const void *dh, const 
 /* fp32 rows x[t * xs ..][0..n) rounded to `type` (the router's rows for the calls above) */
 int hy_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, int64_t ldo, hipStream_t s);
 
+/* ---- What stands around the 16-bit products of a block: the norm in front of it, a router with groups, the gradients of both,
+   low-rank adapters beside a projection.  Types are HY_F32, HY_F16 or HY_BF16; matrices as above (rows ld* elements apart, any
+   size and alignment, 16-byte rows fastest); no atomics. */
+#define HY_NORM_LAYER 0
+#define HY_NORM_RMS 1
+#define HY_NORM_MAX (1 << 22)   /* most values of a row */
+
+/* Norm of m rows of n values: s = x (+ add), y = (s - mean) rstd w (+ b) with rstd = 1 / sqrt(mean of (s - mean)^2 + eps); RMS:
+   without the mean.  add and total (x's type; NULL: none): total receives s as rounded to x's type, which is what is normed; it may
+   be x or add.  y goes to out (of out_type) and out32 (fp32), one of which may be NULL; out or out32 may be x where the types
+   agree.  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  Sums are fp32. */
+int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, int64_t ldadd, void *total, int64_t ldt, const float *w, const float *b,
+            float eps, int m, int n, void *out, int out_type, int64_t ldo, float *out32, int64_t ldo32, float *mean, float *rstd, hipStream_t s);
+/* Its gradients from dy (of dy_type), the normed rows x (total, where something was added) and their statistics: with
+   h = (x - mean) rstd and g = dy w,  dx = rstd (g - mean(g) - h mean(g h)) + resid  (RMS: no mean, no mean(g)),
+   dw = sum over the rows of dy h,  db = sum of dy (either NULL: not wanted), added to what is there with accumulate != 0; m = 0
+   gives zeros.  resid (x's type; NULL: none) is the gradient that passes by on the residual stream; dx, of x's type, may be x,
+   resid or dy.  ws: hy_norm_bwd_ws_bytes(m, n) bytes (which may be 0; not needed without dw and db), 16-byte aligned, for calls
+   on one stream; nothing in it is kept. */
+size_t hy_norm_bwd_ws_bytes(int m, int n);
+int hy_norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, const void *dy, int64_t lddy, const float *w, const float *mean,
+                const float *rstd, const void *resid, int64_t ldr, int m, int n, void *dx, int64_t lddx, float *dw, float *db, int accumulate,
+                void *ws, size_t ws_bytes, hipStream_t s);
+
+#define HY_SCORE_SOFTMAX 0
+#define HY_SCORE_SIGMOID 1
+/* Routing with groups: scores s = softmax or sigmoid of logits[t][0 .. n_expert), c = s + bias (NULL: none); the experts lie in
+   n_group equal runs, a run's worth is the sum of its group_best (1 or 2) largest c; among the top_group best runs the k experts
+   with the largest c, ties to the lower index; wts = s scale, or with renorm != 0 s scale / (sum of the chosen s), 0 where that
+   sum is 0.  The choice is that of the formula in 64 bits.  An expert whose logit is -inf, or whose c is NaN or -inf, is
+   never chosen (a NaN or +inf logit makes every softmax score of its token NaN), nor is a run with fewer than group_best others;
+   places that are left get id -1 and weight 0, which the calls for experts skip.  n_expert <= 1024, n_group <= 64, k <= 64,
+   nt < 2^24.  ids and wts [nt][k]. */
+int hy_moe_route_groups(const float *logits, int64_t ls, int n_expert, const float *bias, int score, int n_group, int top_group, int group_best,
+                        int k, int renorm, float scale, int32_t *ids, float *wts, int nt, hipStream_t s);
+/* Gradient of its wts with respect to the logits, for the experts in ids as they were chosen (the choice and the bias have
+   none): dlogits [nt][n_expert] (of `type`) from dwts [nt][k]; zeros where an expert was not chosen, unless scores are softmax
+   without renorm.  An id outside the experts takes no part. */
+int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int score, const int32_t *ids, int k, int renorm, float scale,
+                            const float *dwts, void *dlogits, int type, int64_t ldd, int nt, hipStream_t s);
+
+/* Low-rank adapters of many requests beside a shared projection: out[t] = resid[t] + scale_a B_a (A_a x[t]) with a = ids[t], for m
+   rows x [m][k]; a row whose id is outside [0, n_local) gets resid[t] alone (zeros without resid).  A [n_local][r][k] and
+   B [n_local][n][r], contiguous, of `type`; scale: n_local floats (NULL: 1); resid and out of out_type (`type` or HY_F32), resid may
+   be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32.  r at most
+   HY_LORA_MAX_RANK.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned, as hy_linear_dw's. */
+#define HY_LORA_MAX_RANK 256
+size_t hy_lora_ws_bytes(int m, int r, int k);
+int hy_lora(int type, const void *A, const void *B, const float *scale, int n_local, int r, int k, int n, const void *x, int64_t ldx, int m,
+            const int32_t *ids, const void *resid, int64_t ldr, void *out, int out_type, int64_t ldo, void *ws, size_t ws_bytes, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

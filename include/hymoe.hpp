@@ -230,6 +230,32 @@ inline void deq_row_test(int type, const uint8_t *row, int n, float *out, hipStr
     check(hy_dequant_row(type, row, n, out, s));
 }
 
+// ---- around the 16-bit products: norms, routing with groups, low-rank adapters (hymoe.h)
+inline void norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, int64_t ldadd, void *total, int64_t ldt, const float *w,
+                 const float *b, float eps, int m, int n, void *out, int out_type, int64_t ldo, float *out32, int64_t ldo32, float *mean, float *rstd,
+                 hipStream_t s) {
+    check(hy_norm(kind, x_type, x, ldx, add, ldadd, total, ldt, w, b, eps, m, n, out, out_type, ldo, out32, ldo32, mean, rstd, s));
+}
+inline size_t norm_bwd_ws_bytes(int m, int n) { return hy_norm_bwd_ws_bytes(m, n); }
+inline void norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, const void *dy, int64_t lddy, const float *w, const float *mean,
+                     const float *rstd, const void *resid, int64_t ldr, int m, int n, void *dx, int64_t lddx, float *dw, float *db, bool accumulate,
+                     void *ws, size_t ws_bytes, hipStream_t s) {
+    check(hy_norm_bwd(kind, x_type, x, ldx, dy_type, dy, lddy, w, mean, rstd, resid, ldr, m, n, dx, lddx, dw, db, accumulate, ws, ws_bytes, s));
+}
+inline void moe_route_groups(const float *logits, int64_t ls, int n_expert, const float *bias, int score, int n_group, int top_group, int group_best,
+                             int k, bool renorm, float scale, int *ids, float *wts, int nt, hipStream_t s) {
+    check(hy_moe_route_groups(logits, ls, n_expert, bias, score, n_group, top_group, group_best, k, renorm, scale, ids, wts, nt, s));
+}
+inline void moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int score, const int *ids, int k, bool renorm, float scale,
+                                 const float *dwts, void *dlogits, int type, int64_t ldd, int nt, hipStream_t s) {
+    check(hy_moe_route_groups_bwd(logits, ls, n_expert, score, ids, k, renorm, scale, dwts, dlogits, type, ldd, nt, s));
+}
+inline size_t lora_ws_bytes(int m, int r, int k) { return hy_lora_ws_bytes(m, r, k); }
+inline void lora(int type, const void *A, const void *B, const float *scale, int n_local, int r, int k, int n, const void *x, int64_t ldx, int m,
+                 const int *ids, const void *resid, int64_t ldr, void *out, int out_type, int64_t ldo, void *ws, size_t ws_bytes, hipStream_t s) {
+    check(hy_lora(type, A, B, scale, n_local, r, k, n, x, ldx, m, ids, resid, ldr, out, out_type, ldo, ws, ws_bytes, s));
+}
+
 // ---- 16-bit matrix products (hymoe.h: hy_linear and the experts' hy_moe16_* calls), std::runtime_error on failure
 inline void linear(int type, const void *W, int64_t ldw, int n, int k, const void *x, int64_t ldx, int m, const float *bias, int act,
                    const void *resid, int64_t ldr, void *z, int64_t ldz, void *out, int out_type, int64_t ldo, hipStream_t s) {
