@@ -25,6 +25,22 @@ template <typename T, bool AL> __device__ __forceinline__ v8<T> lora_ld8(const T
     }
     return v;
 }
+// Lanes 2 i and 2 i + 1 (neighbouring rows of an operand or output) exchange one 16-byte piece: the even lane keeps p and gives q,
+// the odd lane keeps q and gives p.  Memory is then met eight lanes to a row and 128 bytes, as whole lines; a row's own four
+// lanes alone meet 64 bytes, which come and go at about half the rate.
+template <typename V> __device__ __forceinline__ void pair_swap(V &p, V &q) {
+    static_assert(sizeof(V) == 16, "");
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const bool odd = threadIdx.x & 1;
+    i32x4 a = __builtin_bit_cast(i32x4, p), b = __builtin_bit_cast(i32x4, q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int got = dpp_i<DPP_XOR1>(odd ? a[i] : b[i]);
+        if (odd) a[i] = got; else b[i] = got;
+    }
+    p = __builtin_bit_cast(V, a);
+    q = __builtin_bit_cast(V, b);
+}
 // the adapter of lane i's row for lanes below ROWS, -1 where there is none
 template <int ROWS> __device__ __forceinline__ int lora_id(const LoraArgs &a, int r0) {
     const int lane = threadIdx.x & 63;
@@ -33,57 +49,197 @@ template <int ROWS> __device__ __forceinline__ int lora_id(const LoraArgs &a, in
     return (uint32_t) id < (uint32_t) a.n_local ? id : -1;
 }
 
-// Low products of 16 rows over part blockIdx.y of the contraction, RT tiles of 16 ranks at a time; the four waves take every
-// fourth 64 values and are added up in LDS.  A lane's 16 neighbouring values of a row are two products' operands (which of the
-// contraction's values meet in which product does not matter as long as both operands agree), so that four lanes read 128
-// neighbouring bytes.  The adapters of the tile are dealt out over blockIdx.z.
-template <typename T, int RT, bool ALX, bool ALA> __global__ __launch_bounds__(256) void k_lora_low(const LoraArgs a) {
+// Low products of 16 RW rows over a part of the contraction, RT tiles of 16 ranks at a time; the four waves take every
+// fourth 64 values and are added up in LDS.  The adapters of the tile are dealt out over blockIdx.z.
+template <typename T, int RT, int RW> struct LowStep {   // a step's operands; as loaded: piece 0 of the even row, piece 1 of the odd one
+    v8<T> x[RW][2], w[RT][2];
+    __device__ __forceinline__ void load(const T *const (&xr)[RW][2], const T *const (&A)[RT][2], int at) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) { x[i][0] = *(const v8<T> *) (xr[i][0] + at); x[i][1] = *(const v8<T> *) (xr[i][1] + at); }
+#pragma unroll
+        for (int j = 0; j < RT; ++j) { w[j][0] = *(const v8<T> *) (A[j][0] + at); w[j][1] = *(const v8<T> *) (A[j][1] + at); }
+    }
+    __device__ __forceinline__ void swap() {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) pair_swap(x[i][0], x[i][1]);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) pair_swap(w[j][0], w[j][1]);
+    }
+    __device__ __forceinline__ void add(f4 (&acc)[RW][RT]) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < RW; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[i][j] = mfma16(w[j][h], x[i][h], acc[i][j]);
+    }
+};
+// Between the loads of a step and the products of the one before: else the compiler moves the loads to where they are used, and
+// nothing is in flight while the products run
+__device__ __forceinline__ void lora_keep_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <typename T, int RT, int RW, bool AL> __global__ __launch_bounds__(256) void k_lora_low(const LoraArgs a) {
     __shared__ float s_acc[4][16][16 * RT + 4];
+    constexpr int ROWS = 16 * RW, STEP = 256;   // (a wave's own 64 values, then the other waves')
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
-    const int r0 = blockIdx.x * 16, k0 = blockIdx.y * a.klen, k1 = min(a.k, k0 + a.klen);
-    const int id = lora_id<16>(a, r0);
+    const int w = xcd_tile(blockIdx.x, gridDim.x), part = w % a.splits;   // neighbouring tiles on one XCD: they share adapters
+    const int r0 = w / a.splits * ROWS, k0 = part * a.klen, k1 = min(a.k, k0 + a.klen);
+    const int id = lora_id<ROWS>(a, r0);
     uint64_t left = __ballot(id >= 0);
-    const T *xr = (const T *) a.x + (int64_t) min(r0 + i16, a.m - 1) * a.ldx;
+    const int odd = lane & 1;
+    const T *x[RW][2];   // rows of the lane pair, from its piece of a step on: the even lane's is the first 8 q values, the odd one's 32 values behind
+#pragma unroll
+    for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[i][h] = (const T *) a.x + (int64_t) min(r0 + 16 * i + (i16 & ~1) + h, a.m - 1) * a.ldx + 8 * q + 32 * odd;
     for (int turn = 0; left; ++turn) {
         const int ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
         const uint64_t mine = __ballot(id == ad);
         left &= ~mine;
         if (turn % gridDim.z != blockIdx.z) continue;
         for (int rb = 0; rb < a.r; rb += 16 * RT) {
-            const T *A[RT];
+            const T *A[RT][2];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) A[j] = (const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + i16, a.r - 1)) * a.k;
-            f4 acc[RT] = {};
-            for (int kk = k0 + 64 * wave; kk < k1; kk += 256) {
-                const int c = kk + 16 * q;
-                const v8<T> x0 = lora_ld8<T, ALX>(xr, c, k1), x1 = lora_ld8<T, ALX>(xr, c + 8, k1);
-                v8<T> a0[RT], a1[RT];
+            for (int j = 0; j < RT; ++j)
 #pragma unroll
-                for (int j = 0; j < RT; ++j) { a0[j] = lora_ld8<T, ALA>(A[j], c, k1); a1[j] = lora_ld8<T, ALA>(A[j], c + 8, k1); }
+                for (int h = 0; h < 2; ++h) A[j][h] = (const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + (i16 & ~1) + h, a.r - 1)) * a.k + 8 * q + 32 * odd;
+            f4 acc[RW][RT] = {};
+            int kk = __builtin_amdgcn_readfirstlane(k0 + 64 * wave);
+            if constexpr (AL) {
+                // whole steps, two sets of operands in turns: the loads ask no condition (the last step's are its own again), so that
+                // the compiler counts those in flight and products wait for their own operands only
+                const int last = k1 - kk >= 64 ? kk + (k1 - kk - 64) / STEP * STEP : -1;
+                if (last >= 0) {
+                    LowStep<T, RT, RW> s0, s1;
+                    s0.load(x, A, kk);
+                    for (;;) {
+                        s1.load(x, A, min(kk + STEP, last));
+                        lora_keep_order();
+                        s0.swap();
+                        s0.add(acc);
+                        if ((kk += STEP) > last) break;
+                        s0.load(x, A, min(kk + STEP, last));
+                        lora_keep_order();
+                        s1.swap();
+                        s1.add(acc);
+                        if ((kk += STEP) > last) break;
+                    }
+                }
+            }
+            for (; kk < k1; kk += STEP) {   // the lane's own rows, up to the part's end
+                LowStep<T, RT, RW> s;
 #pragma unroll
-                for (int j = 0; j < RT; ++j) { acc[j] = mfma16(a0[j], x0, acc[j]); acc[j] = mfma16(a1[j], x1, acc[j]); }
+                for (int h = 0; h < 2; ++h) {
+                    const int c = kk + 8 * q + 32 * h;
+#pragma unroll
+                    for (int i = 0; i < RW; ++i) s.x[i][h] = lora_ld8<T, AL>((const T *) a.x + (int64_t) min(r0 + 16 * i + i16, a.m - 1) * a.ldx, c, k1);
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) s.w[j][h] = lora_ld8<T, AL>((const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + i16, a.r - 1)) * a.k, c, k1);
+                }
+                s.add(acc);
             }
 #pragma unroll
-            for (int j = 0; j < RT; ++j) *(f4 *) &s_acc[wave][i16][16 * j + 4 * q] = acc[j];
-            __syncthreads();
-            for (int i = threadIdx.x; i < 16 * 16 * RT; i += 256) {
-                const int row = i / (16 * RT), c = i % (16 * RT);
-                if ((mine >> row & 1) && rb + c < a.r)
-                    a.low[((int64_t) blockIdx.y * a.m + r0 + row) * a.r + rb + c] = (s_acc[0][row][c] + s_acc[1][row][c]) + (s_acc[2][row][c] + s_acc[3][row][c]);
+            for (int i = 0; i < RW; ++i) {
+                if (!(mine >> (16 * i) & 0xffff)) continue;   // (the same in every wave)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) *(f4 *) &s_acc[wave][i16][16 * j + 4 * q] = acc[i][j];
+                __syncthreads();
+                for (int e = threadIdx.x; e < 16 * 16 * RT; e += 256) {
+                    const int row = e / (16 * RT), c = e % (16 * RT);
+                    if ((mine >> (16 * i + row) & 1) && rb + c < a.r)
+                        a.low[((int64_t) part * a.m + r0 + 16 * i + row) * a.r + rb + c] = (s_acc[0][row][c] + s_acc[1][row][c]) + (s_acc[2][row][c] + s_acc[3][row][c]);
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
     }
 }
 
-// out of 16 RT rows x 256 columns, 64 columns a wave.  A lane holds 16 neighbouring columns of a row: column tile j's operand row i
-// is column 16 (i / 4) + 4 j + i % 4.  R: the rank rounded up to 32, as the LDS rows hold it.
-template <typename T, int RT, int R, bool ALB> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a) {
-    constexpr int LD = R + 8, ROWS = 16 * RT;
+// the sums over the parts of N low products from rank c on (those below r), c a multiple of N; VEC: rows of whole 16-byte pieces
+template <int N, bool VEC> __device__ __forceinline__ void lora_sum(const float *low, int64_t between, int splits, int c, int r, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+    if (c >= r) return;
+    constexpr int U = N >= 16 ? 2 : N >= 8 ? 4 : 8;   // parts on their way together
+    for (int sp = 0; sp < splits; sp += U) {
+        float p[U][N];
+#pragma unroll
+        for (int h = 0; h < U; ++h) {
+            const float *at = low + (int64_t) min(sp + h, splits - 1) * between + c;
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[h][i] = 0.0f;
+            if constexpr (VEC && N % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) if (c + i < r) { const f4 f = *(const f4 *) (at + i); p[h][i] = f[0]; p[h][i + 1] = f[1]; p[h][i + 2] = f[2]; p[h][i + 3] = f[3]; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) if (c + i < r) p[h][i] = at[i];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < U; ++h)
+            if (sp + h < splits) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] += p[h][i];
+            }
+    }
+}
+
+// 16 bytes of outputs
+template <typename O> struct Piece { typedef v8<O> type; };
+template <> struct Piece<float> { typedef f4 type; };
+
+// The second product and the epilogue: 16 RT rows x 64 columns a wave and item; the block's four waves have the same rows, whose
+// low products they keep in LDS as the matrix instructions' operands.  Column tile j's operand row i is column 16 j + i for fp32
+// outputs and 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4 for 16-bit ones, so that a lane holds 16-byte pieces of its row.  A turn of 64
+// columns is an item for each of the rows' adapters: its columns of B, its rows' residual, products, outputs (a row tile where
+// prompts meet is multiplied for each).  Up to rank 64 the next item's loads are on their way while an item is worked on.
+// KK: ranks in units of 32.  AL: B, resid and out are whole 16-byte pieces, and there is a resid.
+template <typename T, typename O, int RT, int KK, bool AL> struct UpItem {
+    typedef typename Piece<O>::type PT;
+    static constexpr int PN = 16 / sizeof(O), NP = 16 / PN, LOADS = 4 * KK + RT * NP;   // values of a piece, a lane's pieces of a row, loads
+    v8<T> b[KK][4];
+    PT res[RT][NP];
+    uint64_t mine, write;   // the item's rows that have its adapter, and all that it writes
+    int c0;
+
+    // piece p belongs to the lane pair's even row (p % 2 = 0) or odd row: even lanes have the columns of pieces 2 (p / 2), odd ones those of the next
+    __device__ __forceinline__ static int row_of(int i, int p, int lane) { return 16 * i + (lane & 14) + (p & 1); }
+    __device__ __forceinline__ int col_of(int p, int lane) const { return c0 + (2 * (p >> 1) + (lane & 1)) * 4 * PN + PN * (lane >> 4); }
+    __device__ __forceinline__ void load(const LoraArgs &a, int ad, const char *rbase, uint32_t ldr, int lane) {
+        const int q = lane >> 4, i16 = lane & 15;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = min(c0 + (PN == 4 ? 16 * j + i16 : 32 * (j >> 1) + 8 * (i16 >> 2) + 4 * (j & 1) + (i16 & 3)), a.n - 1);
+            const T *B = (const T *) a.B + ((int64_t) max(ad, 0) * a.n + c) * a.r;
+#pragma unroll
+            for (int h = 0; h < KK; ++h) {   // ranks behind the last come from one before it (zeroed at their use)
+                if constexpr (AL) b[h][j] = *(const v8<T> *) (B + min(32 * h + 8 * q, a.r - 8));
+                else b[h][j] = lora_ld8<T, false>(B, 32 * h + 8 * q, a.r);
+            }
+        }
+        if constexpr (AL) {   // a row that is not to be written: one that is, as for other lanes
+            const int first = __builtin_ctzll(write);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const uint32_t row = write >> row_of(i, p, lane) & 1 ? row_of(i, p, lane) : first;
+                    res[i][p] = *(const PT *) (rbase + (row * ldr + min(col_of(p, lane), a.n - PN) * (uint32_t) sizeof(O)));
+                }
+        }
+    }
+};
+template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a, int gy) {
+    typedef UpItem<T, O, RT, KK, AL> Item;
+    constexpr int R = 32 * KK, LD = R + 8, ROWS = 16 * RT, PN = Item::PN, NP = Item::NP;
     __shared__ __attribute__((aligned(16))) T s_hi[ROWS * LD], s_lo[ROWS * LD];
     __shared__ float s_scale[ROWS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
-    const int r0 = blockIdx.x * ROWS, c0 = (blockIdx.y * 4 + wave) * 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
+    const int blk = xcd_tile(blockIdx.x, gridDim.x);   // neighbouring tiles on one XCD: they share adapters
+    const int r0 = blk / gy * ROWS;
     const int id = lora_id<ROWS>(a, r0);
     // the adapters of the tile that are this block's: their rows
     uint64_t left = __ballot(id >= 0), rows = 0;
@@ -92,21 +248,39 @@ template <typename T, int RT, int R, bool ALB> __global__ __launch_bounds__(256)
         left &= ~mine;
         if (turn % gridDim.z == blockIdx.z) rows |= mine;
     }
-    // their low products, four threads a row and 32 ranks
-    constexpr int TPR = 256 / ROWS, PER = R / TPR;   // threads a row, values a thread
-    {
+    // rows without an adapter are the first blocks'
+    uint64_t none = __ballot(id < 0 && lane < ROWS && r0 + lane < a.m);
+    if (blockIdx.z || (a.resid == a.out && a.ldr == a.ldo)) none = 0;
+    if (!(rows | none)) return;   // (the same in every wave)
+    // the tile's rows by 32-bit offsets (AL: rows of less than 2^24 bytes)
+    const char *rbase = (const char *) a.resid + (int64_t) r0 * a.ldr * (int) sizeof(O);
+    char *obase = (char *) a.out + (int64_t) r0 * a.ldo * (int) sizeof(O);
+    const uint32_t ldr = (uint32_t) a.ldr * (uint32_t) sizeof(O), ldo = (uint32_t) a.ldo * (uint32_t) sizeof(O);
+    int c0 = (blk % gy * 4 + wave) * 64;
+    left = rows;   // those of the turn's items that are still to come
+    auto next = [&](Item &s) {   // the next item's loads
+        const int ad = left ? __builtin_amdgcn_readlane(id, __builtin_ctzll(left)) : -1;
+        s.mine = left ? __ballot(id == ad) : 0;
+        s.write = s.mine | (left == rows ? none : 0);   // with the first of a turn those without an adapter
+        s.c0 = min(c0, a.n - 1);
+        s.load(a, ad, rbase, ldr, lane);
+        left &= ~s.mine;
+        if (!left) { left = rows; c0 += gy * 256; }
+    };
+    Item s0, s1;
+    next(s0);   // on its way while the low products are added up
+    // TPR threads a row with PER neighbouring ranks each
+    constexpr int TPR = 256 / ROWS, PER = R / TPR;
+    if (rows) {
         const int row = threadIdx.x / TPR, t = threadIdx.x % TPR;
         float v[PER], top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = 0.0f;
-        if (rows >> row & 1) {
-            const float *low = a.low + (int64_t) (r0 + row) * a.r;
-            for (int sp = 0; sp < a.splits; ++sp, low += (int64_t) a.m * a.r)
-#pragma unroll
-                for (int i = 0; i < PER; ++i) if (t + TPR * i < a.r) v[i] += low[t + TPR * i];
-        }
+        const float *low = a.low + (int64_t) (r0 + row) * a.r;
+        const int64_t between = (int64_t) a.m * a.r;
+        const int end = rows >> row & 1 ? a.r : 0;
+        if (a.r % 4 == 0) lora_sum<PER, true>(low, between, a.splits, t * PER, end, v);
+        else lora_sum<PER, false>(low, between, a.splits, t * PER, end, v);
         float up = 1.0f;
-        if constexpr (sizeof(T) == 2 && __is_same(T, f16)) {
+        if constexpr (__is_same(T, f16)) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) top = fmaxf(top, fabsf(v[i]));
 #pragma unroll
@@ -114,103 +288,149 @@ template <typename T, int RT, int R, bool ALB> __global__ __launch_bounds__(256)
             const int e = (int) (__float_as_uint(top) >> 23) - 127;   // 2^e <= top
             if (top < __builtin_huge_valf() && e > -100) up = __uint_as_float((uint32_t) (127 + min(max(13 - e, -113), 113)) << 23);   // the largest to 2^13 .. 2^14
         }
-        if (t == 0) s_scale[row] = 1.0f / up;
+        if (t == 0) {
+            const int my = end ? a.ids[r0 + row] : 0;
+            s_scale[row] = (a.scale && end ? a.scale[my] : 1.0f) * (1.0f / up);
+        }
+        constexpr int P = PER < 8 ? PER : 8;
+        typedef T vt __attribute__((ext_vector_type(P)));
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const float u = v[i] * up;
-            const T hi = (T) u;
-            const float rest = u - (float) hi;
-            s_hi[row * LD + t + TPR * i] = hi;
-            s_lo[row * LD + t + TPR * i] = rest - rest == 0.0f ? (T) rest : (T) 0.0f;   // (none of an infinity)
+        for (int g = 0; g < PER; g += P) {
+            vt hi, lo;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float u = v[g + i] * up;
+                hi[i] = (T) u;
+                const float rest = u - (float) hi[i];
+                lo[i] = rest - rest == 0.0f ? (T) rest : (T) 0.0f;   // (none of an infinity)
+            }
+            *(vt *) &s_hi[row * LD + t * PER + g] = hi;
+            *(vt *) &s_lo[row * LD + t * PER + g] = lo;
         }
     }
     __syncthreads();
-    if (c0 >= a.n) return;
-    f4 out[RT][4] = {};
-    left = rows;
-    while (left) {
-        const int ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const uint64_t mine = __ballot(id == ad);
-        left &= ~mine;
-        f4 acc[RT][4] = {};
-#pragma unroll 1
-        for (int kk = 0; kk < a.r; kk += 32) {
-            v8<T> b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = min(c0 + 16 * (i16 >> 2) + 4 * j + (i16 & 3), a.n - 1);
-                b[j] = lora_ld8<T, ALB>((const T *) a.B + ((int64_t) ad * a.n + c) * a.r, kk + 8 * q, a.r);
-            }
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                if (!(mine >> (16 * i) & 0xffff)) continue;   // (the same in every lane)
-                const v8<T> hi = *(const v8<T> *) &s_hi[(16 * i + i16) * LD + kk + 8 * q], lo = *(const v8<T> *) &s_lo[(16 * i + i16) * LD + kk + 8 * q];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { acc[i][j] = mfma16(b[j], lo, acc[i][j]); acc[i][j] = mfma16(b[j], hi, acc[i][j]); }
-            }
-        }
-        const float sc = a.scale ? a.scale[ad] : 1.0f;
+    auto work = [&](const Item &s) {
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            if (!(mine >> (16 * i + i16) & 1)) continue;
-            const float s = sc * s_scale[16 * i + i16];
+            if (!(s.write >> (16 * i) & 0xffff)) continue;
+            const int r = 16 * i + i16;
+            f4 acc[4] = {};
+            if (s.mine >> (16 * i) & 0xffff) {
+#pragma unroll
+                for (int h = 0; h < KK; ++h) {
+                    const v8<T> hi = *(const v8<T> *) &s_hi[r * LD + 32 * h + 8 * q], lo = *(const v8<T> *) &s_lo[r * LD + 32 * h + 8 * q];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const v8<T> w = !AL || 32 * h + 8 * q < a.r ? s.b[h][j] : v8<T>{};
+                        acc[j] = mfma16(w, lo, acc[j]);
+                        acc[j] = mfma16(w, hi, acc[j]);
+                    }
+                }
+            }
+            const bool has = s.mine >> r & 1;
+            const float sc = has ? s_scale[r] : 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[i][j][e] = acc[i][j][e] * s;
+                for (int e = 0; e < 4; ++e) acc[j][e] = has ? acc[j][e] * sc : 0.0f;   // (nothing of other adapters' values)
+            if constexpr (AL) {
+#pragma unroll
+                for (int p = 0; p < NP; p += 2) {
+                    // the pair's pieces change places: those of piece p and p + 1 become the even row's and the odd row's
+#pragma unroll
+                    for (int e = 0; e < PN / 4; ++e) pair_swap(acc[p * (PN / 4) + e], acc[(p + 1) * (PN / 4) + e]);
+#pragma unroll
+                    for (int o = p; o < p + 2; ++o) {
+                        typename Item::PT v;
+#pragma unroll
+                        for (int e = 0; e < PN; ++e) v[e] = (O) (acc[o * (PN / 4) + (e >> 2)][e & 3] + (float) s.res[i][o][e]);
+                        const int row = Item::row_of(i, o, lane), c = s.col_of(o, lane);
+                        if ((s.write >> row & 1) && c < a.n) *(typename Item::PT *) (obase + ((uint32_t) row * ldo + (uint32_t) c * (uint32_t) sizeof(O))) = v;
+                    }
+                }
+            } else if (s.write >> r & 1) {
+                const int64_t row = r0 + r;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = s.c0 + (PN == 4 ? 16 * j + 4 * q : 32 * (j >> 1) + 8 * q + 4 * (j & 1)), n = min(4, a.n - c);
+                    if (n <= 0) continue;
+                    float o[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+                    if (a.resid) add_n<T, 4>(a.resid, row * a.ldr + c, o, n, PN == 4, a.vec);
+                    put_n<T, 4>(a.out, row * a.ldo + c, o, n, PN == 4, a.vec);
+                }
+            }
         }
-    }
-    // this block's rows; those without an adapter are the first blocks'
-    const uint64_t none = __ballot(id < 0 && lane < ROWS && r0 + lane < a.m);
-    const uint64_t write = blockIdx.z == 0 && !(a.resid == a.out && a.ldr == a.ldo) ? rows | none : rows;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        if (!(write >> (16 * i + i16) & 1)) continue;
-        const int64_t row = r0 + 16 * i + i16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = c0 + 16 * q + 8 * h, n = min(8, a.n - c);
-            if (n <= 0) continue;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = out[i][2 * h + (e >> 2)][e & 3];
-            if (a.resid) add_n<T, 8>(a.resid, row * a.ldr + c, v, n, a.out_f32, a.vec);
-            put_n<T, 8>(a.out, row * a.ldo + c, v, n, a.out_f32, a.vec);
+    };
+    // the item's own loads have come when only the next one's are out (told to the compiler here: behind stores that only some lanes
+    // make it could not count, and would wait for the next item's loads as well)
+    auto arrived = [] {
+        constexpr int L = Item::LOADS;
+        lora_keep_order();
+        __builtin_amdgcn_s_waitcnt((L & 15) | 0x0F70 | (L >> 4 & 3) << 14);
+        lora_keep_order();
+    };
+    if ((blk % gy * 4 + wave) * 64 >= a.n) return;
+    if constexpr (AL && KK <= 2) {
+        for (;;) {
+            if (c0 >= a.n) { work(s0); break; }   // (the last item)
+            next(s1);
+            arrived();
+            work(s0);
+            if (c0 >= a.n) { work(s1); break; }
+            next(s0);
+            arrived();
+            work(s1);
+        }
+    } else {   // (two items of high rank do not fit the registers)
+        for (;;) {
+            work(s0);
+            if (c0 >= a.n) break;
+            next(s0);
         }
     }
 }
 
-// Parts of at least 256 values of the contraction, as many as make 512 blocks of 16 rows
+// Few rows: tiles of 16, parts of at least 256 values of the contraction.  Many: tiles of 32, parts of at least 1024 (the second
+// launch reads every part again).  As many parts as make 512 blocks.
+constexpr int LORA_MANY = 256;
 LoraCut lora_cut(int m, int k) {
-    const int tiles = (m + 15) / 16, most = std::max(1, std::min(32, (k + 255) / 256));
+    const bool many = m >= LORA_MANY;
+    const int rows = many ? 32 : 16, least = many ? 1024 : 256;
+    const int tiles = (m + rows - 1) / rows, most = std::max(1, std::min(32, (k + least - 1) / least));
     const int want = std::max(1, std::min(most, (512 + tiles - 1) / std::max(1, tiles)));
     const int klen = ((k + want - 1) / want + 255) / 256 * 256;
     return LoraCut{(int) (((int64_t) k + klen - 1) / klen), klen};
 }
 
+// how many of a tile's adapters go side by side, in blocks of their own
+static uint32_t lora_deal(int64_t blocks) { return (uint32_t) std::max<int64_t>(1, std::min<int64_t>(16, 1024 / std::max<int64_t>(1, blocks))); }
 static bool lora_al(const void *p, int64_t ld) { return ((uintptr_t) p & 15) == 0 && ld % 8 == 0; }
 
+template <typename T, typename O> static int launch_up(const LoraArgs &a, hipStream_t s) {
+    const bool al = lora_al(a.B, a.r) && a.vec && a.n % 8 == 0 && a.resid && a.ldr < 1 << 22 && a.ldo < 1 << 22, tall = a.r <= 64 && a.m >= LORA_MANY;
+    constexpr int TALL = sizeof(O) == 4 ? 2 : 4;   // row tiles whose residual fits the registers twice
+    const int tiles = tall ? (a.m + 16 * TALL - 1) / (16 * TALL) : (a.m + 15) / 16, cols = (a.n + 255) / 256;
+    // many rows: about two blocks a CU, that take several turns with their rows' low products
+    const int turns = std::max(1, (int) (((int64_t) tiles * cols + 511) / 512)), gy = (cols + turns - 1) / turns;
+    const dim3 up(tiles * gy, 1, tall ? 1 : lora_deal((int64_t) tiles * gy));
+#define HY_UP(RT, KK) { if (al) k_lora_up<T, O, RT, KK, true><<<up, 256, 0, s>>>(a, gy); else k_lora_up<T, O, RT, KK, false><<<up, 256, 0, s>>>(a, gy); }
+    if (a.r <= 32) { if (tall) HY_UP(TALL, 1) else HY_UP(1, 1) }
+    else if (a.r <= 64) { if (tall) HY_UP(TALL, 2) else HY_UP(1, 2) }
+    else if (a.r <= 128) HY_UP(1, 4)
+    else HY_UP(1, 8)
+#undef HY_UP
+    return check_launch("hy_lora");
+}
 template <typename T> static int launch_lora_t(const LoraArgs &a, hipStream_t s) {
-    const char *what = "hy_lora";
-    const int tiles = (a.m + 15) / 16;
-    const bool alx = lora_al(a.x, a.ldx) && a.k % 8 == 0, ala = lora_al(a.A, a.k), alb = lora_al(a.B, a.r);
-    const dim3 low(tiles, a.splits, std::max(1, std::min(16, 1024 / std::max(1, tiles * a.splits))));
-#define HY_LOW(RT) { if (alx && ala) k_lora_low<T, RT, true, true><<<low, 256, 0, s>>>(a); \
-                     else k_lora_low<T, RT, false, false><<<low, 256, 0, s>>>(a); }
+    const bool many = a.m >= LORA_MANY, al = lora_al(a.x, a.ldx) && lora_al(a.A, a.k);
+    const int tiles = (a.m + (many ? 31 : 15)) / (many ? 32 : 16);
+    const dim3 low(tiles * a.splits, 1, many ? 4 : lora_deal((int64_t) tiles * a.splits));
+#define HY_LOW(RT) { if (many) { if (al) k_lora_low<T, RT, 2, true><<<low, 256, 0, s>>>(a); else k_lora_low<T, RT, 2, false><<<low, 256, 0, s>>>(a); } \
+                     else { if (al) k_lora_low<T, RT, 1, true><<<low, 256, 0, s>>>(a); else k_lora_low<T, RT, 1, false><<<low, 256, 0, s>>>(a); } }
     if (a.r <= 16) HY_LOW(1) else if (a.r <= 32) HY_LOW(2) else HY_LOW(4)
 #undef HY_LOW
-    if (const int rc = check_launch(what)) return rc;
-    const int cols = (a.n + 255) / 256;
-    const bool tall = a.r <= 64 && a.m >= 256;
-    const int rt = tall ? (a.m + 63) / 64 : tiles;
-    const dim3 up(rt, cols, std::max(1, std::min(16, 1024 / std::max(1, rt * cols))));
-#define HY_UP(RT, R) { if (alb) k_lora_up<T, RT, R, true><<<up, 256, 0, s>>>(a); else k_lora_up<T, RT, R, false><<<up, 256, 0, s>>>(a); }
-    if (a.r <= 32) { if (tall) HY_UP(4, 32) else HY_UP(1, 32) }
-    else if (a.r <= 64) { if (tall) HY_UP(4, 64) else HY_UP(1, 64) }
-    else if (a.r <= 128) HY_UP(1, 128)
-    else HY_UP(1, 256)
-#undef HY_UP
-    return check_launch(what);
+    if (const int rc = check_launch("hy_lora")) return rc;
+    return a.out_f32 ? launch_up<T, float>(a, s) : launch_up<T, T>(a, s);
 }
 int launch_lora(int type, const LoraArgs &a, hipStream_t s) { return type == HY_BF16 ? launch_lora_t<bf16>(a, s) : launch_lora_t<f16>(a, s); }
 
