@@ -12,65 +12,70 @@
 
 namespace hy {
 
-// A thread's V pieces of 8 values of a row that T threads share.  VEC: piece j is columns 8 (j T + t) .. + 7, moved in 16-byte
-// pieces; else its value i is column (8 j + i) T + t, so that neighbouring threads touch neighbouring values.
-template <int T, bool VEC> __device__ __forceinline__ int norm_col(int t, int j, int i) { return VEC ? 8 * (j * T + t) + i : (8 * j + i) * T + t; }
+// A thread's 8 V values of a row that T threads share.  VEC: in pieces of 16 bytes of the row's type X (PW = 4 or 8 neighbours),
+// piece p at column PW (p T + t), so that neighbouring threads move neighbouring pieces (fp32 rows by 8 neighbours a thread instead:
+// the gradient of 8192 x 4096 94 us for 86); else value k is column k T + t.
+template <int T, int PW, bool VEC> __device__ __forceinline__ int norm_col(int t, int j, int i) {
+    return VEC ? PW * ((8 / PW * j + i / PW) * T + t) + i % PW : (8 * j + i) * T + t;
+}
+template <typename Y, int PW> using Neighbours = Y __attribute__((ext_vector_type(PW)));
 
-template <typename X> __device__ __forceinline__ void norm_ld8(const X *p, float (&v)[8]) {
-    if constexpr (sizeof(X) == 4) {
-        const f4 a = *(const f4 *) p, b = *(const f4 *) (p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-    } else {
-        const v8<X> a = *(const v8<X> *) p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float) a[i];
-    }
-}
-template <typename X> __device__ __forceinline__ void norm_st8(X *p, const float (&v)[8]) {
-    if constexpr (sizeof(X) == 4) {
-        *(f4 *) p = f4{v[0], v[1], v[2], v[3]};
-        *(f4 *) (p + 4) = f4{v[4], v[5], v[6], v[7]};
-    } else {
-        v8<X> a;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = (X) v[i];
-        *(v8<X> *) p = a;
-    }
-}
-// piece j of a row of n values, zeros behind its end
-template <typename X, int T, bool VEC> __device__ __forceinline__ void norm_load(const X *row, int t, int j, int n, float (&v)[8]) {
+// a thread's values 8 j .. + 7 of a row of n values, zeros behind its end.  Y: the type of this row, whose columns go by PW
+template <typename Y, int T, int PW, bool VEC> __device__ __forceinline__ void norm_load(const Y *row, int t, int j, int n, float (&v)[8]) {
     if constexpr (VEC) {
-        const int c = norm_col<T, true>(t, j, 0);
-        if (c + 8 <= n) { norm_ld8<X>(row + c, v); return; }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = norm_col<T, VEC>(t, j, i);
-        v[i] = c < n ? (float) row[c] : 0.0f;
+        for (int h = 0; h < 8; h += PW) {
+            const int c = norm_col<T, PW, true>(t, j, h);
+            if (c + PW <= n) {
+                const Neighbours<Y, PW> a = *(const Neighbours<Y, PW> *) (row + c);
+#pragma unroll
+                for (int i = 0; i < PW; ++i) v[h + i] = (float) a[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < PW; ++i) v[h + i] = c + i < n ? (float) row[c + i] : 0.0f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = norm_col<T, PW, false>(t, j, i);
+            v[i] = c < n ? (float) row[c] : 0.0f;
+        }
     }
 }
-template <typename X, int T, bool VEC> __device__ __forceinline__ void norm_store(X *row, int t, int j, int n, const float (&v)[8]) {
+template <typename Y, int T, int PW, bool VEC> __device__ __forceinline__ void norm_store(Y *row, int t, int j, int n, const float (&v)[8]) {
     if constexpr (VEC) {
-        const int c = norm_col<T, true>(t, j, 0);
-        if (c + 8 <= n) { norm_st8<X>(row + c, v); return; }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = norm_col<T, VEC>(t, j, i);
-        if (c < n) row[c] = (X) v[i];
+        for (int h = 0; h < 8; h += PW) {
+            const int c = norm_col<T, PW, true>(t, j, h);
+            if (c + PW <= n) {
+                Neighbours<Y, PW> a;
+#pragma unroll
+                for (int i = 0; i < PW; ++i) a[i] = (Y) v[h + i];
+                *(Neighbours<Y, PW> *) (row + c) = a;
+            } else {
+#pragma unroll
+                for (int i = 0; i < PW; ++i) if (c + i < n) row[c + i] = (Y) v[h + i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = norm_col<T, PW, false>(t, j, i);
+            if (c < n) row[c] = (Y) v[i];
+        }
     }
 }
 // the same where the type is known at run time only (the same for every thread)
-template <int T, bool VEC> __device__ __forceinline__ void norm_load_as(int type, const void *base, int64_t at, int t, int j, int n, float (&v)[8]) {
-    if (type == HY_F32) norm_load<float, T, VEC>((const float *) base + at, t, j, n, v);
-    else if (type == HY_BF16) norm_load<bf16, T, VEC>((const bf16 *) base + at, t, j, n, v);
-    else norm_load<f16, T, VEC>((const f16 *) base + at, t, j, n, v);
+template <int T, int PW, bool VEC> __device__ __forceinline__ void norm_load_as(int type, const void *base, int64_t at, int t, int j, int n, float (&v)[8]) {
+    if (type == HY_F32) norm_load<float, T, PW, VEC>((const float *) base + at, t, j, n, v);
+    else if (type == HY_BF16) norm_load<bf16, T, PW, VEC>((const bf16 *) base + at, t, j, n, v);
+    else norm_load<f16, T, PW, VEC>((const f16 *) base + at, t, j, n, v);
 }
-template <int T, bool VEC> __device__ __forceinline__ void norm_store_as(int type, void *base, int64_t at, int t, int j, int n, const float (&v)[8]) {
-    if (type == HY_F32) norm_store<float, T, VEC>((float *) base + at, t, j, n, v);
-    else if (type == HY_BF16) norm_store<bf16, T, VEC>((bf16 *) base + at, t, j, n, v);
-    else norm_store<f16, T, VEC>((f16 *) base + at, t, j, n, v);
+template <int T, int PW, bool VEC> __device__ __forceinline__ void norm_store_as(int type, void *base, int64_t at, int t, int j, int n, const float (&v)[8]) {
+    if (type == HY_F32) norm_store<float, T, PW, VEC>((float *) base + at, t, j, n, v);
+    else if (type == HY_BF16) norm_store<bf16, T, PW, VEC>((bf16 *) base + at, t, j, n, v);
+    else norm_store<f16, T, PW, VEC>((f16 *) base + at, t, j, n, v);
 }
 
 // the sum of v over the T threads of a row; `s`: this row's T / 64 floats of LDS, written anew by each call
@@ -88,19 +93,19 @@ template <int T> __device__ __forceinline__ float row_sum(float v, float *s) {
 
 constexpr int NORM_BLOCKS = 1 << 20;   // most blocks of a launch: they go on to further rows
 
-// T threads a row of up to 8 V T values, max(T, 256) threads a block
-template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T < 256 ? 256 : T) void k_norm(const NormArgs a) {
-    constexpr int NT = T < 256 ? 256 : T, G = NT / T;
+// T threads a row of up to 8 V T values; a block has one row, or four of a wave each (T = 64: no barrier)
+template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
+    constexpr int NT = T == 64 ? 256 : T, G = NT / T, PW = 16 / sizeof(X);
     __shared__ float s_sum[3][NT / 64];
     const int t = threadIdx.x % T;
     for (int64_t row = (int64_t) blockIdx.x * G + threadIdx.x / T; row < a.m; row += (int64_t) gridDim.x * G) {
         float v[V][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) norm_load<X, T, VEC>((const X *) a.x + row * a.ldx, t, j, a.n, v[j]);
+        for (int j = 0; j < V; ++j) norm_load<X, T, PW, VEC>((const X *) a.x + row * a.ldx, t, j, a.n, v[j]);
         if (a.add) {
             float d[V][8];
 #pragma unroll
-            for (int j = 0; j < V; ++j) norm_load<X, T, VEC>((const X *) a.add + row * a.lda, t, j, a.n, d[j]);
+            for (int j = 0; j < V; ++j) norm_load<X, T, PW, VEC>((const X *) a.add + row * a.lda, t, j, a.n, d[j]);
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -108,7 +113,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T < 2
         }
         if (a.total) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) norm_store<X, T, VEC>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
+            for (int j = 0; j < V; ++j) norm_store<X, T, PW, VEC>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
         }
         float mu = 0.0f, q = 0.0f;
         if (a.layer) {
@@ -121,7 +126,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T < 2
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (norm_col<T, VEC>(t, j, i) < a.n) e += v[j][i] - mu;
+                for (int i = 0; i < 8; ++i) if (norm_col<T, PW, VEC>(t, j, i) < a.n) e += v[j][i] - mu;
             mu += row_sum<T>(e, s_sum[2]) / (float) a.n;
         }
 #pragma unroll
@@ -129,7 +134,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T < 2
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 v[j][i] -= mu;
-                if (norm_col<T, VEC>(t, j, i) < a.n) q = fmaf(v[j][i], v[j][i], q);
+                if (norm_col<T, PW, VEC>(t, j, i) < a.n) q = fmaf(v[j][i], v[j][i], q);
             }
         const float r = 1.0f / sqrtf(row_sum<T>(q, s_sum[1]) / (float) a.n + a.eps);
         if (t == 0) {
@@ -138,20 +143,20 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T < 2
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (norm_col<T, VEC>(t, j, 0) >= a.n) continue;
+            if (norm_col<T, PW, VEC>(t, j, 0) >= a.n) continue;
             float w[8], y[8];
-            norm_load<float, T, VEC>(a.w, t, j, a.n, w);
+            norm_load<float, T, PW, VEC>(a.w, t, j, a.n, w);
             if (a.b) {
                 float b[8];
-                norm_load<float, T, VEC>(a.b, t, j, a.n, b);
+                norm_load<float, T, PW, VEC>(a.b, t, j, a.n, b);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = fmaf(v[j][i] * r, w[i], b[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = v[j][i] * r * w[i];
             }
-            if (a.out) norm_store_as<T, VEC>(a.o_type, a.out, row * a.ldo, t, j, a.n, y);
-            if (a.out32) norm_store<float, T, VEC>(a.out32 + row * a.ldo32, t, j, a.n, y);
+            if (a.out) norm_store_as<T, PW, VEC>(a.o_type, a.out, row * a.ldo, t, j, a.n, y);
+            if (a.out32) norm_store<float, T, PW, VEC>(a.out32 + row * a.ldo32, t, j, a.n, y);
         }
         if constexpr (T > 64) lds_barrier();   // the sums are read before the next row's are written
     }
@@ -194,15 +199,15 @@ template <typename X> __global__ __launch_bounds__(1024) void k_norm_long(const 
 
 template <typename X, bool VEC> static void launch_norm_t(const NormArgs &a, hipStream_t s) {
     auto grid = [&](int rows) { return dim3((uint32_t) std::min<int64_t>(((int64_t) a.m + rows - 1) / rows, NORM_BLOCKS)); };
-#define HY_NORM(T, V) k_norm<X, T, V, VEC><<<grid(T < 256 ? 256 / T : 1), T < 256 ? 256 : T, 0, s>>>(a)
+#define HY_NORM(T, V) k_norm<X, T, V, VEC><<<grid(T == 64 ? 4 : 1), T == 64 ? 256 : T, 0, s>>>(a)
     if (a.n > 16384) { k_norm_long<X><<<grid(1), 1024, 0, s>>>(a); return; }
+    // 8 values a thread: a row in the registers of one wave (n 4096: 64 a thread) keeps too few rows of a CU under way (8192 x 4096:
+    // 64 values a thread 114 us, 32 95, 16 85, 8 82)
     if (a.n <= 512) HY_NORM(64, 1);
-    else if (a.m >= 1024 && a.n <= 1024) HY_NORM(64, 2);
-    else if (a.m >= 1024 && a.n <= 2048) HY_NORM(64, 4);
-    else if (a.m >= 1024 && a.n <= 4096) HY_NORM(64, 8);
+    else if (a.n <= 1024) HY_NORM(128, 1);
     else if (a.n <= 2048) HY_NORM(256, 1);
-    else if (a.n <= 4096) HY_NORM(256, 2);
-    else if (a.n <= 8192) { if (a.m >= 1024) HY_NORM(256, 4); else HY_NORM(1024, 1); }
+    else if (a.n <= 4096) HY_NORM(512, 1);
+    else if (a.n <= 8192) HY_NORM(1024, 1);
     else HY_NORM(1024, 2);
 #undef HY_NORM
 }
@@ -215,50 +220,46 @@ int launch_norm(int x_type, const NormArgs &a, bool vec, hipStream_t s) {
 
 // ------------------------------------------------------------------ backward
 
-constexpr int NB_T = 512;         // threads a block: NB_T / T rows at a time
-constexpr int NB_BLOCKS = 512;    // most blocks: two a CU
-constexpr int NB_LONG = 8192;    // longer rows than this take k_norm_bwd_long
-
-__host__ __device__ constexpr int nb_threads(int n) { return n <= 1024 ? 64 : n <= 4096 ? 256 : NB_T; }   // threads a row
+// 8 values a thread here too: 16 of them (and their sums, 16 or 32 more) leave one block a CU (8192 x 4096 fp32: 104 us for 87).
+// Three blocks of 512 threads a CU and two of 1024; with two of 512 87.5 us for 85.7, with four 94 (more sums to join).
+constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
+__host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
+__host__ __device__ constexpr int nb_block_threads(int T) { return T < 512 ? 512 : T; }
 
 int norm_bwd_parts(int m, int n) {
-    const int g = n > NB_LONG ? 16 : NB_T / nb_threads(n);
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, NB_BLOCKS);
+    const int T = nb_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 512 : 768);
 }
 
-// T threads a row, NB_T / T rows at a time; block b takes rows G b .. + G - 1 of every G gridDim.x
-template <typename X, int T, int V, bool LAYER, bool VEC> __global__ __launch_bounds__(NB_T) void k_norm_bwd(const NormBwdArgs a) {
-    constexpr int G = NB_T / T, W = T / 64, COLS = 8 * V * T;
-    __shared__ float s_sum[2][2][NB_T / 64];
+// T threads a row of up to 8 T values, G rows at a time; block b takes rows G b .. + G - 1 of every G gridDim.x
+template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64, COLS = 8 * T, PW = 16 / sizeof(X);
+    __shared__ float s_sum[2][2][NT / 64];
     __shared__ float s_join[G > 1 ? G * COLS : 1];
     const int t = threadIdx.x % T, g = threadIdx.x / T, wave = threadIdx.x >> 6;
-    float dw[V][8] = {}, db[LAYER ? V : 1][8] = {};
+    float dw[8] = {}, db[8] = {};
     int turn = 0;
     for (int64_t first = (int64_t) blockIdx.x * G; first < a.m; first += (int64_t) gridDim.x * G, turn ^= 1) {
         const int64_t row = first + g;
         const bool on = row < a.m;   // (the other threads go along for the barriers)
-        float x[V][8], dy[V][8], c1 = 0.0f, c2 = 0.0f, r = 0.0f, mu = 0.0f;
+        float x[8], dy[8], e[8] = {}, c1 = 0.0f, c2 = 0.0f, r = 0.0f, mu = 0.0f;
         if (on) {
+            float w[8];
             r = a.rstd[row];
             if (LAYER) mu = a.mean[row];
+            norm_load<X, T, PW, VEC>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
+            norm_load_as<T, PW, VEC>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
+            norm_load<float, T, PW, VEC>(a.w, t, 0, a.n, w);
+            if (a.resid) norm_load<X, T, PW, VEC>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
-            for (int j = 0; j < V; ++j) norm_load<X, T, VEC>((const X *) a.x + row * a.ldx, t, j, a.n, x[j]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) norm_load_as<T, VEC>(a.y_type, a.dy, row * a.ldy, t, j, a.n, dy[j]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float w[8];
-                norm_load<float, T, VEC>(a.w, t, j, a.n, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float h = (x[j][i] - mu) * r;
-                    dw[j][i] = fmaf(dy[j][i], h, dw[j][i]);
-                    if (LAYER) db[j][i] += dy[j][i];
-                    x[j][i] = h;
-                    dy[j][i] *= w[i];   // zeros behind the row's end
-                    if (LAYER) c1 += dy[j][i];
-                    c2 = fmaf(dy[j][i], h, c2);
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float h = (x[i] - mu) * r;
+                dw[i] = fmaf(dy[i], h, dw[i]);
+                if (LAYER) db[i] += dy[i];
+                x[i] = h;
+                dy[i] *= w[i];   // zeros behind the row's end
+                if (LAYER) c1 += dy[i];
+                c2 = fmaf(dy[i], h, c2);
             }
         }
         c2 = wave_sum_xor(c2);
@@ -270,23 +271,13 @@ template <typename X, int T, int V, bool LAYER, bool VEC> __global__ __launch_bo
 #pragma unroll
             for (int i = 0; i < W; ++i) { c2 += s_sum[turn][0][g * W + i]; if (LAYER) c1 += s_sum[turn][1][g * W + i]; }
         }
-        if (on) {
+        if (on && norm_col<T, PW, VEC>(t, 0, 0) < a.n) {
             c1 /= (float) a.n;
             c2 /= (float) a.n;
+            float o[8];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (norm_col<T, VEC>(t, j, 0) >= a.n) continue;
-                float o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[j][i] - c1 : dy[j][i]) - x[j][i] * c2);
-                if (a.resid) {
-                    float e[8];
-                    norm_load<X, T, VEC>((const X *) a.resid + row * a.ldr, t, j, a.n, e);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] += e[i];
-                }
-                norm_store<X, T, VEC>((X *) a.dx + row * a.ldd, t, j, a.n, o);
-            }
+            for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[i] - c1 : dy[i]) - x[i] * c2) + e[i];
+            norm_store<X, T, PW, VEC>((X *) a.dx + row * a.ldd, t, 0, a.n, o);
         }
     }
     // the block's sums: over its G rows, in their order
@@ -299,11 +290,9 @@ template <typename X, int T, int V, bool LAYER, bool VEC> __global__ __launch_bo
         if constexpr (G > 1) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s_join[g * COLS + norm_col<T, VEC>(t, j, i)] = which ? db[LAYER ? j : 0][i] : dw[j][i];
+            for (int i = 0; i < 8; ++i) s_join[g * COLS + norm_col<T, PW, VEC>(t, 0, i)] = which ? db[i] : dw[i];
             __syncthreads();
-            for (int c = threadIdx.x; c < a.n; c += NB_T) {
+            for (int c = threadIdx.x; c < a.n; c += NT) {
                 float v = 0.0f;
 #pragma unroll
                 for (int k = 0; k < G; ++k) v += s_join[k * COLS + c];
@@ -311,13 +300,11 @@ template <typename X, int T, int V, bool LAYER, bool VEC> __global__ __launch_bo
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int c = norm_col<T, VEC>(t, j, i);
-                    const float v = which ? db[LAYER ? j : 0][i] : dw[j][i];
-                    if (c < a.n) to[c] = acc ? to[c] + v : v;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int c = norm_col<T, PW, VEC>(t, 0, i);
+                const float v = which ? db[i] : dw[i];
+                if (c < a.n) to[c] = acc ? to[c] + v : v;
+            }
         }
     }
 }
@@ -393,12 +380,14 @@ __global__ __launch_bounds__(256) void k_norm_zero(float *dw, float *db, int n) 
 template <typename X, bool LAYER, bool VEC> static void launch_norm_bwd_t(const NormBwdArgs &a, hipStream_t s) {
     const dim3 grid(a.parts);
     const int n = a.n;
-#define HY_NB(T, V) k_norm_bwd<X, T, V, LAYER, VEC><<<grid, NB_T, 0, s>>>(a)
-    if (n <= 512) HY_NB(64, 1);
-    else if (n <= 1024) HY_NB(64, 2);
-    else if (n <= 2048) HY_NB(256, 1);
-    else if (n <= 4096) HY_NB(256, 2);
-    else HY_NB(512, 2);
+#define HY_NB(T) k_norm_bwd<X, T, LAYER, VEC><<<grid, nb_block_threads(T), 0, s>>>(a)
+    switch (nb_row_threads(n)) {
+    case 64: HY_NB(64); break;
+    case 128: HY_NB(128); break;
+    case 256: HY_NB(256); break;
+    case 512: HY_NB(512); break;
+    default: HY_NB(1024);
+    }
 #undef HY_NB
 }
 template <typename X> static void launch_norm_bwd_x(bool layer, const NormBwdArgs &a, bool vec, hipStream_t s) {
