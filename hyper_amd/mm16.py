@@ -5,8 +5,11 @@ The functions call libhymoe's C ABI (include/hymoe.h) and write into tensors the
 raises ValueError here or HyError from the library.  They run on `stream` (None: the current stream of the tensors'
 device).  Matrices are row-major with contiguous rows; rows may lie apart (views of wider tensors).
 
-Moe16LayerRunner strings them together for one layer: router, routing, grouping, gate/up, down, combine, and the backward
-pass of the experts.
+Beside them what stands around the products of a block: norms and their gradients, routing with groups of experts and its
+gradient, low-rank adapters of many requests.
+
+Moe16LayerRunner strings them together for one layer: norm, router, routing, grouping, gate/up, down, combine, and the backward
+pass.
 """
 import ctypes
 from typing import Optional
@@ -466,18 +469,40 @@ def lora(L: Lora16, x, ids, out, resid=None, ws=None, stream=None):
 
 # ------------------------------------------------------------------ one MoE layer
 
+class Norm16:
+    """The norm in front of a layer: weights w and b (float32, b None for an RMS norm), eps and kind as norm takes them."""
+
+    def __init__(self, w: torch.Tensor, b: Optional[torch.Tensor] = None, eps: float = 1e-5, kind: str = "rms"):
+        _named(NORMS, "norm", kind)
+        if kind == "rms" and b is not None:
+            raise ValueError("an RMS norm has no b")
+        _vec("w", w, 1, torch.float32)
+        _vec("b", b, w.numel(), torch.float32)
+        self.w, self.b, self.eps, self.kind = w, b, float(eps), kind
+
+
+class Router16:
+    """How route_groups routes a layer's tokens (its arguments but the logits and k)."""
+
+    def __init__(self, score="softmax", bias: Optional[torch.Tensor] = None, n_group=1, top_group=1, group_best=1, renorm=True, scale=1.0):
+        _named(SCORES, "score", score)
+        self.how = dict(score=score, bias=bias, n_group=n_group, top_group=top_group, group_best=group_best, renorm=renorm, scale=float(scale))
+
+
 class Moe16LayerRunner:
     """Workspace and call sequence for one MoE layer with 16-bit experts, as moe.MoeLayerRunner has it for quantized ones:
-    router GEMV, softmax routing, then by ids (up to `decode_rows` rows) or grouped: gate/up, down, combine.
+    router GEMV, softmax routing, then by ids (up to `decode_rows` rows) or grouped: gate/up, down, combine.  `norm`: a Norm16 in
+    front of it all; `router`: a Router16 in place of the softmax routing, which backward then covers as well.
 
     forward(x) takes [nt, d] float32 rows; pairs whose expert dev.slot does not hold at the time add nothing to the output.  With
     keep=True it keeps what backward(dy) needs, the slot table among it; backward is for layers whose experts were all local
     when the runner was made.  `shared`: an always-on expert (a Moe16Dev with one matrix) added with weight 1; backward leaves it
-    and the router out."""
+    out, and the router unless the runner was made with `router`."""
 
     decode_rows = 2   # by ids every pair reads its expert's matrices; grouped, an expert's rows share them
 
-    def __init__(self, dev: Moe16Dev, W_r: torch.Tensor, k: int, max_rows: int, shared: Optional[Moe16Dev] = None):
+    def __init__(self, dev: Moe16Dev, W_r: torch.Tensor, k: int, max_rows: int, shared: Optional[Moe16Dev] = None,
+                 norm: Optional[Norm16] = None, router: Optional[Router16] = None):
         if dev.gate is None or dev.down is None or dev.gate.dtype != dev.down.dtype:
             raise ValueError("the experts need gate, up and down of one type")
         if W_r.dtype not in (torch.float32, torch.bfloat16) or W_r.dim() != 2 or not W_r.is_contiguous() or \
@@ -490,7 +515,12 @@ class Moe16LayerRunner:
         if shared is not None and (shared.gate is None or shared.down is None or shared.n != dev.n or shared.gate.dtype != dev.gate.dtype
                                    or shared.down.dtype != dev.gate.dtype):
             raise ValueError("the shared expert must have the experts' d_model and type")
+        if norm is not None and (norm.w.numel() != dev.n or norm.w.device != W_r.device):
+            raise ValueError(f"the norm must have {dev.n} weights on {W_r.device}")
+        if router is not None and router.how["bias"] is not None:
+            _vec("the router's bias", router.how["bias"], dev.slot.numel(), torch.float32)
         self.dev, self.W_r, self.k, self.shared, self.max_rows = dev, W_r, k, shared, int(max_rows)
+        self.norm, self.router = norm, router
         self.E, self.d, self.ff, self.dtype, device = dev.slot.numel(), dev.n, dev.ff, dev.gate.dtype, W_r.device
         T, P = self.max_rows, self.max_rows * k
         new = lambda *s, dtype=self.dtype: torch.empty(*s, dtype=dtype, device=device)  # noqa: E731
@@ -501,7 +531,9 @@ class Moe16LayerRunner:
         self.out = new(T, self.d, dtype=torch.float32)
         self.sh_y = new(T, self.d, dtype=torch.float32) if shared is not None else None
         self.sh_h = new(T, shared.ff) if shared is not None else None
-        self.g = self.u = self.kept_dev = None
+        self.xn = new(T, self.d, dtype=torch.float32) if norm is not None else None   # the router's rows
+        self.mean, self.rstd = (new(T, dtype=torch.float32), new(T, dtype=torch.float32)) if norm is not None else (None, None)
+        self.g = self.u = self.kept_dev = self.x_in = None
         self.kept = None   # rows of the last forward(keep=True); None: there was another one since, or none
 
     def _rows(self, x):
@@ -528,12 +560,22 @@ class Moe16LayerRunner:
             if keep and self.g is None:
                 self.g, self.u = torch.empty_like(self.h), torch.empty_like(self.h)
                 self.kept_dev = Moe16Dev(self.dev.gate, self.dev.up, self.dev.down, torch.empty_like(self.dev.slot), self.dev.clamp)
+                self.x_in = torch.empty_like(self.xn) if self.norm is not None else None
             if nt == 0:
                 self.kept = 0 if keep else None
                 return self.out[:0]
-            moe.gemv_f32(self.W_r, self.E, self.d, x, x.stride(0), self.logits, self.E, nt, stream)
-            moe.moe_route(self.logits, self.E, self.E, k, self.ids, self.wts, None, nt, stream)
-            rows16(x, self.x16[:nt], stream)
+            N = self.norm
+            if N is not None:
+                norm(x, N.w, self.x16[:nt], b=N.b, eps=N.eps, kind=N.kind, total=self.x_in[:nt] if keep else None, out32=self.xn[:nt],
+                     mean=self.mean if N.kind == "layer" else None, rstd=self.rstd, stream=stream)
+            rows = x if N is None else self.xn
+            moe.gemv_f32(self.W_r, self.E, self.d, rows, rows.stride(0), self.logits, self.E, nt, stream)
+            if self.router is None:
+                moe.moe_route(self.logits, self.E, self.E, k, self.ids, self.wts, None, nt, stream)
+            else:
+                route_groups(self.logits[:nt], self.ids[:P].view(nt, k), self.wts[:P].view(nt, k), stream=stream, **self.router.how)
+            if N is None:
+                rows16(x, self.x16[:nt], stream)
             how = dict(ids=self.ids) if nt <= self.decode_rows and not keep else self._group(nt, stream)
             gu = {}
             if keep:
@@ -549,10 +591,20 @@ class Moe16LayerRunner:
         self.kept = nt if keep else None
         return self.out[:nt]
 
-    def backward(self, dy: torch.Tensor, stream=None) -> dict:
+    def backward(self, dy: torch.Tensor, stream=None, dx_add: Optional[torch.Tensor] = None, resid: Optional[torch.Tensor] = None) -> dict:
         """Gradients of the routed experts for the last forward(keep=True): dy [nt, d] float32 -> {"dx": [nt, d] float32 (the
-        experts' part), "dwts": [nt, k] (of the routing weights), "gate", "up", "down": float32}."""
+        experts' part), "dwts": [nt, k] (of the routing weights), "gate", "up", "down": float32}.
+
+        Made with `router`: also "W_r" (float32), and the router's part in dx.  Made with `norm`: dx is that of the rows before the
+        norm, and "norm_w", "norm_b" (float32, norm_b None for an RMS norm) are added.  dx_add [nt, d] float32: what else the rows that
+        the experts see get (from a shared expert), added to theirs; resid [nt, d] float32, with `norm`: the gradient that passes by on
+        the residual stream, added to dx."""
         nt, k = self._rows(dy), self.k
+        for name, t in (("dx_add", dx_add), ("resid", resid)):
+            if t is not None:
+                _pairs(name, t, nt, self.d, torch.float32)
+        if resid is not None and self.norm is None:
+            raise ValueError("resid goes with a norm")
         if nt != self.kept:
             raise ValueError("backward follows forward(keep=True) of the same rows")
         if not self.all_local:
@@ -569,8 +621,25 @@ class Moe16LayerRunner:
             swiglu_bwd(self.g[:P], self.u[:P], dh, self.wts[:P], dg, du, hw, dwts.view(-1), clamp=dev.clamp,
                        order=self.order, order_n=self.order_n)
             moe16_gate_up_dx(dev, dg, du, P, *grp, dxp)
-            moe16_reduce(dev, None, None, dxp, k, dx, nt, self.ids)
+            moe16_reduce(dev, dx_add, None, dxp, k, dx, nt, self.ids)
             moe16_dw(dev, dg, 1, self.x16[:nt], k, P, *grp, W["gate"])
             moe16_dw(dev, du, 1, self.x16[:nt], k, P, *grp, W["up"])
             moe16_dw(dev, dy16, k, hw, 1, P, *grp, W["down"])
+            if self.router is not None:
+                # the logits' gradient in the experts' type, as every product's operands here (half a step of it in each)
+                dl, W["W_r"] = new(nt, self.E), new(self.E, self.d, dtype=torch.float32)
+                how = self.router.how
+                route_groups_bwd(self.logits[:nt], self.ids[:P].view(nt, k), dwts, dl, score=how["score"], renorm=how["renorm"], scale=how["scale"])
+                ws = new(linear_dw_ws_bytes(nt, self.E, self.d), dtype=torch.uint8)
+                linear_dw(dl, self.x16[:nt], W["W_r"], ws=ws)
+                W_r = self.W_r if self.W_r.dtype == self.dtype else self.W_r.to(self.dtype)
+                linear_dx(W_r, dl, dx, resid=dx)
+            if self.norm is not None:
+                N, dxn = self.norm, dx
+                dx = torch.empty_like(dxn)
+                W["norm_w"] = new(self.d, dtype=torch.float32)
+                W["norm_b"] = new(self.d, dtype=torch.float32) if N.b is not None else None
+                ws = new(norm_bwd_ws_bytes(nt, self.d), dtype=torch.uint8)
+                norm_bwd(self.x_in[:nt], dxn, N.w, self.rstd, dx, mean=self.mean if N.kind == "layer" else None, kind=N.kind, resid=resid,
+                         dw=W["norm_w"], db=W["norm_b"], ws=ws)
         return {"dx": dx, "dwts": dwts, **W}
