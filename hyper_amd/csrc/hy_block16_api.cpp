@@ -74,14 +74,12 @@ int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, i
     a.x = x; a.add = add; a.total = total; a.out = out; a.out32 = out32; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd;
     a.ldx = ldx; a.lda = ldadd; a.ldt = ldt; a.ldo = ldo; a.ldo32 = ldo32; a.m = m; a.n = n; a.o_type = out_type; a.eps = eps;
     a.layer = kind == HY_NORM_LAYER;
-    const bool vec = vec16(x, ldx, xb) && vec16(add, ldadd, xb) && vec16(total, ldt, xb) && vec16(out, ldo, ob) && vec16(out32, ldo32, 4) &&
-                     !misaligned(w, 16) && !misaligned(b, 16);
-    return launch_norm(x_type, a, vec, s);
+    return launch_norm(x_type, a, s);
 }
 
 size_t hy_norm_bwd_ws_bytes(int m, int n) {
     if (m <= 0 || n <= 0 || n > HY_NORM_MAX) return 0;
-    const int parts = norm_bwd_parts(m, n);
+    const int parts = norm_bwd_parts(m, n, false);
     return parts > 1 ? 2 * sizeof(float) * (size_t) parts * (size_t) n : 0;
 }
 
@@ -109,10 +107,9 @@ int hy_norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, c
     NormBwdArgs a{};
     a.x = x; a.dy = dy; a.resid = resid; a.dx = dx; a.w = w; a.mean = kind == HY_NORM_LAYER ? mean : nullptr; a.rstd = rstd; a.dw = dw; a.db = db;
     a.ldx = ldx; a.ldy = lddy; a.ldr = ldr; a.ldd = lddx; a.m = m; a.n = n; a.y_type = dy_type; a.accumulate = accumulate != 0;
-    a.parts = m ? norm_bwd_parts(m, n) : 0;
+    a.parts = m ? norm_bwd_parts(m, n, x_type == HY_F32) : 0;
     a.part = a.parts > 1 ? (float *) ws : nullptr;
-    const bool vec = vec16(x, ldx, xb) && vec16(dy, lddy, yb) && vec16(resid, ldr, xb) && vec16(dx, lddx, xb) && !misaligned(w, 16);
-    return launch_norm_bwd(x_type, kind == HY_NORM_LAYER, a, vec, s);
+    return launch_norm_bwd(x_type, kind == HY_NORM_LAYER, a, s);
 }
 
 int hy_moe_route_groups(const float *logits, int64_t ls, int n_expert, const float *bias, int score, int n_group, int top_group, int group_best,
@@ -168,12 +165,11 @@ int hy_lora(int type, const void *A, const void *B, const float *scale, int n_lo
     HY_TRY(check_ws(what, ws, ws_bytes, hy_lora_ws_bytes(m, r, k)));
     const LoraCut cut = lora_cut(m, k);
     HY_TRY(check_blocks(what, (int64_t) ((m + 15) / 16) * ((n + 255) / 256)));
-    if ((n + 255) / 256 > 65535) { set_error("%s: n %d (up to 2^24 - 256)", what, n); return HY_EBAD_SHAPE; }
+    if (ldo > HY_LORA_MAX_STRIDE || (resid && ldr > HY_LORA_MAX_STRIDE) || n > HY_LORA_MAX_STRIDE) { set_error("%s: rows of out or resid more than 2^22 values apart", what); return HY_EBAD_SHAPE; }
     LoraArgs a{};
     a.A = A; a.B = B; a.x = x; a.scale = scale; a.ids = ids; a.resid = resid; a.out = out; a.low = (float *) ws;
     a.ldx = ldx; a.ldr = ldr; a.ldo = ldo; a.m = m; a.n = n; a.k = k; a.r = r; a.n_local = n_local;
     a.splits = cut.splits; a.klen = cut.klen; a.out_f32 = out_type == HY_F32;
-    a.vec = vec16(out, ldo, ob) && vec16(resid, ldr, ob);
     return launch_lora(type, a, s);
 }
 

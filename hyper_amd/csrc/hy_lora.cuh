@@ -15,7 +15,6 @@ struct LoraArgs {
     int m, n, k, r, n_local;
     int splits, klen;   // the contraction cut into `splits` parts of klen values
     int out_f32;
-    int vec;            // out and resid can be moved in 16-byte pieces
 };
 struct LoraCut { int splits, klen; };
 LoraCut lora_cut(int m, int k);

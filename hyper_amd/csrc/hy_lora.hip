@@ -14,14 +14,17 @@
 
 namespace hy {
 
-// eight values of a row at column c, zeros behind its end; AL: the rows are whole 16-byte pieces
-template <typename T, bool AL> __device__ __forceinline__ v8<T> lora_ld8(const T *row, int c, int end) {
-    v8<T> v = {};
-    if constexpr (AL) {
-        if (c < end) v = *(const v8<T> *) (row + c);
-    } else {
+// N neighbours wherever they start: the memory takes any alignment (rows of odd lengths in single values instead: 4096 rows,
+// 4096 -> 7161, rank 64, 303 us)
+template <typename Y, int N> struct LoraVec { typedef Y vec __attribute__((ext_vector_type(N))); typedef vec type __attribute__((aligned(sizeof(Y)))); };
+template <typename Y, int N> __device__ __forceinline__ typename LoraVec<Y, N>::vec lora_get(const Y *p) { return *(const typename LoraVec<Y, N>::type *) p; }
+// N values of a row at column c, zeros behind its end
+template <typename Y, int N> __device__ __forceinline__ typename LoraVec<Y, N>::vec lora_ld(const Y *row, int c, int end) {
+    typename LoraVec<Y, N>::vec v = {};
+    if (c + N <= end) v = lora_get<Y, N>(row + c);
+    else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (c + i < end) v[i] = row[c + i];
+        for (int i = 0; i < N; ++i) if (c + i < end) v[i] = row[c + i];
     }
     return v;
 }
@@ -55,9 +58,9 @@ template <typename T, int RT, int RW> struct LowStep {   // a step's operands; a
     v8<T> x[RW][2], w[RT][2];
     __device__ __forceinline__ void load(const T *const (&xr)[RW][2], const T *const (&A)[RT][2], int at) {
 #pragma unroll
-        for (int i = 0; i < RW; ++i) { x[i][0] = *(const v8<T> *) (xr[i][0] + at); x[i][1] = *(const v8<T> *) (xr[i][1] + at); }
+        for (int i = 0; i < RW; ++i) { x[i][0] = lora_get<T, 8>(xr[i][0] + at); x[i][1] = lora_get<T, 8>(xr[i][1] + at); }
 #pragma unroll
-        for (int j = 0; j < RT; ++j) { w[j][0] = *(const v8<T> *) (A[j][0] + at); w[j][1] = *(const v8<T> *) (A[j][1] + at); }
+        for (int j = 0; j < RT; ++j) { w[j][0] = lora_get<T, 8>(A[j][0] + at); w[j][1] = lora_get<T, 8>(A[j][1] + at); }
     }
     __device__ __forceinline__ void swap() {
 #pragma unroll
@@ -80,7 +83,7 @@ __device__ __forceinline__ void lora_keep_order() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
-template <typename T, int RT, int RW, bool AL> __global__ __launch_bounds__(256) void k_lora_low(const LoraArgs a) {
+template <typename T, int RT, int RW> __global__ __launch_bounds__(256) void k_lora_low(const LoraArgs a) {
     __shared__ float s_acc[4][16][16 * RT + 4];
     constexpr int ROWS = 16 * RW, STEP = 256;   // (a wave's own 64 values, then the other waves')
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
@@ -107,25 +110,23 @@ template <typename T, int RT, int RW, bool AL> __global__ __launch_bounds__(256)
                 for (int h = 0; h < 2; ++h) A[j][h] = (const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + (i16 & ~1) + h, a.r - 1)) * a.k + 8 * q + 32 * odd;
             f4 acc[RW][RT] = {};
             int kk = __builtin_amdgcn_readfirstlane(k0 + 64 * wave);
-            if constexpr (AL) {
-                // whole steps, two sets of operands in turns: the loads ask no condition (the last step's are its own again), so that
-                // the compiler counts those in flight and products wait for their own operands only
-                const int last = k1 - kk >= 64 ? kk + (k1 - kk - 64) / STEP * STEP : -1;
-                if (last >= 0) {
-                    LowStep<T, RT, RW> s0, s1;
-                    s0.load(x, A, kk);
-                    for (;;) {
-                        s1.load(x, A, min(kk + STEP, last));
-                        lora_keep_order();
-                        s0.swap();
-                        s0.add(acc);
-                        if ((kk += STEP) > last) break;
-                        s0.load(x, A, min(kk + STEP, last));
-                        lora_keep_order();
-                        s1.swap();
-                        s1.add(acc);
-                        if ((kk += STEP) > last) break;
-                    }
+            // whole steps, two sets of operands in turns: the loads ask no condition (the last step's are its own again), so that the
+            // compiler counts those in flight and products wait for their own operands only
+            const int last = k1 - kk >= 64 ? kk + (k1 - kk - 64) / STEP * STEP : -1;
+            if (last >= 0) {
+                LowStep<T, RT, RW> s0, s1;
+                s0.load(x, A, kk);
+                for (;;) {
+                    s1.load(x, A, min(kk + STEP, last));
+                    lora_keep_order();
+                    s0.swap();
+                    s0.add(acc);
+                    if ((kk += STEP) > last) break;
+                    s0.load(x, A, min(kk + STEP, last));
+                    lora_keep_order();
+                    s1.swap();
+                    s1.add(acc);
+                    if ((kk += STEP) > last) break;
                 }
             }
             for (; kk < k1; kk += STEP) {   // the lane's own rows, up to the part's end
@@ -134,9 +135,9 @@ template <typename T, int RT, int RW, bool AL> __global__ __launch_bounds__(256)
                 for (int h = 0; h < 2; ++h) {
                     const int c = kk + 8 * q + 32 * h;
 #pragma unroll
-                    for (int i = 0; i < RW; ++i) s.x[i][h] = lora_ld8<T, AL>((const T *) a.x + (int64_t) min(r0 + 16 * i + i16, a.m - 1) * a.ldx, c, k1);
+                    for (int i = 0; i < RW; ++i) s.x[i][h] = lora_ld<T, 8>((const T *) a.x + (int64_t) min(r0 + 16 * i + i16, a.m - 1) * a.ldx, c, k1);
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) s.w[j][h] = lora_ld8<T, AL>((const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + i16, a.r - 1)) * a.k, c, k1);
+                    for (int j = 0; j < RT; ++j) s.w[j][h] = lora_ld<T, 8>((const T *) a.A + ((int64_t) ad * a.r + min(rb + 16 * j + i16, a.r - 1)) * a.k, c, k1);
                 }
                 s.add(acc);
             }
@@ -157,49 +158,37 @@ template <typename T, int RT, int RW, bool AL> __global__ __launch_bounds__(256)
     }
 }
 
-// the sums over the parts of N low products from rank c on (those below r), c a multiple of N; VEC: rows of whole 16-byte pieces
-template <int N, bool VEC> __device__ __forceinline__ void lora_sum(const float *low, int64_t between, int splits, int c, int r, float (&v)[N]) {
+// the sums over the parts of N low products from rank c on (those below r)
+template <int N> __device__ __forceinline__ void lora_sum(const float *low, int64_t between, int splits, int c, int r, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.0f;
     if (c >= r) return;
-    constexpr int U = N >= 16 ? 2 : N >= 8 ? 4 : 8;   // parts on their way together
+    constexpr int U = N >= 16 ? 2 : N >= 8 ? 4 : 8, P = N < 4 ? N : 4;   // parts on their way together
     for (int sp = 0; sp < splits; sp += U) {
-        float p[U][N];
+        typename LoraVec<float, P>::vec p[U][N / P];
 #pragma unroll
-        for (int h = 0; h < U; ++h) {
-            const float *at = low + (int64_t) min(sp + h, splits - 1) * between + c;
+        for (int h = 0; h < U; ++h)
 #pragma unroll
-            for (int i = 0; i < N; ++i) p[h][i] = 0.0f;
-            if constexpr (VEC && N % 4 == 0) {
-#pragma unroll
-                for (int i = 0; i < N; i += 4) if (c + i < r) { const f4 f = *(const f4 *) (at + i); p[h][i] = f[0]; p[h][i + 1] = f[1]; p[h][i + 2] = f[2]; p[h][i + 3] = f[3]; }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) if (c + i < r) p[h][i] = at[i];
-            }
-        }
+            for (int i = 0; i < N / P; ++i) p[h][i] = lora_ld<float, P>(low + (int64_t) min(sp + h, splits - 1) * between, c + P * i, r);
 #pragma unroll
         for (int h = 0; h < U; ++h)
             if (sp + h < splits) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] += p[h][i];
+                for (int i = 0; i < N; ++i) v[i] += p[h][i / P][i % P];
             }
     }
 }
-
-// 16 bytes of outputs
-template <typename O> struct Piece { typedef v8<O> type; };
-template <> struct Piece<float> { typedef f4 type; };
 
 // The second product and the epilogue: 16 RT rows x 64 columns a wave and item; the block's four waves have the same rows, whose
 // low products they keep in LDS as the matrix instructions' operands.  Column tile j's operand row i is column 16 j + i for fp32
 // outputs and 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4 for 16-bit ones, so that a lane holds 16-byte pieces of its row.  A turn of 64
 // columns is an item for each of the rows' adapters: its columns of B, its rows' residual, products, outputs (a row tile where
 // prompts meet is multiplied for each).  Up to rank 64 the next item's loads are on their way while an item is worked on.
-// KK: ranks in units of 32.  AL: B, resid and out are whole 16-byte pieces, and there is a resid.
-template <typename T, typename O, int RT, int KK, bool AL> struct UpItem {
-    typedef typename Piece<O>::type PT;
+// KK: ranks in units of 32.  WHOLE: n and r are multiples of 8 and there is a resid; pieces then lie inside or outside as a whole, loads
+// ask no condition and outside ones are clamped (with conditions 4096 rows, 4096 -> 7168, rank 64: 89 us for 66).
+template <typename T, typename O, int RT, int KK, bool WHOLE> struct UpItem {
     static constexpr int PN = 16 / sizeof(O), NP = 16 / PN, LOADS = 4 * KK + RT * NP;   // values of a piece, a lane's pieces of a row, loads
+    typedef typename LoraVec<O, PN>::vec PT;
     v8<T> b[KK][4];
     PT res[RT][NP];
     uint64_t mine, write;   // the item's rows that have its adapter, and all that it writes
@@ -210,30 +199,50 @@ template <typename T, typename O, int RT, int KK, bool AL> struct UpItem {
     __device__ __forceinline__ int col_of(int p, int lane) const { return c0 + (2 * (p >> 1) + (lane & 1)) * 4 * PN + PN * (lane >> 4); }
     __device__ __forceinline__ void load(const LoraArgs &a, int ad, const char *rbase, uint32_t ldr, int lane) {
         const int q = lane >> 4, i16 = lane & 15;
+        // ranks behind the last are other ranks (WHOLE: taken out piece by piece at their use) or the next rows' values (taken out by mask());
+        // at the end of all matrices there are none
+        const int64_t base = (int64_t) max(ad, 0) * a.n * a.r;
+        const bool inside = WHOLE || base + (int64_t) min(c0 + 63, a.n - 1) * a.r + 32 * KK <= (int64_t) a.n_local * a.n * a.r;   // (the same in every lane)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int c = min(c0 + (PN == 4 ? 16 * j + i16 : 32 * (j >> 1) + 8 * (i16 >> 2) + 4 * (j & 1) + (i16 & 3)), a.n - 1);
-            const T *B = (const T *) a.B + ((int64_t) max(ad, 0) * a.n + c) * a.r;
+            const T *B = (const T *) a.B + base + (int64_t) c * a.r;
 #pragma unroll
-            for (int h = 0; h < KK; ++h) {   // ranks behind the last come from one before it (zeroed at their use)
-                if constexpr (AL) b[h][j] = *(const v8<T> *) (B + min(32 * h + 8 * q, a.r - 8));
-                else b[h][j] = lora_ld8<T, false>(B, 32 * h + 8 * q, a.r);
+            for (int h = 0; h < KK; ++h) {
+                const int at = 32 * h + 8 * q;
+                if (WHOLE) b[h][j] = lora_get<T, 8>(B + min(at, a.r - 8));
+                else if (inside) b[h][j] = lora_get<T, 8>(B + at);
+                else b[h][j] = lora_ld<T, 8>(B, at, a.r);
             }
         }
-        if constexpr (AL) {   // a row that is not to be written: one that is, as for other lanes
-            const int first = __builtin_ctzll(write);
+        const int first = __builtin_ctzll(write);
+        auto at = [&](int i, int p) {   // a row that is not to be written: one that is, as for other lanes
+            const uint32_t row = write >> row_of(i, p, lane) & 1 ? row_of(i, p, lane) : first;
+            return row * ldr;
+        };
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const uint32_t row = write >> row_of(i, p, lane) & 1 ? row_of(i, p, lane) : first;
-                    res[i][p] = *(const PT *) (rbase + (row * ldr + min(col_of(p, lane), a.n - PN) * (uint32_t) sizeof(O)));
-                }
+            for (int p = 0; p < NP; ++p) {
+                if (WHOLE) res[i][p] = lora_get<O, PN>((const O *) (rbase + (at(i, p) + min(col_of(p, lane), a.n - PN) * (uint32_t) sizeof(O))));
+                else res[i][p] = a.resid ? lora_ld<O, PN>((const O *) (rbase + at(i, p)), col_of(p, lane), a.n) : PT{};
+            }
+    }
+    __device__ __forceinline__ void mask(int r, int q) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int h = 0; h < KK; ++h) {
+            const int n = r - 32 * h - 8 * q;   // values of the piece that are the row's
+            u32x4 m;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0xffffu : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[h][j] = __builtin_bit_cast(v8<T>, __builtin_bit_cast(u32x4, b[h][j]) & m);
         }
     }
 };
-template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a, int gy) {
-    typedef UpItem<T, O, RT, KK, AL> Item;
+template <typename T, typename O, int RT, int KK, bool WHOLE> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a, int gy) {
+    typedef UpItem<T, O, RT, KK, WHOLE> Item;
     constexpr int R = 32 * KK, LD = R + 8, ROWS = 16 * RT, PN = Item::PN, NP = Item::NP;
     __shared__ __attribute__((aligned(16))) T s_hi[ROWS * LD], s_lo[ROWS * LD];
     __shared__ float s_scale[ROWS];
@@ -252,7 +261,7 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
     uint64_t none = __ballot(id < 0 && lane < ROWS && r0 + lane < a.m);
     if (blockIdx.z || (a.resid == a.out && a.ldr == a.ldo)) none = 0;
     if (!(rows | none)) return;   // (the same in every wave)
-    // the tile's rows by 32-bit offsets (AL: rows of less than 2^24 bytes)
+    // the tile's rows by 32-bit offsets (rows of at most 2^24 bytes)
     const char *rbase = (const char *) a.resid + (int64_t) r0 * a.ldr * (int) sizeof(O);
     char *obase = (char *) a.out + (int64_t) r0 * a.ldo * (int) sizeof(O);
     const uint32_t ldr = (uint32_t) a.ldr * (uint32_t) sizeof(O), ldo = (uint32_t) a.ldo * (uint32_t) sizeof(O);
@@ -277,8 +286,7 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
         const float *low = a.low + (int64_t) (r0 + row) * a.r;
         const int64_t between = (int64_t) a.m * a.r;
         const int end = rows >> row & 1 ? a.r : 0;
-        if (a.r % 4 == 0) lora_sum<PER, true>(low, between, a.splits, t * PER, end, v);
-        else lora_sum<PER, false>(low, between, a.splits, t * PER, end, v);
+        lora_sum<PER>(low, between, a.splits, t * PER, end, v);
         float up = 1.0f;
         if constexpr (__is_same(T, f16)) {
 #pragma unroll
@@ -309,7 +317,8 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
         }
     }
     __syncthreads();
-    auto work = [&](const Item &s) {
+    auto work = [&](Item &s) {
+        if (!WHOLE && (a.r & 31)) s.mask(a.r, q);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (!(s.write >> (16 * i) & 0xffff)) continue;
@@ -321,7 +330,7 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
                     const v8<T> hi = *(const v8<T> *) &s_hi[r * LD + 32 * h + 8 * q], lo = *(const v8<T> *) &s_lo[r * LD + 32 * h + 8 * q];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const v8<T> w = !AL || 32 * h + 8 * q < a.r ? s.b[h][j] : v8<T>{};
+                        const v8<T> w = !WHOLE || 32 * h + 8 * q < a.r ? s.b[h][j] : v8<T>{};
                         acc[j] = mfma16(w, lo, acc[j]);
                         acc[j] = mfma16(w, hi, acc[j]);
                     }
@@ -333,30 +342,24 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[j][e] = has ? acc[j][e] * sc : 0.0f;   // (nothing of other adapters' values)
-            if constexpr (AL) {
 #pragma unroll
-                for (int p = 0; p < NP; p += 2) {
-                    // the pair's pieces change places: those of piece p and p + 1 become the even row's and the odd row's
+            for (int p = 0; p < NP; p += 2) {
+                // the pair's pieces change places: those of piece p and p + 1 become the even row's and the odd row's
 #pragma unroll
-                    for (int e = 0; e < PN / 4; ++e) pair_swap(acc[p * (PN / 4) + e], acc[(p + 1) * (PN / 4) + e]);
+                for (int e = 0; e < PN / 4; ++e) pair_swap(acc[p * (PN / 4) + e], acc[(p + 1) * (PN / 4) + e]);
 #pragma unroll
-                    for (int o = p; o < p + 2; ++o) {
-                        typename Item::PT v;
+                for (int o = p; o < p + 2; ++o) {
+                    typename LoraVec<O, PN>::type v;
 #pragma unroll
-                        for (int e = 0; e < PN; ++e) v[e] = (O) (acc[o * (PN / 4) + (e >> 2)][e & 3] + (float) s.res[i][o][e]);
-                        const int row = Item::row_of(i, o, lane), c = s.col_of(o, lane);
-                        if ((s.write >> row & 1) && c < a.n) *(typename Item::PT *) (obase + ((uint32_t) row * ldo + (uint32_t) c * (uint32_t) sizeof(O))) = v;
+                    for (int e = 0; e < PN; ++e) v[e] = (O) (acc[o * (PN / 4) + (e >> 2)][e & 3] + (float) s.res[i][o][e]);
+                    const int row = Item::row_of(i, o, lane), c = s.col_of(o, lane);
+                    if (!(s.write >> row & 1) || c >= a.n) continue;
+                    O *to = (O *) (obase + ((uint32_t) row * ldo + (uint32_t) c * (uint32_t) sizeof(O)));
+                    if (WHOLE || c + PN <= a.n) *(typename LoraVec<O, PN>::type *) to = v;
+                    else {
+#pragma unroll
+                        for (int e = 0; e < PN; ++e) if (c + e < a.n) to[e] = v[e];
                     }
-                }
-            } else if (s.write >> r & 1) {
-                const int64_t row = r0 + r;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = s.c0 + (PN == 4 ? 16 * j + 4 * q : 32 * (j >> 1) + 8 * q + 4 * (j & 1)), n = min(4, a.n - c);
-                    if (n <= 0) continue;
-                    float o[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
-                    if (a.resid) add_n<T, 4>(a.resid, row * a.ldr + c, o, n, PN == 4, a.vec);
-                    put_n<T, 4>(a.out, row * a.ldo + c, o, n, PN == 4, a.vec);
                 }
             }
         }
@@ -370,7 +373,7 @@ template <typename T, typename O, int RT, int KK, bool AL> __global__ __launch_b
         lora_keep_order();
     };
     if ((blk % gy * 4 + wave) * 64 >= a.n) return;
-    if constexpr (AL && KK <= 2) {
+    if constexpr (KK <= 2) {
         for (;;) {
             if (c0 >= a.n) { work(s0); break; }   // (the last item)
             next(s1);
@@ -402,18 +405,18 @@ LoraCut lora_cut(int m, int k) {
     return LoraCut{(int) (((int64_t) k + klen - 1) / klen), klen};
 }
 
-// how many of a tile's adapters go side by side, in blocks of their own
-static uint32_t lora_deal(int64_t blocks) { return (uint32_t) std::max<int64_t>(1, std::min<int64_t>(16, 1024 / std::max<int64_t>(1, blocks))); }
-static bool lora_al(const void *p, int64_t ld) { return ((uintptr_t) p & 15) == 0 && ld % 8 == 0; }
+// how many of a tile's adapters go side by side, in blocks of their own, up to `most` blocks in all (a tile of one adapter leaves the
+// others empty)
+static uint32_t lora_deal(int64_t blocks, int most) { return (uint32_t) std::max<int64_t>(1, std::min<int64_t>(16, most / std::max<int64_t>(1, blocks))); }
 
 template <typename T, typename O> static int launch_up(const LoraArgs &a, hipStream_t s) {
-    const bool al = lora_al(a.B, a.r) && a.vec && a.n % 8 == 0 && a.resid && a.ldr < 1 << 22 && a.ldo < 1 << 22, tall = a.r <= 64 && a.m >= LORA_MANY;
+    const bool whole = a.n % 8 == 0 && a.r % 8 == 0 && a.resid, tall = a.r <= 64 && a.m >= LORA_MANY;
     constexpr int TALL = sizeof(O) == 4 ? 2 : 4;   // row tiles whose residual fits the registers twice
     const int tiles = tall ? (a.m + 16 * TALL - 1) / (16 * TALL) : (a.m + 15) / 16, cols = (a.n + 255) / 256;
     // many rows: about two blocks a CU, that take several turns with their rows' low products
     const int turns = std::max(1, (int) (((int64_t) tiles * cols + 511) / 512)), gy = (cols + turns - 1) / turns;
-    const dim3 up(tiles * gy, 1, tall ? 1 : lora_deal((int64_t) tiles * gy));
-#define HY_UP(RT, KK) { if (al) k_lora_up<T, O, RT, KK, true><<<up, 256, 0, s>>>(a, gy); else k_lora_up<T, O, RT, KK, false><<<up, 256, 0, s>>>(a, gy); }
+    const dim3 up(tiles * gy, 1, lora_deal((int64_t) tiles * gy, tall ? 512 : 1024));
+#define HY_UP(RT, KK) { if (whole) k_lora_up<T, O, RT, KK, true><<<up, 256, 0, s>>>(a, gy); else k_lora_up<T, O, RT, KK, false><<<up, 256, 0, s>>>(a, gy); }
     if (a.r <= 32) { if (tall) HY_UP(TALL, 1) else HY_UP(1, 1) }
     else if (a.r <= 64) { if (tall) HY_UP(TALL, 2) else HY_UP(1, 2) }
     else if (a.r <= 128) HY_UP(1, 4)
@@ -422,11 +425,10 @@ template <typename T, typename O> static int launch_up(const LoraArgs &a, hipStr
     return check_launch("hy_lora");
 }
 template <typename T> static int launch_lora_t(const LoraArgs &a, hipStream_t s) {
-    const bool many = a.m >= LORA_MANY, al = lora_al(a.x, a.ldx) && lora_al(a.A, a.k);
+    const bool many = a.m >= LORA_MANY;
     const int tiles = (a.m + (many ? 31 : 15)) / (many ? 32 : 16);
-    const dim3 low(tiles * a.splits, 1, many ? 4 : lora_deal((int64_t) tiles * a.splits));
-#define HY_LOW(RT) { if (many) { if (al) k_lora_low<T, RT, 2, true><<<low, 256, 0, s>>>(a); else k_lora_low<T, RT, 2, false><<<low, 256, 0, s>>>(a); } \
-                     else { if (al) k_lora_low<T, RT, 1, true><<<low, 256, 0, s>>>(a); else k_lora_low<T, RT, 1, false><<<low, 256, 0, s>>>(a); } }
+    const dim3 low(tiles * a.splits, 1, lora_deal((int64_t) tiles * a.splits, many ? 2048 : 1024));
+#define HY_LOW(RT) { if (many) k_lora_low<T, RT, 2><<<low, 256, 0, s>>>(a); else k_lora_low<T, RT, 1><<<low, 256, 0, s>>>(a); }
     if (a.r <= 16) HY_LOW(1) else if (a.r <= 32) HY_LOW(2) else HY_LOW(4)
 #undef HY_LOW
     if (const int rc = check_launch("hy_lora")) return rc;

@@ -26,8 +26,8 @@ struct NormBwdArgs {
     int m, n, y_type, parts;
     bool accumulate;
 };
-int launch_norm(int x_type, const NormArgs &a, bool vec, hipStream_t s);
-int norm_bwd_parts(int m, int n);
-int launch_norm_bwd(int x_type, bool layer, const NormBwdArgs &a, bool vec, hipStream_t s);
+int launch_norm(int x_type, const NormArgs &a, hipStream_t s);
+int norm_bwd_parts(int m, int n, bool x32);   // (the most with x32 false)
+int launch_norm_bwd(int x_type, bool layer, const NormBwdArgs &a, hipStream_t s);
 
 } // namespace hy

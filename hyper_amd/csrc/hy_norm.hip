@@ -12,70 +12,55 @@
 
 namespace hy {
 
-// A thread's 8 V values of a row that T threads share.  VEC: in pieces of 16 bytes of the row's type X (PW = 4 or 8 neighbours),
-// piece p at column PW (p T + t), so that neighbouring threads move neighbouring pieces (fp32 rows by 8 neighbours a thread instead:
-// the gradient of 8192 x 4096 94 us for 86); else value k is column k T + t.
-template <int T, int PW, bool VEC> __device__ __forceinline__ int norm_col(int t, int j, int i) {
-    return VEC ? PW * ((8 / PW * j + i / PW) * T + t) + i % PW : (8 * j + i) * T + t;
-}
-template <typename Y, int PW> using Neighbours = Y __attribute__((ext_vector_type(PW)));
+// A thread's 8 V values of a row that T threads share, in pieces of 16 bytes of the row's type X (PW = 4 or 8 neighbours): piece p at
+// column PW (p T + t), so that neighbouring threads move neighbouring pieces (fp32 rows by 8 neighbours a thread instead: the
+// gradient of 8192 x 4096 94 us for 86).
+template <int T, int PW> __device__ __forceinline__ int norm_col(int t, int j, int i) { return PW * ((8 / PW * j + i / PW) * T + t) + i % PW; }
+// PW neighbours wherever they start (the memory takes any alignment; rows of odd lengths one value at a time instead: 8192 x 4095
+// bf16 142 us for 101)
+template <typename Y, int PW> struct NeighboursOf { typedef Y vec __attribute__((ext_vector_type(PW))); typedef vec type __attribute__((aligned(sizeof(Y)))); };
+template <typename Y, int PW> using Neighbours = typename NeighboursOf<Y, PW>::type;
 
 // a thread's values 8 j .. + 7 of a row of n values, zeros behind its end.  Y: the type of this row, whose columns go by PW
-template <typename Y, int T, int PW, bool VEC> __device__ __forceinline__ void norm_load(const Y *row, int t, int j, int n, float (&v)[8]) {
-    if constexpr (VEC) {
+template <typename Y, int T, int PW> __device__ __forceinline__ void norm_load(const Y *row, int t, int j, int n, float (&v)[8]) {
 #pragma unroll
-        for (int h = 0; h < 8; h += PW) {
-            const int c = norm_col<T, PW, true>(t, j, h);
-            if (c + PW <= n) {
-                const Neighbours<Y, PW> a = *(const Neighbours<Y, PW> *) (row + c);
+    for (int h = 0; h < 8; h += PW) {
+        const int c = norm_col<T, PW>(t, j, h);
+        if (c + PW <= n) {
+            const Neighbours<Y, PW> a = *(const Neighbours<Y, PW> *) (row + c);
 #pragma unroll
-                for (int i = 0; i < PW; ++i) v[h + i] = (float) a[i];
-            } else {
+            for (int i = 0; i < PW; ++i) v[h + i] = (float) a[i];
+        } else {
 #pragma unroll
-                for (int i = 0; i < PW; ++i) v[h + i] = c + i < n ? (float) row[c + i] : 0.0f;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = norm_col<T, PW, false>(t, j, i);
-            v[i] = c < n ? (float) row[c] : 0.0f;
+            for (int i = 0; i < PW; ++i) v[h + i] = c + i < n ? (float) row[c + i] : 0.0f;
         }
     }
 }
-template <typename Y, int T, int PW, bool VEC> __device__ __forceinline__ void norm_store(Y *row, int t, int j, int n, const float (&v)[8]) {
-    if constexpr (VEC) {
+template <typename Y, int T, int PW> __device__ __forceinline__ void norm_store(Y *row, int t, int j, int n, const float (&v)[8]) {
 #pragma unroll
-        for (int h = 0; h < 8; h += PW) {
-            const int c = norm_col<T, PW, true>(t, j, h);
-            if (c + PW <= n) {
-                Neighbours<Y, PW> a;
+    for (int h = 0; h < 8; h += PW) {
+        const int c = norm_col<T, PW>(t, j, h);
+        if (c + PW <= n) {
+            Neighbours<Y, PW> a;
 #pragma unroll
-                for (int i = 0; i < PW; ++i) a[i] = (Y) v[h + i];
-                *(Neighbours<Y, PW> *) (row + c) = a;
-            } else {
+            for (int i = 0; i < PW; ++i) a[i] = (Y) v[h + i];
+            *(Neighbours<Y, PW> *) (row + c) = a;
+        } else {
 #pragma unroll
-                for (int i = 0; i < PW; ++i) if (c + i < n) row[c + i] = (Y) v[h + i];
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = norm_col<T, PW, false>(t, j, i);
-            if (c < n) row[c] = (Y) v[i];
+            for (int i = 0; i < PW; ++i) if (c + i < n) row[c + i] = (Y) v[h + i];
         }
     }
 }
 // the same where the type is known at run time only (the same for every thread)
-template <int T, int PW, bool VEC> __device__ __forceinline__ void norm_load_as(int type, const void *base, int64_t at, int t, int j, int n, float (&v)[8]) {
-    if (type == HY_F32) norm_load<float, T, PW, VEC>((const float *) base + at, t, j, n, v);
-    else if (type == HY_BF16) norm_load<bf16, T, PW, VEC>((const bf16 *) base + at, t, j, n, v);
-    else norm_load<f16, T, PW, VEC>((const f16 *) base + at, t, j, n, v);
+template <int T, int PW> __device__ __forceinline__ void norm_load_as(int type, const void *base, int64_t at, int t, int j, int n, float (&v)[8]) {
+    if (type == HY_F32) norm_load<float, T, PW>((const float *) base + at, t, j, n, v);
+    else if (type == HY_BF16) norm_load<bf16, T, PW>((const bf16 *) base + at, t, j, n, v);
+    else norm_load<f16, T, PW>((const f16 *) base + at, t, j, n, v);
 }
-template <int T, int PW, bool VEC> __device__ __forceinline__ void norm_store_as(int type, void *base, int64_t at, int t, int j, int n, const float (&v)[8]) {
-    if (type == HY_F32) norm_store<float, T, PW, VEC>((float *) base + at, t, j, n, v);
-    else if (type == HY_BF16) norm_store<bf16, T, PW, VEC>((bf16 *) base + at, t, j, n, v);
-    else norm_store<f16, T, PW, VEC>((f16 *) base + at, t, j, n, v);
+template <int T, int PW> __device__ __forceinline__ void norm_store_as(int type, void *base, int64_t at, int t, int j, int n, const float (&v)[8]) {
+    if (type == HY_F32) norm_store<float, T, PW>((float *) base + at, t, j, n, v);
+    else if (type == HY_BF16) norm_store<bf16, T, PW>((bf16 *) base + at, t, j, n, v);
+    else norm_store<f16, T, PW>((f16 *) base + at, t, j, n, v);
 }
 
 // the sum of v over the T threads of a row; `s`: this row's T / 64 floats of LDS, written anew by each call
@@ -94,18 +79,18 @@ template <int T> __device__ __forceinline__ float row_sum(float v, float *s) {
 constexpr int NORM_BLOCKS = 1 << 20;   // most blocks of a launch: they go on to further rows
 
 // T threads a row of up to 8 V T values; a block has one row, or four of a wave each (T = 64: no barrier)
-template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
+template <typename X, int T, int V> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
     constexpr int NT = T == 64 ? 256 : T, G = NT / T, PW = 16 / sizeof(X);
     __shared__ float s_sum[3][NT / 64];
     const int t = threadIdx.x % T;
     for (int64_t row = (int64_t) blockIdx.x * G + threadIdx.x / T; row < a.m; row += (int64_t) gridDim.x * G) {
         float v[V][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) norm_load<X, T, PW, VEC>((const X *) a.x + row * a.ldx, t, j, a.n, v[j]);
+        for (int j = 0; j < V; ++j) norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, j, a.n, v[j]);
         if (a.add) {
             float d[V][8];
 #pragma unroll
-            for (int j = 0; j < V; ++j) norm_load<X, T, PW, VEC>((const X *) a.add + row * a.lda, t, j, a.n, d[j]);
+            for (int j = 0; j < V; ++j) norm_load<X, T, PW>((const X *) a.add + row * a.lda, t, j, a.n, d[j]);
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -113,7 +98,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 
         }
         if (a.total) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) norm_store<X, T, PW, VEC>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
+            for (int j = 0; j < V; ++j) norm_store<X, T, PW>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
         }
         float mu = 0.0f, q = 0.0f;
         if (a.layer) {
@@ -126,7 +111,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (norm_col<T, PW, VEC>(t, j, i) < a.n) e += v[j][i] - mu;
+                for (int i = 0; i < 8; ++i) if (norm_col<T, PW>(t, j, i) < a.n) e += v[j][i] - mu;
             mu += row_sum<T>(e, s_sum[2]) / (float) a.n;
         }
 #pragma unroll
@@ -134,7 +119,7 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 v[j][i] -= mu;
-                if (norm_col<T, PW, VEC>(t, j, i) < a.n) q = fmaf(v[j][i], v[j][i], q);
+                if (norm_col<T, PW>(t, j, i) < a.n) q = fmaf(v[j][i], v[j][i], q);
             }
         const float r = 1.0f / sqrtf(row_sum<T>(q, s_sum[1]) / (float) a.n + a.eps);
         if (t == 0) {
@@ -143,20 +128,20 @@ template <typename X, int T, int V, bool VEC> __global__ __launch_bounds__(T == 
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (norm_col<T, PW, VEC>(t, j, 0) >= a.n) continue;
+            if (norm_col<T, PW>(t, j, 0) >= a.n) continue;
             float w[8], y[8];
-            norm_load<float, T, PW, VEC>(a.w, t, j, a.n, w);
+            norm_load<float, T, PW>(a.w, t, j, a.n, w);
             if (a.b) {
                 float b[8];
-                norm_load<float, T, PW, VEC>(a.b, t, j, a.n, b);
+                norm_load<float, T, PW>(a.b, t, j, a.n, b);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = fmaf(v[j][i] * r, w[i], b[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = v[j][i] * r * w[i];
             }
-            if (a.out) norm_store_as<T, PW, VEC>(a.o_type, a.out, row * a.ldo, t, j, a.n, y);
-            if (a.out32) norm_store<float, T, PW, VEC>(a.out32 + row * a.ldo32, t, j, a.n, y);
+            if (a.out) norm_store_as<T, PW>(a.o_type, a.out, row * a.ldo, t, j, a.n, y);
+            if (a.out32) norm_store<float, T, PW>(a.out32 + row * a.ldo32, t, j, a.n, y);
         }
         if constexpr (T > 64) lds_barrier();   // the sums are read before the next row's are written
     }
@@ -197,49 +182,50 @@ template <typename X> __global__ __launch_bounds__(1024) void k_norm_long(const 
     }
 }
 
-template <typename X, bool VEC> static void launch_norm_t(const NormArgs &a, hipStream_t s) {
+template <typename X> static void launch_norm_t(const NormArgs &a, hipStream_t s) {
     auto grid = [&](int rows) { return dim3((uint32_t) std::min<int64_t>(((int64_t) a.m + rows - 1) / rows, NORM_BLOCKS)); };
-#define HY_NORM(T, V) k_norm<X, T, V, VEC><<<grid(T == 64 ? 4 : 1), T == 64 ? 256 : T, 0, s>>>(a)
+#define HY_NORM(T, V) k_norm<X, T, V><<<grid(T == 64 ? 4 : 1), T == 64 ? 256 : T, 0, s>>>(a)
     if (a.n > 16384) { k_norm_long<X><<<grid(1), 1024, 0, s>>>(a); return; }
-    // 8 values a thread: a row in the registers of one wave (n 4096: 64 a thread) keeps too few rows of a CU under way (8192 x 4096:
-    // 64 values a thread 114 us, 32 95, 16 85, 8 82)
+    // 8 values a thread: a row in the registers of one wave (n 4096: 64 a thread) keeps too few rows of a CU under way (RMS of fp32
+    // 8192 x 4096: 64 values a thread 114 us, 32 95, 16 85, 8 82; layer norm 16 98, 8 84).  16-bit rows wait for their sums rather:
+    // 16 values, half as many waves to join (layer norm 56 us for 63, RMS 49 for 48)
     if (a.n <= 512) HY_NORM(64, 1);
     else if (a.n <= 1024) HY_NORM(128, 1);
     else if (a.n <= 2048) HY_NORM(256, 1);
-    else if (a.n <= 4096) HY_NORM(512, 1);
+    else if (a.n <= 4096) { if (sizeof(X) == 2) HY_NORM(256, 2); else HY_NORM(512, 1); }
     else if (a.n <= 8192) HY_NORM(1024, 1);
     else HY_NORM(1024, 2);
 #undef HY_NORM
 }
-int launch_norm(int x_type, const NormArgs &a, bool vec, hipStream_t s) {
-    if (x_type == HY_F32) vec ? launch_norm_t<float, true>(a, s) : launch_norm_t<float, false>(a, s);
-    else if (x_type == HY_BF16) vec ? launch_norm_t<bf16, true>(a, s) : launch_norm_t<bf16, false>(a, s);
-    else vec ? launch_norm_t<f16, true>(a, s) : launch_norm_t<f16, false>(a, s);
+int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
+    if (x_type == HY_F32) launch_norm_t<float>(a, s);
+    else if (x_type == HY_BF16) launch_norm_t<bf16>(a, s);
+    else launch_norm_t<f16>(a, s);
     return check_launch("hy_norm");
 }
 
 // ------------------------------------------------------------------ backward
 
 // 8 values a thread here too: 16 of them (and their sums, 16 or 32 more) leave one block a CU (8192 x 4096 fp32: 104 us for 87).
-// Three blocks of 512 threads a CU and two of 1024; with two of 512 87.5 us for 85.7, with four 94 (more sums to join).
+// Blocks: as many as join their sums in less than they save.  fp32 rows, two of 512 threads a CU or three, 8192 x 4096: RMS 90.5 and
+// 91.1 us, layer norm 96.6 and 109; 16-bit rows 61 and 57, 70 and 67.
 constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
 __host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
 __host__ __device__ constexpr int nb_block_threads(int T) { return T < 512 ? 512 : T; }
 
-int norm_bwd_parts(int m, int n) {
+int norm_bwd_parts(int m, int n, bool x32) {
     const int T = nb_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 512 : 768);
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 || x32 ? 512 : 768);
 }
 
-// T threads a row of up to 8 T values, G rows at a time; block b takes rows G b .. + G - 1 of every G gridDim.x
-template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
-    constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64, COLS = 8 * T, PW = 16 / sizeof(X);
+// T threads a row of up to 8 T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
+// and db of the thread's columns over its rows
+template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[8], float (&db)[8]) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64, PW = 16 / sizeof(X);
     __shared__ float s_sum[2][2][NT / 64];
-    __shared__ float s_join[G > 1 ? G * COLS : 1];
     const int t = threadIdx.x % T, g = threadIdx.x / T, wave = threadIdx.x >> 6;
-    float dw[8] = {}, db[8] = {};
     int turn = 0;
-    for (int64_t first = (int64_t) blockIdx.x * G; first < a.m; first += (int64_t) gridDim.x * G, turn ^= 1) {
+    for (int64_t first = (int64_t) blockIdx.x * G; first < a.m; first += (int64_t) blocks * G, turn ^= 1) {
         const int64_t row = first + g;
         const bool on = row < a.m;   // (the other threads go along for the barriers)
         float x[8], dy[8], e[8] = {}, c1 = 0.0f, c2 = 0.0f, r = 0.0f, mu = 0.0f;
@@ -247,15 +233,15 @@ template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(
             float w[8];
             r = a.rstd[row];
             if (LAYER) mu = a.mean[row];
-            norm_load<X, T, PW, VEC>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
-            norm_load_as<T, PW, VEC>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
-            norm_load<float, T, PW, VEC>(a.w, t, 0, a.n, w);
-            if (a.resid) norm_load<X, T, PW, VEC>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
+            norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
+            norm_load_as<T, PW>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
+            norm_load<float, T, PW>(a.w, t, 0, a.n, w);
+            if (a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float h = (x[i] - mu) * r;
-                dw[i] = fmaf(dy[i], h, dw[i]);
-                if (LAYER) db[i] += dy[i];
+                if (SUMS) dw[i] = fmaf(dy[i], h, dw[i]);
+                if (SUMS && LAYER) db[i] += dy[i];
                 x[i] = h;
                 dy[i] *= w[i];   // zeros behind the row's end
                 if (LAYER) c1 += dy[i];
@@ -271,15 +257,22 @@ template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(
 #pragma unroll
             for (int i = 0; i < W; ++i) { c2 += s_sum[turn][0][g * W + i]; if (LAYER) c1 += s_sum[turn][1][g * W + i]; }
         }
-        if (on && norm_col<T, PW, VEC>(t, 0, 0) < a.n) {
+        if (on && norm_col<T, PW>(t, 0, 0) < a.n) {
             c1 /= (float) a.n;
             c2 /= (float) a.n;
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[i] - c1 : dy[i]) - x[i] * c2) + e[i];
-            norm_store<X, T, PW, VEC>((X *) a.dx + row * a.ldd, t, 0, a.n, o);
+            norm_store<X, T, PW>((X *) a.dx + row * a.ldd, t, 0, a.n, o);
         }
     }
+}
+template <typename X, int T, bool LAYER> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, COLS = 8 * T, PW = 16 / sizeof(X);
+    __shared__ float s_join[G > 1 ? G * COLS : 1];
+    const int t = threadIdx.x % T, g = threadIdx.x / T;
+    float dw[8] = {}, db[8] = {};
+    norm_bwd_rows<X, T, LAYER, true>(a, gridDim.x, dw, db);
     // the block's sums: over its G rows, in their order
 #pragma unroll
     for (int which = 0; which < (LAYER ? 2 : 1); ++which) {
@@ -290,7 +283,7 @@ template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(
         if constexpr (G > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s_join[g * COLS + norm_col<T, PW, VEC>(t, 0, i)] = which ? db[i] : dw[i];
+            for (int i = 0; i < 8; ++i) s_join[g * COLS + norm_col<T, PW>(t, 0, i)] = which ? db[i] : dw[i];
             __syncthreads();
             for (int c = threadIdx.x; c < a.n; c += NT) {
                 float v = 0.0f;
@@ -301,7 +294,7 @@ template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = norm_col<T, PW, VEC>(t, 0, i);
+                const int c = norm_col<T, PW>(t, 0, i);
                 const float v = which ? db[i] : dw[i];
                 if (c < a.n) to[c] = acc ? to[c] + v : v;
             }
@@ -309,10 +302,59 @@ template <typename X, int T, bool LAYER, bool VEC> __global__ __launch_bounds__(
     }
 }
 
-// rows longer than a block's registers: dx by one block a row in two passes ...
-template <typename X> __device__ __forceinline__ float dy_at(int type, const void *dy, int64_t at) {
-    return type == HY_F32 ? ((const float *) dy)[at] : type == HY_BF16 ? (float) ((const bf16 *) dy)[at] : (float) ((const f16 *) dy)[at];
+// Few rows: the sums over the rows by blocks of their own beside the rows' blocks, each 32 columns and every 16th row a thread, so that
+// one launch does (a second costs 3.5 us of the calling thread).  They read x and dy once more.
+__device__ __forceinline__ float norm_value(int type, const void *base, int64_t at) {
+    return type == HY_F32 ? ((const float *) base)[at] : type == HY_BF16 ? (float) ((const bf16 *) base)[at] : (float) ((const f16 *) base)[at];
 }
+template <typename X, int T, bool LAYER> __global__ __launch_bounds__(512) void k_norm_bwd_few(const NormBwdArgs a, int blocks) {
+    static_assert(nb_block_threads(T) == 512, "");
+    if ((int) blockIdx.x < blocks) {
+        float none[8];
+        norm_bwd_rows<X, T, LAYER, false>(a, blocks, none, none);
+        return;
+    }
+    __shared__ float s[2][16][32];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, col = ((int) blockIdx.x - blocks) * 32 + c;
+    float dw = 0.0f, db = 0.0f;
+    auto sum = [&](auto *dys) {
+        const X *x = (const X *) a.x + col;
+        for (int r0 = g; r0 < a.m; r0 += 16 * 8) {   // eight rows' values on their way together
+            float xv[8], dv[8], rv[8], mv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = min(r0 + 16 * i, a.m - 1);
+                xv[i] = (float) x[row * a.ldx];
+                dv[i] = (float) dys[row * a.ldy + col];
+                rv[i] = a.rstd[row];
+                mv[i] = LAYER ? a.mean[row] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = r0 + 16 * i < a.m;
+                dw = in ? fmaf(dv[i], (xv[i] - mv[i]) * rv[i], dw) : dw;
+                if (LAYER) db += in ? dv[i] : 0.0f;
+            }
+        }
+    };
+    if (col < a.n) {
+        if (a.y_type == HY_F32) sum((const float *) a.dy);
+        else if (a.y_type == HY_BF16) sum((const bf16 *) a.dy);
+        else sum((const f16 *) a.dy);
+    }
+    s[0][g][c] = dw;
+    s[1][g][c] = db;
+    __syncthreads();
+    float *out = g == 0 ? a.dw : g == 1 && LAYER ? a.db : nullptr;
+    if (out && col < a.n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += s[g][i][c];
+        out[col] = a.accumulate ? out[col] + v : v;
+    }
+}
+
+// rows longer than a block's registers: dx by one block a row in two passes ...
 template <typename X> __global__ __launch_bounds__(1024) void k_norm_dx_long(const NormBwdArgs a) {
     __shared__ float s_sum[2][16];
     for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
@@ -320,14 +362,14 @@ template <typename X> __global__ __launch_bounds__(1024) void k_norm_dx_long(con
         const float r = a.rstd[row], mu = a.mean ? a.mean[row] : 0.0f;
         float c1 = 0.0f, c2 = 0.0f;
         for (int c = threadIdx.x; c < a.n; c += 1024) {
-            const float g = dy_at<X>(a.y_type, a.dy, row * a.ldy + c) * a.w[c];
+            const float g = norm_value(a.y_type, a.dy, row * a.ldy + c) * a.w[c];
             c1 += g;
             c2 = fmaf(g, ((float) x[c] - mu) * r, c2);
         }
         c1 = a.mean ? row_sum<1024>(c1, s_sum[0]) / (float) a.n : 0.0f;
         c2 = row_sum<1024>(c2, s_sum[1]) / (float) a.n;
         for (int c = threadIdx.x; c < a.n; c += 1024) {
-            const float g = dy_at<X>(a.y_type, a.dy, row * a.ldy + c) * a.w[c], h = ((float) x[c] - mu) * r;
+            const float g = norm_value(a.y_type, a.dy, row * a.ldy + c) * a.w[c], h = ((float) x[c] - mu) * r;
             const float v = r * (g - c1 - h * c2);
             ((X *) a.dx)[row * a.ldd + c] = (X) (a.resid ? v + (float) ((const X *) a.resid)[row * a.ldr + c] : v);
         }
@@ -340,7 +382,7 @@ template <typename X> __global__ __launch_bounds__(256) void k_norm_dw_long(cons
     if (c >= a.n) return;
     float dw = 0.0f, db = 0.0f;
     for (int64_t row = blockIdx.y; row < a.m; row += gridDim.y) {
-        const float dy = dy_at<X>(a.y_type, a.dy, row * a.ldy + c), mu = a.mean ? a.mean[row] : 0.0f;
+        const float dy = norm_value(a.y_type, a.dy, row * a.ldy + c), mu = a.mean ? a.mean[row] : 0.0f;
         dw = fmaf(dy, ((float) ((const X *) a.x)[row * a.ldx + c] - mu) * a.rstd[row], dw);
         db += dy;
     }
@@ -377,10 +419,28 @@ __global__ __launch_bounds__(256) void k_norm_zero(float *dw, float *db, int n) 
     }
 }
 
-template <typename X, bool LAYER, bool VEC> static void launch_norm_bwd_t(const NormBwdArgs &a, hipStream_t s) {
+// Calls that k_norm_bwd_few is faster for, microseconds a call among others, fp16 layer norm and fp32 RMS: 509 x 1001 14.7 (k_norm_bwd and
+// k_norm_join 17.4) and 12.5 (15.1); 1000 x 2048 14.6 (16.7) and 12.6 (15.2); 1000 x 4096 17.5 (29.9) and 18.4 (15.9); 2000 x 1001
+// 19.8 (16.7) and 18.0 (15.3)
+static bool norm_bwd_few(const NormBwdArgs &a, int x_bytes) {
+    return a.parts > 1 && (a.dw || a.db) && a.m <= 1024 && a.n <= 4096 && a.m * a.n * x_bytes <= 1 << 23;
+}
+template <typename X, bool LAYER> static void launch_norm_bwd_t(const NormBwdArgs &a, hipStream_t s) {
     const dim3 grid(a.parts);
     const int n = a.n;
-#define HY_NB(T) k_norm_bwd<X, T, LAYER, VEC><<<grid, nb_block_threads(T), 0, s>>>(a)
+    if (norm_bwd_few(a, sizeof(X))) {
+        const int T = nb_row_threads(n), g = nb_block_threads(T) / T, blocks = (a.m + g - 1) / g, cols = (n + 31) / 32;
+        auto go = [&](int rows, int all) {   // `rows` blocks of rows, then those of columns
+            if (T == 64) k_norm_bwd_few<X, 64, LAYER><<<all, 512, 0, s>>>(a, rows);
+            else if (T == 128) k_norm_bwd_few<X, 128, LAYER><<<all, 512, 0, s>>>(a, rows);
+            else if (T == 256) k_norm_bwd_few<X, 256, LAYER><<<all, 512, 0, s>>>(a, rows);
+            else k_norm_bwd_few<X, 512, LAYER><<<all, 512, 0, s>>>(a, rows);
+        };
+        if (a.dx != a.x && a.dx != a.dy) go(blocks, blocks + cols);
+        else { go(0, cols); go(blocks, blocks); }   // dx takes the place of what the columns' blocks read: after them
+        return;
+    }
+#define HY_NB(T) k_norm_bwd<X, T, LAYER><<<grid, nb_block_threads(T), 0, s>>>(a)
     switch (nb_row_threads(n)) {
     case 64: HY_NB(64); break;
     case 128: HY_NB(128); break;
@@ -390,24 +450,24 @@ template <typename X, bool LAYER, bool VEC> static void launch_norm_bwd_t(const 
     }
 #undef HY_NB
 }
-template <typename X> static void launch_norm_bwd_x(bool layer, const NormBwdArgs &a, bool vec, hipStream_t s) {
+template <typename X> static void launch_norm_bwd_x(bool layer, const NormBwdArgs &a, hipStream_t s) {
     if (a.n > NB_LONG) {
         if (a.dw || a.db) k_norm_dw_long<X><<<dim3((a.n + 255) / 256, a.parts), 256, 0, s>>>(a);
         k_norm_dx_long<X><<<(uint32_t) std::min(a.m, NORM_BLOCKS), 1024, 0, s>>>(a);
-    } else if (layer) vec ? launch_norm_bwd_t<X, true, true>(a, s) : launch_norm_bwd_t<X, true, false>(a, s);
-    else vec ? launch_norm_bwd_t<X, false, true>(a, s) : launch_norm_bwd_t<X, false, false>(a, s);
+    } else if (layer) launch_norm_bwd_t<X, true>(a, s);
+    else launch_norm_bwd_t<X, false>(a, s);
 }
-int launch_norm_bwd(int x_type, bool layer, const NormBwdArgs &a, bool vec, hipStream_t s) {
+int launch_norm_bwd(int x_type, bool layer, const NormBwdArgs &a, hipStream_t s) {
     const char *what = "hy_norm_bwd";
     if (a.m == 0) {
         if (!a.accumulate && (a.dw || a.db)) k_norm_zero<<<(uint32_t) std::min((a.n + 255) / 256, 4096), 256, 0, s>>>(a.dw, a.db, a.n);
         return check_launch(what);
     }
-    if (x_type == HY_F32) launch_norm_bwd_x<float>(layer, a, vec, s);
-    else if (x_type == HY_BF16) launch_norm_bwd_x<bf16>(layer, a, vec, s);
-    else launch_norm_bwd_x<f16>(layer, a, vec, s);
+    if (x_type == HY_F32) launch_norm_bwd_x<float>(layer, a, s);
+    else if (x_type == HY_BF16) launch_norm_bwd_x<bf16>(layer, a, s);
+    else launch_norm_bwd_x<f16>(layer, a, s);
     if (const int rc = check_launch(what)) return rc;
-    if (a.part && (a.dw || a.db)) {
+    if (a.part && (a.dw || a.db) && !norm_bwd_few(a, x_type == HY_F32 ? 4 : 2)) {
         k_norm_join<<<dim3((a.n + 63) / 64, a.db ? 2 : 1), 1024, 0, s>>>(a.part, a.parts, a.n, a.dw, a.db, a.accumulate);
         return check_launch(what);
     }

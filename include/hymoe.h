@@ -416,9 +416,11 @@ int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int s
 /* Low-rank adapters of many requests beside a shared projection: out[t] = resid[t] + scale_a B_a (A_a x[t]) with a = ids[t], for m
    rows x [m][k]; a row whose id is outside [0, n_local) gets resid[t] alone (zeros without resid).  A [n_local][r][k] and
    B [n_local][n][r], contiguous, of `type`; scale: n_local floats (NULL: 1); resid and out of out_type (`type` or HY_F32), resid may
-   be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32.  r at most
-   HY_LORA_MAX_RANK.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned, as hy_linear_dw's. */
+   be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32 (a value that is not
+   finite in B, or in A or x and so in a low product, makes its row's outputs inf or NaN, those of no other row).  r at most
+   HY_LORA_MAX_RANK, rows of out and resid at most HY_LORA_MAX_STRIDE values apart.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned, as hy_linear_dw's. */
 #define HY_LORA_MAX_RANK 256
+#define HY_LORA_MAX_STRIDE (1 << 22)
 size_t hy_lora_ws_bytes(int m, int r, int k);
 int hy_lora(int type, const void *A, const void *B, const float *scale, int n_local, int r, int k, int n, const void *x, int64_t ldx, int m,
             const int32_t *ids, const void *resid, int64_t ldr, void *out, int out_type, int64_t ldo, void *ws, size_t ws_bytes, hipStream_t s);

@@ -94,6 +94,25 @@ def test_lora_rows(m):
         check_ints(m, 96, 264, 64, 9, FP, FP, some_ids(gen(m + 1), m, 9, how), dev, m, in_place=True)
 
 
+@pytest.mark.parametrize("r", [8, 20, 64, 72])
+def test_lora_many_rows_of_mixed_requests(r):
+    """a large batch of single tokens: every tile has many adapters; odd and whole columns, both outputs, with and without a residual"""
+    dev = torch.device("cuda:0")
+    for i, (n, ot) in enumerate(((264, BF), (257, F32), (200, F32), (97, BF))):
+        ids = some_ids(gen(r + i), 300 + 57 * i, 23, "each")
+        check_ints(ids.numel(), 130, n, r, 23, BF, ot, ids, dev, r + i, with_resid=i != 2, pad=(0, 1)[i % 2], in_place=i == 1)
+
+
+def test_lora_ends_of_the_matrices():
+    """the last rows of the last adapter with nothing behind them: ranks and columns of every remainder"""
+    dev = torch.device("cuda:0")
+    for r in (1, 3, 7, 12, 31, 33, 63):
+        for n in (1, 5, 64, 66):
+            ids = torch.full((20,), 1, dtype=torch.int32)
+            check_ints(20, 40, n, r, 2, FP, F32, ids, dev, r + n)
+            check_ints(260, 40, n, r, 2, BF, BF, torch.full((260,), 1, dtype=torch.int32), dev, r + n)
+
+
 def test_lora_no_adapters_and_no_rows():
     dev = torch.device("cuda:0")
     ids = torch.full((50,), -1, dtype=torch.int32)
