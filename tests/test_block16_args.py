@@ -84,7 +84,7 @@ def test_lora_refusals():
     need = lib().hy_lora_ws_bytes(8, 16, 64)
     assert need == 8 * 16 * 4 and lib().hy_lora_ws_bytes(0, 16, 64) == 0 and lib().hy_lora_ws_bytes(8, 300, 64) == 0
     assert _lora(ws=None) == I and _lora(wsb=need - 1) == I and _lora(ws=ctypes.c_void_p(72)) == S
-    assert _lora(m=1 << 28, n=1 << 14, ldo=1 << 14) == S and _lora(n=1 << 25, ldo=1 << 25) == S
+    assert _lora(m=1 << 28, n=1 << 14, ldo=1 << 14, wsb=1 << 45) == S and _lora(n=1 << 25, ldo=1 << 25) == S
     assert _lora(ldo=(1 << 22) + 1) == S and _lora(resid=P, ldr=(1 << 22) + 1) == S and b"2^22" in lib().hy_last_error()
     assert _lora(m=0, x=None, out=None, ids=None, ws=None) == OK
 
