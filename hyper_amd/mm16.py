@@ -365,11 +365,14 @@ def norm(x, w, out=None, b=None, eps=1e-5, kind="layer", add=None, total=None, o
     if w is None:
         raise ValueError("w is needed")
     _vec("w", w, n, torch.float32)
-    _vec("b", b, n, torch.float32)
-    _vec("mean", mean, m, torch.float32)
-    _vec("rstd", rstd, m, torch.float32)
+    if b is not None:
+        _vec("b", b, n, torch.float32)
+    if mean is not None:
+        _vec("mean", mean, m, torch.float32)
+    if rstd is not None:
+        _vec("rstd", rstd, m, torch.float32)
     _call(lib().hy_norm, x, stream, (w, out, b, add, total, out32, mean, rstd),
-          ki, xt, _p(x), ldx, _p(add), lda, _p(total), ldt, _p(w), _p(b), eps, m, n, _p(out), ot, ldo, _p(out32), ldo32, _p(mean), _p(rstd))
+          ki, xt, x.data_ptr(), ldx, _p(add), lda, _p(total), ldt, w.data_ptr(), _p(b), eps, m, n, _p(out), ot, ldo, _p(out32), ldo32, _p(mean), _p(rstd))
 
 
 def norm_bwd_ws_bytes(m: int, n: int) -> int:
@@ -388,13 +391,12 @@ def norm_bwd(x, dy, w, rstd, dx, mean=None, kind="layer", resid=None, dw=None, d
     if w is None or rstd is None or (mean is None and ki == 0):
         raise ValueError("w, rstd and a layer norm's mean are needed")
     _vec("w", w, n, torch.float32)
-    _vec("mean", mean, m, torch.float32)
     _vec("rstd", rstd, m, torch.float32)
-    _vec("dw", dw, n, torch.float32)
-    _vec("db", db, n, torch.float32)
-    _vec("ws", ws, 0, torch.uint8)
+    for name, v, k, dt in (("mean", mean, m, torch.float32), ("dw", dw, n, torch.float32), ("db", db, n, torch.float32), ("ws", ws, 0, torch.uint8)):
+        if v is not None:
+            _vec(name, v, k, dt)
     _call(lib().hy_norm_bwd, x, stream, (dy, w, rstd, dx, mean, resid, dw, db, ws),
-          ki, xt, _p(x), ldx, yt, _p(dy), ldy, _p(w), _p(mean), _p(rstd), _p(resid), ldr, m, n, _p(dx), ldd, _p(dw), _p(db), int(bool(accumulate)),
+          ki, xt, x.data_ptr(), ldx, yt, dy.data_ptr(), ldy, w.data_ptr(), _p(mean), rstd.data_ptr(), _p(resid), ldr, m, n, dx.data_ptr(), ldd, _p(dw), _p(db), int(bool(accumulate)),
           _p(ws), 0 if ws is None else ws.numel())
 
 
@@ -412,11 +414,12 @@ def route_groups(logits, ids, wts, score="softmax", bias=None, n_group=1, top_gr
     chosen; places that are left get id -1 and weight 0, which the calls for experts skip."""
     sc, (nt, E), k = _named(SCORES, "score", score), logits.shape, ids.shape[-1]
     ls = _mat("logits", logits, nt, E, torch.float32)
-    _vec("bias", bias, E, torch.float32)
+    if bias is not None:
+        _vec("bias", bias, E, torch.float32)
     _rows_of("ids", ids, nt, k, torch.int32)
     _rows_of("wts", wts, nt, k, torch.float32)
     _call(lib().hy_moe_route_groups, logits, stream, (ids, wts, bias),
-          _p(logits), ls, E, _p(bias), sc, n_group, top_group, group_best, k, int(bool(renorm)), scale, _p(ids), _p(wts), nt)
+          logits.data_ptr(), ls, E, _p(bias), sc, n_group, top_group, group_best, k, 1 if renorm else 0, scale, ids.data_ptr(), wts.data_ptr(), nt)
 
 
 def route_groups_bwd(logits, ids, dwts, dlogits, score="softmax", renorm=True, scale=1.0, stream=None):
@@ -427,7 +430,7 @@ def route_groups_bwd(logits, ids, dwts, dlogits, score="softmax", renorm=True, s
     _rows_of("ids", ids, nt, k, torch.int32)
     _rows_of("dwts", dwts, nt, k, torch.float32)
     _call(lib().hy_moe_route_groups_bwd, logits, stream, (ids, dwts, dlogits),
-          _p(logits), ls, E, sc, _p(ids), k, int(bool(renorm)), scale, _p(dwts), _p(dlogits), ty, ldd, nt)
+          logits.data_ptr(), ls, E, sc, ids.data_ptr(), k, 1 if renorm else 0, scale, dwts.data_ptr(), dlogits.data_ptr(), ty, ldd, nt)
 
 
 # ------------------------------------------------------------------ low-rank adapters
@@ -446,6 +449,7 @@ class Lora16:
         self.type, (self.n_local, self.r, self.k), self.n = _type16(A), A.shape, B.shape[1]
         _vec("scale", scale, self.n_local, torch.float32)
         self.A, self.B, self.scale = A, B, scale
+        self.ptrs = A.data_ptr(), B.data_ptr(), _p(scale)
 
 
 def lora_ws_bytes(L: Lora16, m: int) -> int:
@@ -461,9 +465,10 @@ def lora(L: Lora16, x, ids, out, resid=None, ws=None, stream=None):
     ldx, ldo = _mat("x", x, m, L.k, dt), _mat("out", out, m, L.n, dt, torch.float32)
     ldr = _mat("resid", resid, m, L.n, out.dtype) if resid is not None else 0
     _vec("ids", ids, m, torch.int32)
-    _vec("ws", ws, 0, torch.uint8)
+    if ws is not None:
+        _vec("ws", ws, 0, torch.uint8)
     _call(lib().hy_lora, L.A, stream, (x, ids, out, resid, ws),
-          L.type, _p(L.A), _p(L.B), _p(L.scale), L.n_local, L.r, L.k, L.n, _p(x), ldx, m, _p(ids), _p(resid), ldr, _p(out), _TYPE[out.dtype], ldo,
+          L.type, L.ptrs[0], L.ptrs[1], L.ptrs[2], L.n_local, L.r, L.k, L.n, x.data_ptr(), ldx, m, ids.data_ptr(), _p(resid), ldr, out.data_ptr(), _TYPE[out.dtype], ldo,
           _p(ws), 0 if ws is None else ws.numel())
 
 
