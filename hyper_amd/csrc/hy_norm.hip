@@ -207,21 +207,22 @@ int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
 // ------------------------------------------------------------------ backward
 
 // 8 values a thread here too: 16 of them (and their sums, 16 or 32 more) leave one block a CU (8192 x 4096 fp32: 104 us for 87).
-// Blocks: as many as join their sums in less than they save.  fp32 rows, two of 512 threads a CU or three, 8192 x 4096: RMS 90.5 and
-// 91.1 us, layer norm 96.6 and 109; 16-bit rows 61 and 57, 70 and 67.
+// Blocks: those that a CU's registers hold, three of 512 threads where they are 16-bit rows, else two (with three, 8192 x 4096 fp32:
+// RMS 91.1 us for 90.5, layer norm 109 for 96.6; their sums are to be joined as well), one of 1024 (4096 x 8192 bf16: 73 us for 85).
 constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
 __host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
 __host__ __device__ constexpr int nb_block_threads(int T) { return T < 512 ? 512 : T; }
 
-int norm_bwd_parts(int m, int n, bool x32) {
+int norm_bwd_parts(int m, int n, bool x32, bool layer) {
     const int T = nb_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 || x32 ? 512 : 768);
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 256 : x32 || (layer && T == 512) ? 512 : 768);
 }
 
 // T threads a row of up to 8 T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
 // and db of the thread's columns over its rows
 template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[8], float (&db)[8]) {
     constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64, PW = 16 / sizeof(X);
+    constexpr bool EARLY = sizeof(X) == 4;   // the residual with the row (16-bit rows: the registers are another block's)
     __shared__ float s_sum[2][2][NT / 64];
     const int t = threadIdx.x % T, g = threadIdx.x / T, wave = threadIdx.x >> 6;
     int turn = 0;
@@ -236,7 +237,7 @@ template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ v
             norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
             norm_load_as<T, PW>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
             norm_load<float, T, PW>(a.w, t, 0, a.n, w);
-            if (a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
+            if (EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float h = (x[i] - mu) * r;
@@ -261,6 +262,7 @@ template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ v
             c1 /= (float) a.n;
             c2 /= (float) a.n;
             float o[8];
+            if (!EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[i] - c1 : dy[i]) - x[i] * c2) + e[i];
             norm_store<X, T, PW>((X *) a.dx + row * a.ldd, t, 0, a.n, o);
