@@ -318,7 +318,7 @@ template <typename T, typename O, int RT, int KK, bool WHOLE> __global__ __launc
     }
     __syncthreads();
     auto work = [&](Item &s) {
-        if (!WHOLE && (a.r & 31)) s.mask(a.r, q);
+        if (!WHOLE && a.r < R) s.mask(a.r, q);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (!(s.write >> (16 * i) & 0xffff)) continue;

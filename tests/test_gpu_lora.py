@@ -209,3 +209,27 @@ def test_lora_beside_a_projection_captured_replayed_and_on_another_stream():
         step(c, s)
         s.synchronize()
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("r", [8, 20, 33, 64, 72, 96, 160, 192, 200, 224])
+def test_lora_columns_and_adapters_do_not_meet(r, dt):
+    """what is not finite in one column of B stays in that column, and in its adapter, where a row of B is read past its ranks:
+    whole multiples of 32 ranks that are fewer than the kernel takes among them"""
+    dev = torch.device("cuda:0")
+    for i, (m, k, n, resid) in enumerate(((6, 64, 72, False), (20, 64, 65, True), (40, 40, 128, True), (300, 64, 66, False))):
+        g = gen(r + 50 * i)
+        A, B, x = ints(g, 3, r, k, lo=-1, hi=1), ints(g, 3, n, r, lo=-2, hi=2), ints(g, m, k, lo=-2, hi=2)
+        res = ints(g, m, n) if resid else None
+        ids = (torch.arange(m) % 2).to(torch.int32)   # adapter 2 has no rows
+        want = lora64(A, B, torch.ones(3, dtype=torch.float64), x, ids, res)
+        bad = torch.zeros(m, n, dtype=torch.bool)
+        B = B.clone()
+        B[0, 5], B[1, 0], B[2, 0] = NAN, NAN, float("inf")
+        bad[0::2, 5], bad[1::2, 0] = True, True
+        L = mm16.Lora16(B=B.to(dt).to(dev), A=A.to(dt).to(dev))
+        out = torch.full((m, n), 7.0, device=dev)
+        mm16.lora(L, x.to(dt).to(dev), ids.to(dev), out, resid=res.float().to(dev) if resid else None, ws=workspace(L, m, dev))
+        out = out.cpu()
+        assert out[bad].isnan().all()
+        same(out.where(~bad, torch.zeros(())), want.where(~bad, torch.zeros((), dtype=torch.float64)), f"rank {r} {dt} case {i}")
