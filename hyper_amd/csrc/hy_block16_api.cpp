@@ -21,6 +21,13 @@ static int check_vec(const char *what, const char *name, const void *p, bool nee
     if (misaligned(p, 4)) { set_error("%s: %s must be 4-byte aligned", what, name); return HY_EBAD_SHAPE; }
     return HY_OK;
 }
+// an output that takes an input's place must lie as it does: a row may only be written by those who have read it
+static int check_place(const char *what, const char *name, const void *out, int64_t ldo, int out_bytes, const char *in_name, const void *in, int64_t ldi,
+                       int in_bytes, int m) {
+    if (!out || out != in || m < 1 || (out_bytes == in_bytes && (m == 1 || ldo == ldi))) return HY_OK;
+    set_error("%s: %s takes the place of %s with other strides or another type", what, name, in_name);
+    return HY_EBAD_SHAPE;
+}
 static int check_norm_sizes(const char *what, int kind, int m, int n) {
     if (kind != HY_NORM_LAYER && kind != HY_NORM_RMS) { set_error("%s: kind %d", what, kind); return HY_EINVAL; }
     if (m < 0) { set_error("%s: %d rows", what, m); return HY_EINVAL; }
@@ -70,6 +77,10 @@ int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, i
     HY_TRY(check_vec(what, "mean", mean, false));
     HY_TRY(check_vec(what, "rstd", rstd, false));
     if (m == 0) return HY_OK;
+    HY_TRY(check_place(what, "total", total, ldt, xb, "x", x, ldx, xb, m));
+    HY_TRY(check_place(what, "total", total, ldt, xb, "add", add, ldadd, xb, m));
+    HY_TRY(check_place(what, "out", out, ldo, ob, "x", x, ldx, xb, m));
+    HY_TRY(check_place(what, "out32", out32, ldo32, 4, "x", x, ldx, xb, m));
     NormArgs a{};
     a.x = x; a.add = add; a.total = total; a.out = out; a.out32 = out32; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd;
     a.ldx = ldx; a.lda = ldadd; a.ldt = ldt; a.ldo = ldo; a.ldo32 = ldo32; a.m = m; a.n = n; a.o_type = out_type; a.eps = eps;
@@ -104,6 +115,9 @@ int hy_norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, c
     HY_TRY(check_vec(what, "db", db, false));
     if (db && kind == HY_NORM_RMS) { set_error("%s: an RMS norm has no b", what); return HY_EINVAL; }
     if (dw || db) HY_TRY(check_ws(what, ws, ws_bytes, hy_norm_bwd_ws_bytes(m, n)));
+    HY_TRY(check_place(what, "dx", dx, lddx, xb, "x", x, ldx, xb, m));
+    HY_TRY(check_place(what, "dx", dx, lddx, xb, "dy", dy, lddy, yb, m));
+    HY_TRY(check_place(what, "dx", dx, lddx, xb, "resid", resid, ldr, xb, m));
     NormBwdArgs a{};
     a.x = x; a.dy = dy; a.resid = resid; a.dx = dx; a.w = w; a.mean = kind == HY_NORM_LAYER ? mean : nullptr; a.rstd = rstd; a.dw = dw; a.db = db;
     a.ldx = ldx; a.ldy = lddy; a.ldr = ldr; a.ldd = lddx; a.m = m; a.n = n; a.y_type = dy_type; a.accumulate = accumulate != 0;
@@ -166,6 +180,7 @@ int hy_lora(int type, const void *A, const void *B, const float *scale, int n_lo
     const LoraCut cut = lora_cut(m, k);
     HY_TRY(check_blocks(what, (int64_t) ((m + 15) / 16) * ((n + 255) / 256)));
     if (ldo > HY_LORA_MAX_STRIDE || (resid && ldr > HY_LORA_MAX_STRIDE) || n > HY_LORA_MAX_STRIDE) { set_error("%s: rows of out or resid more than 2^22 values apart", what); return HY_EBAD_SHAPE; }
+    HY_TRY(check_place(what, "out", out, ldo, ob, "resid", resid, ldr, ob, m));
     LoraArgs a{};
     a.A = A; a.B = B; a.x = x; a.scale = scale; a.ids = ids; a.resid = resid; a.out = out; a.low = (float *) ws;
     a.ldx = ldx; a.ldr = ldr; a.ldo = ldo; a.m = m; a.n = n; a.k = k; a.r = r; a.n_local = n_local;

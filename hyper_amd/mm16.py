@@ -453,7 +453,7 @@ class Lora16:
 
 
 def lora_ws_bytes(L: Lora16, m: int) -> int:
-    """bytes of lora's workspace for m rows"""
+    """bytes of lora's workspace for m rows (fewer may need more: for several m take the most of theirs)"""
     return lib().hy_lora_ws_bytes(m, L.r, L.k)
 
 

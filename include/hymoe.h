@@ -382,7 +382,8 @@ int hy_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, in
 /* Norm of m rows of n values: s = x (+ add), y = (s - mean) rstd w (+ b) with rstd = 1 / sqrt(mean of (s - mean)^2 + eps); RMS:
    without the mean.  add and total (x's type; NULL: none): total receives s as rounded to x's type, which is what is normed; it may
    be x or add.  y goes to out (of out_type) and out32 (fp32), one of which may be NULL; out or out32 may be x where the types
-   agree.  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  Sums are fp32. */
+   agree.  (What takes another matrix's place has its strides and its type's size.)  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  Sums are fp32
+   (values of s beyond 1.8e19 overflow their squares). */
 int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, int64_t ldadd, void *total, int64_t ldt, const float *w, const float *b,
             float eps, int m, int n, void *out, int out_type, int64_t ldo, float *out32, int64_t ldo32, float *mean, float *rstd, hipStream_t s);
 /* Its gradients from dy (of dy_type), the normed rows x (total, where something was added) and their statistics: with
@@ -418,7 +419,8 @@ int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int s
    B [n_local][n][r], contiguous, of `type`; scale: n_local floats (NULL: 1); resid and out of out_type (`type` or HY_F32), resid may
    be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32 (a value that is not
    finite in B, or in A or x and so in a low product, makes its row's outputs inf or NaN, those of no other row).  r at most
-   HY_LORA_MAX_RANK, rows of out and resid at most HY_LORA_MAX_STRIDE values apart.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned, as hy_linear_dw's. */
+   HY_LORA_MAX_RANK, rows of out and resid at most HY_LORA_MAX_STRIDE values apart.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned,
+   as hy_linear_dw's (fewer rows may need more: a workspace for several m has the most of theirs). */
 #define HY_LORA_MAX_RANK 256
 #define HY_LORA_MAX_STRIDE (1 << 22)
 size_t hy_lora_ws_bytes(int m, int r, int k);

@@ -140,3 +140,17 @@ def test_wrappers_refuse():
         mm16.lora(L, h(3, 8), f(2, dt=torch.int32), h(3, 16))
     with pytest.raises(ValueError, match="resid must be"):
         mm16.lora(L, h(3, 8), f(3, dt=torch.int32), h(3, 16), resid=f(3, 16))
+
+
+def test_in_place_with_another_layout_is_refused():
+    """another row would be overwritten before it is read"""
+    q = ctypes.c_void_p(4096)
+    assert _norm(out=P, ot=BF16) == S and b"out takes the place of x" in lib().hy_last_error()
+    assert _norm(out=P, ot=F32, ldo=72) == S and _norm(xt=BF16, out=None, out32=P, ld32=64) == S and _norm(out=q, total=P, ldt=65) == S
+    assert _norm(out=q, add=q, lda=64, total=q, ldt=66) == S and b"place of add" in lib().hy_last_error()
+    assert _norm(out=P, ot=BF16, m=1) == S
+    assert _norm(x=P, ldx=0, out=P, ot=F32) == S
+    assert _bwd(dx=P, x=P, ldd=64, ldx=128, dy=q) == S and b"place of x" in lib().hy_last_error()
+    assert _bwd(x=q, dy=P, yt=BF16, dx=P) == S and b"place of dy" in lib().hy_last_error()
+    assert _bwd(x=q, dy=P, yt=F32, ldy=80, dx=P) == S and _bwd(x=q, dy=q, resid=P, ldr=0, dx=P) == S and b"place of resid" in lib().hy_last_error()
+    assert _lora(out=q, resid=q, ldr=128) == S and b"place of resid" in lib().hy_last_error()
