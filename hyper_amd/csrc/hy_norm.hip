@@ -190,12 +190,21 @@ template <typename X> static void launch_norm_t(const NormArgs &a, hipStream_t s
     if (a.n > 16384) { k_norm_long<X><<<grid(1), 1024, 0, s>>>(a); return; }
     // 8 values a thread: a row in the registers of one wave (n 4096: 64 a thread) keeps too few rows of a CU under way (RMS of fp32
     // 8192 x 4096: 64 values a thread 114 us, 32 95, 16 85, 8 82; layer norm 16 98, 8 84).  16-bit rows wait for their sums rather:
-    // 16 values, half as many waves to join (layer norm 56 us for 63, RMS 49 for 48)
+    // 16 values, half as many waves to join (layer norm 56 us for 63, RMS 49 for 48).  Fewer threads between the powers of two, so that few
+    // have nothing: layer norm of bf16 30000 x 600 31.5 us for 36.5, 20000 x 1200 43 for 50 (fp32 72 for 69), 12000 x 2304 58 for 63 (fp32
+    // 79 for 85), 6000 x 5000 60 for 97 (fp32 90 for 123), 3000 x 9001 58 for 88 (fp32 88 for 107); 512 threads of 16 values for 1024
+    // of 8, which leave one row a CU: 4000 x 7168 57 for 69 (fp32 91 for 96)
+    constexpr bool HALF = sizeof(X) == 2;
     if (a.n <= 512) HY_NORM(64, 1);
+    else if (HALF && a.n <= 768) HY_NORM(64, 2);
     else if (a.n <= 1024) HY_NORM(128, 1);
+    else if (HALF && a.n <= 1536) HY_NORM(192, 1);
     else if (a.n <= 2048) HY_NORM(256, 1);
-    else if (a.n <= 4096) { if (sizeof(X) == 2) HY_NORM(256, 2); else HY_NORM(512, 1); }
-    else if (a.n <= 8192) HY_NORM(1024, 1);
+    else if (a.n <= 2560) HY_NORM(320, 1);
+    else if (a.n <= 4096) { if (HALF) HY_NORM(256, 2); else HY_NORM(512, 1); }
+    else if (a.n <= 6144) HY_NORM(768, 1);
+    else if (a.n <= 8192) HY_NORM(512, 2);
+    else if (a.n <= 12288) HY_NORM(768, 2);
     else HY_NORM(1024, 2);
 #undef HY_NORM
 }
@@ -211,13 +220,17 @@ int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
 // 8 values a thread here too: 16 of them (and their sums, 16 or 32 more) leave one block a CU (8192 x 4096 fp32: 104 us for 87).
 // Blocks: those that a CU's registers hold, three of 512 threads where they are 16-bit rows, else two (with three, 8192 x 4096 fp32:
 // RMS 91.1 us for 90.5, layer norm 109 for 96.6; their sums are to be joined as well), one of 1024 (4096 x 8192 bf16: 73 us for 85).
+// Rows between the powers of two have threads and blocks of their own size: layer norm, fp32 and bf16, 16384 x 1536 59.4 and 37.3 us (by
+// 256 threads a row 66.7 and 38.1), 12000 x 2304 78.5 and 59.6 (by 512: 86.0 and 71.6).  768 threads a row gain nothing above.
 constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
 __host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
-__host__ __device__ constexpr int nb_block_threads(int T) { return T < 512 ? 512 : T; }
+constexpr int nb_many_row_threads(int n) { return n > 1024 && n <= 1536 ? 192 : n > 2048 && n <= 2560 ? 320 : nb_row_threads(n); }
+__host__ __device__ constexpr int nb_block_threads(int T) { return T == 192 ? 384 : T == 320 ? 320 : T < 512 ? 512 : T; }
 
 int norm_bwd_parts(int m, int n, bool x32, bool layer) {
-    const int T = nb_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 256 : x32 || (layer && T == 512) ? 512 : 768);
+    const int T = nb_many_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
+    const int most = T > 512 ? 256 : T == 320 ? (x32 ? 768 : 1024) : T == 192 ? 768 : x32 || (layer && T == 512) ? 512 : 768;
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, most);
 }
 
 // T threads a row of up to 8 T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
@@ -445,10 +458,12 @@ template <typename X, bool LAYER> static void launch_norm_bwd_t(const NormBwdArg
         return;
     }
 #define HY_NB(T) k_norm_bwd<X, T, LAYER><<<grid, nb_block_threads(T), 0, s>>>(a)
-    switch (nb_row_threads(n)) {
+    switch (nb_many_row_threads(n)) {
     case 64: HY_NB(64); break;
     case 128: HY_NB(128); break;
+    case 192: HY_NB(192); break;
     case 256: HY_NB(256); break;
+    case 320: HY_NB(320); break;
     case 512: HY_NB(512); break;
     default: HY_NB(1024);
     }

@@ -296,3 +296,13 @@ def test_norms_captured_replayed_and_on_another_stream():
         s.synchronize()
         for k in a:
             assert torch.equal(a[k], b[k]) and torch.equal(a[k], c[k]), (seed, k)
+
+
+@pytest.mark.parametrize("n", [600, 767, 768, 769, 1025, 1200, 1536, 1537, 2049, 2304, 2560, 2561, 5001, 6144, 6145, 9001, 12288, 12289])
+def test_norm_widths_between_the_powers_of_two(n):
+    """rows that their own number of threads takes, few and many of them, forward and backward"""
+    dev = torch.device("cuda:0")
+    for i, (m, xt) in enumerate(((3, F32), (37, BF), (1700 if n < 4000 else 300, FP), (1700 if n < 4000 else 300, F32))):
+        pad, offset = ((0, 0), (3, 1), (0, 0), (1, 2))[i]
+        check_norm(("layer", "rms")[i % 2], m, n, xt, (BF, F32, FP, F32)[i], i != 1, i % 2 == 0, dev, n + i, pad, offset)
+        check_bwd(("rms", "layer", "layer", "layer")[i], m, n, xt, (F32, BF, F32, FP)[i], i != 0, dev, n + 7 * i, pad, offset)
