@@ -90,7 +90,7 @@ int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, i
 
 size_t hy_norm_bwd_ws_bytes(int m, int n) {
     if (m <= 0 || n <= 0 || n > HY_NORM_MAX) return 0;
-    const int parts = norm_bwd_parts(m, n, false, false);
+    const int parts = norm_bwd_parts(m, n, false);
     return parts > 1 ? 2 * sizeof(float) * (size_t) parts * (size_t) n : 0;
 }
 
@@ -121,7 +121,7 @@ int hy_norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, c
     NormBwdArgs a{};
     a.x = x; a.dy = dy; a.resid = resid; a.dx = dx; a.w = w; a.mean = kind == HY_NORM_LAYER ? mean : nullptr; a.rstd = rstd; a.dw = dw; a.db = db;
     a.ldx = ldx; a.ldy = lddy; a.ldr = ldr; a.ldd = lddx; a.m = m; a.n = n; a.y_type = dy_type; a.accumulate = accumulate != 0;
-    a.parts = m ? norm_bwd_parts(m, n, x_type == HY_F32, kind == HY_NORM_LAYER) : 0;
+    a.parts = m ? norm_bwd_parts(m, n, x_type == HY_F32) : 0;
     a.part = a.parts > 1 ? (float *) ws : nullptr;
     return launch_norm_bwd(x_type, kind == HY_NORM_LAYER, a, s);
 }

@@ -27,7 +27,7 @@ struct NormBwdArgs {
     bool accumulate;
 };
 int launch_norm(int x_type, const NormArgs &a, hipStream_t s);
-int norm_bwd_parts(int m, int n, bool x32, bool layer);   // (the most with both false)
+int norm_bwd_parts(int m, int n, bool x32);   // (the most with false)
 int launch_norm_bwd(int x_type, bool layer, const NormBwdArgs &a, hipStream_t s);
 
 } // namespace hy

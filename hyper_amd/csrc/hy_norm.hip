@@ -19,37 +19,44 @@ namespace hy {
 // gradient of 8192 x 4096 94 us for 86).
 template <int T, int PW> __device__ __forceinline__ int norm_col(int t, int j, int i) { return PW * ((8 / PW * j + i / PW) * T + t) + i % PW; }
 // PW neighbours wherever they start (the memory takes any alignment; rows of odd lengths one value at a time instead: 8192 x 4095
-// bf16 142 us, so 92)
+// bf16 142 us for 59)
 template <typename Y, int PW> struct NeighboursOf { typedef Y vec __attribute__((ext_vector_type(PW))); typedef vec type __attribute__((aligned(sizeof(Y)))); };
 template <typename Y, int PW> using Neighbours = typename NeighboursOf<Y, PW>::type;
 
-// a thread's values 8 j .. + 7 of a row of n values, zeros behind its end.  Y: the type of this row, whose columns go by PW
+// A row's last piece, and what would lie behind it, starts at n - PW instead, so that every load is a whole piece without a condition
+// (values of their own each, by conditions, wait for each other: layer norm of bf16 16384 x 2047 93 us for 63, its gradient 98 for 56); the columns that
+// come twice then are their first thread's, which norm_own says, and the other's copies are cleared before they enter a sum.  Rows
+// shorter than a piece go by single values (PW = 1).
+template <int T, int PW> __device__ __forceinline__ int norm_from(int t, int j, int h, int n) { return min(norm_col<T, PW>(t, j, h), n - PW); }
+template <int T, int PW> __device__ __forceinline__ bool norm_own(int t, int j, int i, int n) {
+    const int h = i - i % PW;
+    return i % PW >= norm_col<T, PW>(t, j, h) - norm_from<T, PW>(t, j, h, n);
+}
+// a thread's values 8 j .. + 7 of a row of n values, n >= PW.  Y: the type of this row, whose columns go by PW
 template <typename Y, int T, int PW> __device__ __forceinline__ void norm_load(const Y *row, int t, int j, int n, float (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 8; h += PW) {
-        const int c = norm_col<T, PW>(t, j, h);
-        if (c + PW <= n) {
-            const Neighbours<Y, PW> a = *(const Neighbours<Y, PW> *) (row + c);
+        const Neighbours<Y, PW> a = *(const Neighbours<Y, PW> *) (row + norm_from<T, PW>(t, j, h, n));
 #pragma unroll
-            for (int i = 0; i < PW; ++i) v[h + i] = (float) a[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < PW; ++i) v[h + i] = c + i < n ? (float) row[c + i] : 0.0f;
-        }
+        for (int i = 0; i < PW; ++i) v[h + i] = (float) a[i];
     }
+}
+template <int T, int PW> __device__ __forceinline__ void norm_clear(int t, int j, int n, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = norm_own<T, PW>(t, j, i, n) ? v[i] : 0.0f;
 }
 template <typename Y, int T, int PW> __device__ __forceinline__ void norm_store(Y *row, int t, int j, int n, const float (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 8; h += PW) {
-        const int c = norm_col<T, PW>(t, j, h);
-        if (c + PW <= n) {
+        const int c = norm_from<T, PW>(t, j, h, n);
+        if (norm_own<T, PW>(t, j, h, n)) {
             Neighbours<Y, PW> a;
 #pragma unroll
             for (int i = 0; i < PW; ++i) a[i] = (Y) v[h + i];
             *(Neighbours<Y, PW> *) (row + c) = a;
-        } else {
+        } else {   // (its own alone: a row in place may not have been read by its other thread)
 #pragma unroll
-            for (int i = 0; i < PW; ++i) if (c + i < n) row[c + i] = (Y) v[h + i];
+            for (int i = 1; i < PW; ++i) if (norm_own<T, PW>(t, j, h + i, n)) row[c + i] = (Y) v[h + i];
         }
     }
 }
@@ -81,8 +88,8 @@ template <int T> __device__ __forceinline__ float row_sum(float v, float *s) {
 constexpr int NORM_BLOCKS = 1 << 20;   // most blocks of a launch: they go on to further rows
 
 // T threads a row of up to 8 V T values; a block has one row, or four of a wave each (T = 64: no barrier)
-template <typename X, int T, int V> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
-    constexpr int NT = T == 64 ? 256 : T, G = NT / T, PW = 16 / sizeof(X);
+template <typename X, int T, int V, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
+    constexpr int NT = T == 64 ? 256 : T, G = NT / T;
     __shared__ float s_sum[3][NT / 64];
     const int t = threadIdx.x % T;
     for (int64_t row = (int64_t) blockIdx.x * G + threadIdx.x / T; row < a.m; row += (int64_t) gridDim.x * G) {
@@ -98,6 +105,8 @@ template <typename X, int T, int V> __global__ __launch_bounds__(T == 64 ? 256 :
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[j][i] = (float) (X) (v[j][i] + d[j][i]);   // the sum as it stands in the stream
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) norm_clear<T, PW>(t, j, a.n, v[j]);
         if (a.total) {
 #pragma unroll
             for (int j = 0; j < V; ++j) norm_store<X, T, PW>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
@@ -113,7 +122,7 @@ template <typename X, int T, int V> __global__ __launch_bounds__(T == 64 ? 256 :
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (norm_col<T, PW>(t, j, i) < a.n) e += v[j][i] - mu;
+                for (int i = 0; i < 8; ++i) if (norm_own<T, PW>(t, j, i, a.n)) e += v[j][i] - mu;
             mu += row_sum<T>(e, s_sum[2]) / (float) a.n;
         }
 #pragma unroll
@@ -121,7 +130,7 @@ template <typename X, int T, int V> __global__ __launch_bounds__(T == 64 ? 256 :
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 v[j][i] -= mu;
-                if (norm_col<T, PW>(t, j, i) < a.n) q = fmaf(v[j][i], v[j][i], q);
+                if (norm_own<T, PW>(t, j, i, a.n)) q = fmaf(v[j][i], v[j][i], q);
             }
         const float r = 1.0f / sqrtf(row_sum<T>(q, s_sum[1]) / (float) a.n + a.eps);
         if (t == 0) {
@@ -190,11 +199,12 @@ template <typename X> static void launch_norm_t(const NormArgs &a, hipStream_t s
     if (a.n > 16384) { k_norm_long<X><<<grid(1), 1024, 0, s>>>(a); return; }
     // 8 values a thread: a row in the registers of one wave (n 4096: 64 a thread) keeps too few rows of a CU under way (RMS of fp32
     // 8192 x 4096: 64 values a thread 114 us, 32 95, 16 85, 8 82; layer norm 16 98, 8 84).  16-bit rows wait for their sums rather:
-    // 16 values, half as many waves to join (layer norm 56 us for 63, RMS 49 for 48).  Fewer threads between the powers of two, so that few
-    // have nothing: layer norm of bf16 30000 x 600 31.5 us for 36.5, 20000 x 1200 43 for 50 (fp32 72 for 69), 12000 x 2304 58 for 63 (fp32
-    // 79 for 85), 6000 x 5000 60 for 97 (fp32 90 for 123), 3000 x 9001 58 for 88 (fp32 88 for 107); 512 threads of 16 values for 1024
-    // of 8, which leave one row a CU: 4000 x 7168 57 for 69 (fp32 91 for 96)
+    // 16 values, half as many waves to join (layer norm 45 us for 48, 8192 x 4093 58 for 68).  Threads between the powers of two, so that
+    // few have nothing (layer norm of bf16 6000 x 5000: 768 threads of 8 values 60 us, 1024 97; fp32 90 and 123; 30000 x 700: one wave
+    // 33 us, two 38), and 512 where 1024 would leave one row a CU (4000 x 7168 bf16 42 us for 61, fp32 87 for 92; 2000 x 14001 bf16 59
+    // for 67, fp32 92 for 95)
     constexpr bool HALF = sizeof(X) == 2;
+    if (a.n < 16 / (int) sizeof(X)) { k_norm<X, 64, 1, 1><<<grid(4), 256, 0, s>>>(a); return; }
     if (a.n <= 512) HY_NORM(64, 1);
     else if (HALF && a.n <= 768) HY_NORM(64, 2);
     else if (a.n <= 1024) HY_NORM(128, 1);
@@ -205,7 +215,7 @@ template <typename X> static void launch_norm_t(const NormArgs &a, hipStream_t s
     else if (a.n <= 6144) HY_NORM(768, 1);
     else if (a.n <= 8192) HY_NORM(512, 2);
     else if (a.n <= 12288) HY_NORM(768, 2);
-    else HY_NORM(1024, 2);
+    else HY_NORM(512, 4);
 #undef HY_NORM
 }
 int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
@@ -218,25 +228,25 @@ int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
 // ------------------------------------------------------------------ backward
 
 // 8 values a thread here too: 16 of them (and their sums, 16 or 32 more) leave one block a CU (8192 x 4096 fp32: 104 us for 87).
-// Blocks: those that a CU's registers hold, three of 512 threads where they are 16-bit rows, else two (with three, 8192 x 4096 fp32:
-// RMS 91.1 us for 90.5, layer norm 109 for 96.6; their sums are to be joined as well), one of 1024 (4096 x 8192 bf16: 73 us for 85).
-// Rows between the powers of two have threads and blocks of their own size: layer norm, fp32 and bf16, 16384 x 1536 59.4 and 37.3 us (by
-// 256 threads a row 66.7 and 38.1), 12000 x 2304 78.5 and 59.6 (by 512: 86.0 and 71.6).  768 threads a row gain nothing above.
+// Blocks: those that a CU holds at a time; more of them begin a second round and have more sums to join (layer norm, 8192 x 4096: fp32 512
+// blocks 83 us, 768 86; bf16 512 57, 768 69; 16384 x 2047: fp32 512 84, bf16 512 57, 768 56; 4000 x 7168 bf16: 256 blocks of 1024
+// threads 55 us, 512 66).  Rows between the powers of two have threads and blocks of their own size (20000 x 1200: 192 threads a row 53 us
+// in fp32 and 38 in bf16, 256 58 and 38; 12000 x 2501: 320 threads 73 and 68, 512 78 and 74; 5000 x 6001: 768 threads 83 and 69, 1024
+// 87 and 71).
 constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
 __host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
-constexpr int nb_many_row_threads(int n) { return n > 1024 && n <= 1536 ? 192 : n > 2048 && n <= 2560 ? 320 : nb_row_threads(n); }
+constexpr int nb_many_row_threads(int n) { return n > 1024 && n <= 1536 ? 192 : n > 2048 && n <= 2560 ? 320 : n > 4096 && n <= 6144 ? 768 : nb_row_threads(n); }
 __host__ __device__ constexpr int nb_block_threads(int T) { return T == 192 ? 384 : T == 320 ? 320 : T < 512 ? 512 : T; }
 
-int norm_bwd_parts(int m, int n, bool x32, bool layer) {
+int norm_bwd_parts(int m, int n, bool x32) {
     const int T = nb_many_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
-    const int most = T > 512 ? 256 : T == 320 ? (x32 ? 768 : 1024) : T == 192 ? 768 : x32 || (layer && T == 512) ? 512 : 768;
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, most);
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 256 : x32 || T == 512 ? 512 : 768);
 }
 
 // T threads a row of up to 8 T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
 // and db of the thread's columns over its rows
-template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[8], float (&db)[8]) {
-    constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64, PW = 16 / sizeof(X);
+template <typename X, int T, bool LAYER, bool SUMS, int PW> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[8], float (&db)[8]) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64;
     constexpr bool EARLY = sizeof(X) == 4;   // the residual with the row (16-bit rows: the registers are another block's)
     __shared__ float s_sum[2][2][NT / 64];
     const int t = threadIdx.x % T, g = threadIdx.x / T, wave = threadIdx.x >> 6;
@@ -251,6 +261,7 @@ template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ v
             if (LAYER) mu = a.mean[row];
             norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
             norm_load_as<T, PW>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
+            norm_clear<T, PW>(t, 0, a.n, dy);
             norm_load<float, T, PW>(a.w, t, 0, a.n, w);
             if (EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
@@ -259,7 +270,7 @@ template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ v
                 if (SUMS) dw[i] = fmaf(dy[i], h, dw[i]);
                 if (SUMS && LAYER) db[i] += dy[i];
                 x[i] = h;
-                dy[i] *= w[i];   // zeros behind the row's end
+                dy[i] *= w[i];   // zeros where the column is another's
                 if (LAYER) c1 += dy[i];
                 c2 = fmaf(dy[i], h, c2);
             }
@@ -284,12 +295,12 @@ template <typename X, int T, bool LAYER, bool SUMS> __device__ __forceinline__ v
         }
     }
 }
-template <typename X, int T, bool LAYER> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
-    constexpr int NT = nb_block_threads(T), G = NT / T, COLS = 8 * T, PW = 16 / sizeof(X);
+template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, COLS = 8 * T;
     __shared__ float s_join[G > 1 ? G * COLS : 1];
     const int t = threadIdx.x % T, g = threadIdx.x / T;
     float dw[8] = {}, db[8] = {};
-    norm_bwd_rows<X, T, LAYER, true>(a, gridDim.x, dw, db);
+    norm_bwd_rows<X, T, LAYER, true, PW>(a, gridDim.x, dw, db);
     // the block's sums: over its G rows, in their order
 #pragma unroll
     for (int which = 0; which < (LAYER ? 2 : 1); ++which) {
@@ -300,7 +311,7 @@ template <typename X, int T, bool LAYER> __global__ __launch_bounds__(nb_block_t
         if constexpr (G > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s_join[g * COLS + norm_col<T, PW>(t, 0, i)] = which ? db[i] : dw[i];
+            for (int i = 0; i < 8; ++i) if (norm_own<T, PW>(t, 0, i, a.n)) s_join[g * COLS + norm_from<T, PW>(t, 0, i - i % PW, a.n) + i % PW] = which ? db[i] : dw[i];
             __syncthreads();
             for (int c = threadIdx.x; c < a.n; c += NT) {
                 float v = 0.0f;
@@ -311,9 +322,9 @@ template <typename X, int T, bool LAYER> __global__ __launch_bounds__(nb_block_t
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = norm_col<T, PW>(t, 0, i);
+                const int c = norm_from<T, PW>(t, 0, i - i % PW, a.n) + i % PW;
                 const float v = which ? db[i] : dw[i];
-                if (c < a.n) to[c] = acc ? to[c] + v : v;
+                if (norm_own<T, PW>(t, 0, i, a.n)) to[c] = acc ? to[c] + v : v;
             }
         }
     }
@@ -324,11 +335,11 @@ template <typename X, int T, bool LAYER> __global__ __launch_bounds__(nb_block_t
 __device__ __forceinline__ float norm_value(int type, const void *base, int64_t at) {
     return type == HY_F32 ? ((const float *) base)[at] : type == HY_BF16 ? (float) ((const bf16 *) base)[at] : (float) ((const f16 *) base)[at];
 }
-template <typename X, int T, bool LAYER> __global__ __launch_bounds__(512) void k_norm_bwd_few(const NormBwdArgs a, int blocks) {
+template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(512) void k_norm_bwd_few(const NormBwdArgs a, int blocks) {
     static_assert(nb_block_threads(T) == 512, "");
     if ((int) blockIdx.x < blocks) {
         float none[8];
-        norm_bwd_rows<X, T, LAYER, false>(a, blocks, none, none);
+        norm_bwd_rows<X, T, LAYER, false, PW>(a, blocks, none, none);
         return;
     }
     __shared__ float s[2][16][32];
@@ -444,11 +455,12 @@ static bool norm_bwd_few(const NormBwdArgs &a, int x_bytes) {
 }
 template <typename X, bool LAYER> static void launch_norm_bwd_t(const NormBwdArgs &a, hipStream_t s) {
     const dim3 grid(a.parts);
-    const int n = a.n;
+    const int n = a.n, PW = 16 / (int) sizeof(X);
     if (norm_bwd_few(a, sizeof(X))) {
         const int T = nb_row_threads(n), g = nb_block_threads(T) / T, blocks = (a.m + g - 1) / g, cols = (n + 31) / 32;
         auto go = [&](int rows, int all) {   // `rows` blocks of rows, then those of columns
-            if (T == 64) k_norm_bwd_few<X, 64, LAYER><<<all, 512, 0, s>>>(a, rows);
+            if (n < PW) k_norm_bwd_few<X, 64, LAYER, 1><<<all, 512, 0, s>>>(a, rows);
+            else if (T == 64) k_norm_bwd_few<X, 64, LAYER><<<all, 512, 0, s>>>(a, rows);
             else if (T == 128) k_norm_bwd_few<X, 128, LAYER><<<all, 512, 0, s>>>(a, rows);
             else if (T == 256) k_norm_bwd_few<X, 256, LAYER><<<all, 512, 0, s>>>(a, rows);
             else k_norm_bwd_few<X, 512, LAYER><<<all, 512, 0, s>>>(a, rows);
@@ -459,12 +471,13 @@ template <typename X, bool LAYER> static void launch_norm_bwd_t(const NormBwdArg
     }
 #define HY_NB(T) k_norm_bwd<X, T, LAYER><<<grid, nb_block_threads(T), 0, s>>>(a)
     switch (nb_many_row_threads(n)) {
-    case 64: HY_NB(64); break;
+    case 64: if (n < PW) k_norm_bwd<X, 64, LAYER, 1><<<grid, 512, 0, s>>>(a); else HY_NB(64); break;
     case 128: HY_NB(128); break;
     case 192: HY_NB(192); break;
     case 256: HY_NB(256); break;
     case 320: HY_NB(320); break;
     case 512: HY_NB(512); break;
+    case 768: HY_NB(768); break;
     default: HY_NB(1024);
     }
 #undef HY_NB

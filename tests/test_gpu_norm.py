@@ -306,3 +306,26 @@ def test_norm_widths_between_the_powers_of_two(n):
         pad, offset = ((0, 0), (3, 1), (0, 0), (1, 2))[i]
         check_norm(("layer", "rms")[i % 2], m, n, xt, (BF, F32, FP, F32)[i], i != 1, i % 2 == 0, dev, n + i, pad, offset)
         check_bwd(("rms", "layer", "layer", "layer")[i], m, n, xt, (F32, BF, F32, FP)[i], i != 0, dev, n + 7 * i, pad, offset)
+
+
+@pytest.mark.parametrize("n", [1, 5, 9, 505, 506, 512, 1001, 1017, 1018, 1024, 1530, 2041, 2042, 2047, 2560, 4089, 4095, 4096, 6143, 8185, 8186, 8192])
+def test_norm_rows_off_their_boundaries(n):
+    """rows whose starts go through every place between two 16-byte boundaries, other matrices' rows at other places, and lengths around
+    those whose threads have no room for it; blocks of one and of several turns"""
+    dev = torch.device("cuda:0")
+    g = gen(n)
+    for i, (m, xt, yt, kind) in enumerate(((9, BF, F32, "layer"), (25, FP, FP, "rms"), (18, F32, BF, "layer"), (1601 if n < 2100 else 1030, BF, BF, "layer"))):
+        check_norm(kind, m, n, xt, yt, i != 2, kind == "layer", dev, n + i, 1 + 2 * i, i, out32=i == 0)
+        check_bwd(kind, m, n, xt, yt, i != 1, dev, n + 9 * i, 1 + 2 * i, 3 - i, accumulate=i == 3)
+        # each matrix with a place of its own
+        x, d, w = rows(g, m, n, xt), rows(g, m, n, xt), torch.rand(n, generator=g).double()
+        w = w.float().double()
+        outs = [torch.full((m, n + p), 7.0, dtype=xt, device=dev)[:, :n] for p in (3, 6)]
+        mm16.norm(put(x, xt, dev, 1, 0), w.float().to(dev), outs[1], kind=kind, add=put(d, xt, dev, 2, 1), total=outs[0])
+        same(outs[0], (x + d).to(F32).to(xt).double(), f"total {m}x{n}")
+        s = outs[0].double().cpu()
+        y, mu, r = norm64(s, w, None, kind == "layer")
+        mu_err = (depth(n) + 2) * u * s.abs().mean(1, keepdim=True) if kind == "layer" else torch.zeros_like(mu)
+        r_rel = 0.5 * ((depth(n) + 4) * u + mu_err ** 2 * r * r) + 3 * u
+        within(outs[1], y, ((s - mu) * r * w).abs() * (r_rel + 4 * u) + mu_err * r * w.abs() + 2 * u * y.abs(), f"{kind} {m}x{n} {xt}")
+        assert (outs[0]._base[:, n:] == 7.0).all() and (outs[1]._base[:, n:] == 7.0).all()
