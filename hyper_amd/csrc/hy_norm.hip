@@ -232,47 +232,56 @@ int launch_norm(int x_type, const NormArgs &a, hipStream_t s) {
 // blocks 83 us, 768 86; bf16 512 57, 768 69; 16384 x 2047: fp32 512 84, bf16 512 57, 768 56; 4000 x 7168 bf16: 256 blocks of 1024
 // threads 55 us, 512 66).  Rows between the powers of two have threads and blocks of their own size (20000 x 1200: 192 threads a row 53 us
 // in fp32 and 38 in bf16, 256 58 and 38; 12000 x 2501: 320 threads 73 and 68, 512 78 and 74; 5000 x 6001: 768 threads 83 and 69, 1024
-// 87 and 71).
-constexpr int NB_LONG = 8192;    // longer rows take k_norm_dx_long and k_norm_dw_long
+// 87 and 71).  From 8192 values on two or four pieces a thread (3000 x 9001: 83 and 67 us; as the longest rows are done 162 and 149).
+constexpr int NB_LONG = 16384;    // longer rows take k_norm_dx_long and k_norm_dw_long
 __host__ __device__ constexpr int nb_row_threads(int n) { return n <= 512 ? 64 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024; }
-constexpr int nb_many_row_threads(int n) { return n > 1024 && n <= 1536 ? 192 : n > 2048 && n <= 2560 ? 320 : n > 4096 && n <= 6144 ? 768 : nb_row_threads(n); }
+constexpr int nb_many_row_threads(int n) { return n > 1024 && n <= 1536 ? 192 : n > 2048 && n <= 2560 ? 320 : (n > 4096 && n <= 6144) || (n > 8192 && n <= 12288) ? 768 : nb_row_threads(n); }
 __host__ __device__ constexpr int nb_block_threads(int T) { return T == 192 ? 384 : T == 320 ? 320 : T < 512 ? 512 : T; }
 
 int norm_bwd_parts(int m, int n, bool x32) {
     const int T = nb_many_row_threads(n), g = n > NB_LONG ? 16 : nb_block_threads(T) / T;
-    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, T > 512 ? 256 : x32 || T == 512 ? 512 : 768);
+    return (int) std::min<int64_t>(((int64_t) m + g - 1) / g, n > 4096 ? 256 : x32 || T == 512 ? 512 : 768);
 }
 
-// T threads a row of up to 8 T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
+// T threads a row of up to 8 V T values, G rows at a time; block b of `blocks` takes rows G b .. + G - 1 of every G blocks.  SUMS: dw
 // and db of the thread's columns over its rows
-template <typename X, int T, bool LAYER, bool SUMS, int PW> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[8], float (&db)[8]) {
+template <typename X, int T, int V, bool LAYER, bool SUMS, int PW> __device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs &a, int blocks, float (&dw)[V][8], float (&db)[V][8]) {
     constexpr int NT = nb_block_threads(T), G = NT / T, W = T / 64;
-    constexpr bool EARLY = sizeof(X) == 4;   // the residual with the row (16-bit rows: the registers are another block's)
+    constexpr bool EARLY = sizeof(X) == 4 && V == 1;   // the residual with the row (else: the registers are another block's)
     __shared__ float s_sum[2][2][NT / 64];
     const int t = threadIdx.x % T, g = threadIdx.x / T, wave = threadIdx.x >> 6;
     int turn = 0;
     for (int64_t first = (int64_t) blockIdx.x * G; first < a.m; first += (int64_t) blocks * G, turn ^= 1) {
         const int64_t row = first + g;
         const bool on = row < a.m;   // (the other threads go along for the barriers)
-        float x[8], dy[8], e[8] = {}, c1 = 0.0f, c2 = 0.0f, r = 0.0f, mu = 0.0f;
+        float x[V][8], dy[V][8], e[8] = {}, c1 = 0.0f, c2 = 0.0f, r = 0.0f, mu = 0.0f;
         if (on) {
-            float w[8];
             r = a.rstd[row];
             if (LAYER) mu = a.mean[row];
-            norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, 0, a.n, x);
-            norm_load_as<T, PW>(a.y_type, a.dy, row * a.ldy, t, 0, a.n, dy);
-            norm_clear<T, PW>(t, 0, a.n, dy);
-            norm_load<float, T, PW>(a.w, t, 0, a.n, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) norm_load<X, T, PW>((const X *) a.x + row * a.ldx, t, j, a.n, x[j]);
+            asm volatile("" ::: "memory");   // (else these loads come behind dy's, whose types are waited for: bf16 8192 x 4096, RMS 53 us for 48)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                norm_load_as<T, PW>(a.y_type, a.dy, row * a.ldy, t, j, a.n, dy[j]);
+                norm_clear<T, PW>(t, j, a.n, dy[j]);
+            }
+            float w[8];
+            if (V == 1) norm_load<float, T, PW>(a.w, t, 0, a.n, w);
             if (EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float h = (x[i] - mu) * r;
-                if (SUMS) dw[i] = fmaf(dy[i], h, dw[i]);
-                if (SUMS && LAYER) db[i] += dy[i];
-                x[i] = h;
-                dy[i] *= w[i];   // zeros where the column is another's
-                if (LAYER) c1 += dy[i];
-                c2 = fmaf(dy[i], h, c2);
+            for (int j = 0; j < V; ++j) {
+                if (V > 1) norm_load<float, T, PW>(a.w, t, j, a.n, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float h = (x[j][i] - mu) * r;
+                    if (SUMS) dw[j][i] = fmaf(dy[j][i], h, dw[j][i]);
+                    if (SUMS && LAYER) db[j][i] += dy[j][i];
+                    x[j][i] = h;
+                    dy[j][i] *= w[i];   // zeros where the column is another's
+                    if (LAYER) c1 += dy[j][i];
+                    c2 = fmaf(dy[j][i], h, c2);
+                }
             }
         }
         c2 = wave_sum_xor(c2);
@@ -284,23 +293,25 @@ template <typename X, int T, bool LAYER, bool SUMS, int PW> __device__ __forcein
 #pragma unroll
             for (int i = 0; i < W; ++i) { c2 += s_sum[turn][0][g * W + i]; if (LAYER) c1 += s_sum[turn][1][g * W + i]; }
         }
-        if (on && norm_col<T, PW>(t, 0, 0) < a.n) {
-            c1 /= (float) a.n;
-            c2 /= (float) a.n;
-            float o[8];
-            if (!EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, 0, a.n, e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[i] - c1 : dy[i]) - x[i] * c2) + e[i];
-            norm_store<X, T, PW>((X *) a.dx + row * a.ldd, t, 0, a.n, o);
+        for (int j = 0; j < V; ++j) {
+            if (on && norm_col<T, PW>(t, j, 0) < a.n) {
+                const float m1 = c1 / (float) a.n, m2 = c2 / (float) a.n;
+                float o[8];
+                if (!EARLY && a.resid) norm_load<X, T, PW>((const X *) a.resid + row * a.ldr, t, j, a.n, e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = r * ((LAYER ? dy[j][i] - m1 : dy[j][i]) - x[j][i] * m2) + e[i];
+                norm_store<X, T, PW>((X *) a.dx + row * a.ldd, t, j, a.n, o);
+            }
         }
     }
 }
-template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
-    constexpr int NT = nb_block_threads(T), G = NT / T, COLS = 8 * T;
+template <typename X, int T, int V, bool LAYER, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(nb_block_threads(T)) void k_norm_bwd(const NormBwdArgs a) {
+    constexpr int NT = nb_block_threads(T), G = NT / T, COLS = 8 * V * T;
     __shared__ float s_join[G > 1 ? G * COLS : 1];
     const int t = threadIdx.x % T, g = threadIdx.x / T;
-    float dw[8] = {}, db[8] = {};
-    norm_bwd_rows<X, T, LAYER, true, PW>(a, gridDim.x, dw, db);
+    float dw[V][8] = {}, db[V][8] = {};
+    norm_bwd_rows<X, T, V, LAYER, true, PW>(a, gridDim.x, dw, db);
     // the block's sums: over its G rows, in their order
 #pragma unroll
     for (int which = 0; which < (LAYER ? 2 : 1); ++which) {
@@ -309,9 +320,10 @@ template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __l
         float *to = a.part ? a.part + ((int64_t) which * gridDim.x + blockIdx.x) * a.n : out;
         const bool acc = !a.part && a.accumulate;
         if constexpr (G > 1) {
+            static_assert(V == 1, "");
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) if (norm_own<T, PW>(t, 0, i, a.n)) s_join[g * COLS + norm_from<T, PW>(t, 0, i - i % PW, a.n) + i % PW] = which ? db[i] : dw[i];
+            for (int i = 0; i < 8; ++i) if (norm_own<T, PW>(t, 0, i, a.n)) s_join[g * COLS + norm_from<T, PW>(t, 0, i - i % PW, a.n) + i % PW] = which ? db[0][i] : dw[0][i];
             __syncthreads();
             for (int c = threadIdx.x; c < a.n; c += NT) {
                 float v = 0.0f;
@@ -321,11 +333,13 @@ template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __l
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int c = norm_from<T, PW>(t, 0, i - i % PW, a.n) + i % PW;
-                const float v = which ? db[i] : dw[i];
-                if (norm_own<T, PW>(t, 0, i, a.n)) to[c] = acc ? to[c] + v : v;
-            }
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int c = norm_from<T, PW>(t, j, i - i % PW, a.n) + i % PW;
+                    const float v = which ? db[j][i] : dw[j][i];
+                    if (norm_own<T, PW>(t, j, i, a.n)) to[c] = acc ? to[c] + v : v;
+                }
         }
     }
 }
@@ -338,8 +352,8 @@ __device__ __forceinline__ float norm_value(int type, const void *base, int64_t 
 template <typename X, int T, bool LAYER, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(512) void k_norm_bwd_few(const NormBwdArgs a, int blocks) {
     static_assert(nb_block_threads(T) == 512, "");
     if ((int) blockIdx.x < blocks) {
-        float none[8];
-        norm_bwd_rows<X, T, LAYER, false, PW>(a, blocks, none, none);
+        float none[1][8];
+        norm_bwd_rows<X, T, 1, LAYER, false, PW>(a, blocks, none, none);
         return;
     }
     __shared__ float s[2][16][32];
@@ -469,16 +483,19 @@ template <typename X, bool LAYER> static void launch_norm_bwd_t(const NormBwdArg
         else { go(0, cols); go(blocks, blocks); }   // dx takes the place of what the columns' blocks read: after them
         return;
     }
-#define HY_NB(T) k_norm_bwd<X, T, LAYER><<<grid, nb_block_threads(T), 0, s>>>(a)
+#define HY_NB(T, V) k_norm_bwd<X, T, V, LAYER><<<grid, nb_block_threads(T), 0, s>>>(a)
     switch (nb_many_row_threads(n)) {
-    case 64: if (n < PW) k_norm_bwd<X, 64, LAYER, 1><<<grid, 512, 0, s>>>(a); else HY_NB(64); break;
-    case 128: HY_NB(128); break;
-    case 192: HY_NB(192); break;
-    case 256: HY_NB(256); break;
-    case 320: HY_NB(320); break;
-    case 512: HY_NB(512); break;
-    case 768: HY_NB(768); break;
-    default: HY_NB(1024);
+    case 64: if (n < PW) k_norm_bwd<X, 64, 1, LAYER, 1><<<grid, 512, 0, s>>>(a); else HY_NB(64, 1); break;
+    case 128: HY_NB(128, 1); break;
+    case 192: HY_NB(192, 1); break;
+    case 256: HY_NB(256, 1); break;
+    case 320: HY_NB(320, 1); break;
+    case 512: HY_NB(512, 1); break;
+    case 768: if (n <= 6144) HY_NB(768, 1); else HY_NB(768, 2); break;
+    default:
+        if (n <= 8192) HY_NB(1024, 1);
+        else if constexpr (LAYER && sizeof(X) == 4) k_norm_bwd<X, 512, 4, LAYER><<<grid, 512, 0, s>>>(a);   // (1024 threads have too few registers)
+        else HY_NB(1024, 2);
     }
 #undef HY_NB
 }
