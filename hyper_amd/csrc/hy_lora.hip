@@ -187,10 +187,13 @@ template <int N> __device__ __forceinline__ void lora_sum(const float *low, int6
 // outputs and 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4 for 16-bit ones, so that a lane holds 16-byte pieces of its row.  A turn of 64
 // columns is an item for each of the rows' adapters: its columns of B, its rows' residual, products, outputs (a row tile where
 // prompts meet is multiplied for each).  Up to rank 64 the next item's loads are on their way while an item is worked on.
-// KK: ranks in units of 32.  WHOLE: n and r are multiples of 8 and there is a resid; pieces then lie inside or outside as a whole, loads
-// ask no condition and outside ones are clamped (with conditions 4096 rows, 4096 -> 7168, rank 64, both launches: 89 us for 66).
-template <typename T, typename O, int RT, int KK, bool WHOLE> struct UpItem {
-    static constexpr int PN = 16 / sizeof(O), NP = 16 / PN, LOADS = 4 * KK + RT * NP;   // values of a piece, a lane's pieces of a row, loads
+// KK: ranks in units of 32.  KIND: UP_WHOLE where n and r are multiples of 8 and there is a resid: pieces then lie inside or outside as a
+// whole, loads ask no condition and outside ones are clamped (with conditions 4096 rows, 4096 -> 7168, rank 64, both launches: 89 us
+// for 66); UP_ALONE the same without a resid (68 us by UP_ANY, 50 so); UP_ANY else.
+enum { UP_ANY, UP_WHOLE, UP_ALONE };
+template <typename T, typename O, int RT, int KK, int KIND> struct UpItem {
+    static constexpr bool WHOLE = KIND != UP_ANY;
+    static constexpr int PN = 16 / sizeof(O), NP = 16 / PN, LOADS = 4 * KK + (KIND == UP_ALONE ? 0 : RT * NP);   // values of a piece, a lane's pieces of a row, loads
     typedef typename LoraVec<O, PN>::vec PT;
     v8<T> b[KK][4];
     PT res[RT][NP];
@@ -227,7 +230,8 @@ template <typename T, typename O, int RT, int KK, bool WHOLE> struct UpItem {
         for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
-                if (WHOLE) res[i][p] = lora_get<O, PN>((const O *) (rbase + (at(i, p) + min(col_of(p, lane), a.n - PN) * (uint32_t) sizeof(O))));
+                if (KIND == UP_ALONE) res[i][p] = PT{};
+                else if (WHOLE) res[i][p] = lora_get<O, PN>((const O *) (rbase + (at(i, p) + min(col_of(p, lane), a.n - PN) * (uint32_t) sizeof(O))));
                 else res[i][p] = a.resid ? lora_ld<O, PN>((const O *) (rbase + at(i, p)), col_of(p, lane), a.n) : PT{};
             }
     }
@@ -244,8 +248,9 @@ template <typename T, typename O, int RT, int KK, bool WHOLE> struct UpItem {
         }
     }
 };
-template <typename T, typename O, int RT, int KK, bool WHOLE> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a, int gy) {
-    typedef UpItem<T, O, RT, KK, WHOLE> Item;
+template <typename T, typename O, int RT, int KK, int KIND> __global__ __launch_bounds__(256) void k_lora_up(const LoraArgs a, int gy) {
+    typedef UpItem<T, O, RT, KK, KIND> Item;
+    constexpr bool WHOLE = Item::WHOLE;
     constexpr int R = 32 * KK, LD = R + 8, ROWS = 16 * RT, PN = Item::PN, NP = Item::NP;
     __shared__ __attribute__((aligned(16))) T s_hi[ROWS * LD], s_lo[ROWS * LD];
     __shared__ float s_scale[ROWS];
@@ -414,13 +419,14 @@ LoraCut lora_cut(int m, int k) {
 static uint32_t lora_deal(int64_t blocks, int most) { return (uint32_t) std::max<int64_t>(1, std::min<int64_t>(16, most / std::max<int64_t>(1, blocks))); }
 
 template <typename T, typename O> static int launch_up(const LoraArgs &a, hipStream_t s) {
-    const bool whole = a.n % 8 == 0 && a.r % 8 == 0 && a.resid, tall = a.r <= 64 && a.m >= LORA_MANY;
+    const bool whole = a.n % 8 == 0 && a.r % 8 == 0, tall = a.r <= 64 && a.m >= LORA_MANY;
     constexpr int TALL = sizeof(O) == 4 ? 2 : 4;   // row tiles whose residual fits the registers twice
     const int tiles = tall ? (a.m + 16 * TALL - 1) / (16 * TALL) : (a.m + 15) / 16, cols = (a.n + 255) / 256;
     // many rows: about two blocks a CU, that take several turns with their rows' low products
     const int turns = std::max(1, (int) (((int64_t) tiles * cols + 511) / 512)), gy = (cols + turns - 1) / turns;
     const dim3 up(tiles * gy, 1, lora_deal((int64_t) tiles * gy, tall ? 512 : 1024));
-#define HY_UP(RT, KK) { if (whole) k_lora_up<T, O, RT, KK, true><<<up, 256, 0, s>>>(a, gy); else k_lora_up<T, O, RT, KK, false><<<up, 256, 0, s>>>(a, gy); }
+#define HY_UP(RT, KK) { if (!whole) k_lora_up<T, O, RT, KK, UP_ANY><<<up, 256, 0, s>>>(a, gy); else if (a.resid) k_lora_up<T, O, RT, KK, UP_WHOLE><<<up, 256, 0, s>>>(a, gy); \
+                       else k_lora_up<T, O, RT, KK, UP_ALONE><<<up, 256, 0, s>>>(a, gy); }
     if (a.r <= 32) { if (tall) HY_UP(TALL, 1) else HY_UP(1, 1) }
     else if (a.r <= 64) { if (tall) HY_UP(TALL, 2) else HY_UP(1, 2) }
     else if (a.r <= 128) HY_UP(1, 4)
