@@ -9,8 +9,8 @@
 // add half a step of the type to every product); fp16 takes them scaled by a power of two of its row, so that no value leaves
 // its range.
 // Bound: single tokens by the launches and the latency of ids, operands and low products in turn (16 rows with an adapter each,
-// rank 16, 4096 x 4096: 4.4 and 6.0 us); prompts by B and the residual on their way through the caches (4096 rows of 24 prompts,
-// rank 64, 4096 -> 7168: 21 and 44 us, 155 MB in the second).
+// rank 16, 4096 x 4096: 4.2 and 6.0 us); prompts by B and the residual on their way through the caches (4096 rows of 24 prompts,
+// rank 64, 4096 -> 7168: 18.5 and 43 us, 155 MB in the second).
 #include "hy_lora.cuh"
 
 #include <algorithm>
