@@ -329,3 +329,38 @@ def test_norm_rows_off_their_boundaries(n):
         r_rel = 0.5 * ((depth(n) + 4) * u + mu_err ** 2 * r * r) + 3 * u
         within(outs[1], y, ((s - mu) * r * w).abs() * (r_rel + 4 * u) + mu_err * r * w.abs() + 2 * u * y.abs(), f"{kind} {m}x{n} {xt}")
         assert (outs[0]._base[:, n:] == 7.0).all() and (outs[1]._base[:, n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("n", [9, 1001, 2047, 4093, 6001, 9001, 14001])
+def test_norm_in_place_with_pieces_that_overlap(n, dt):
+    """rows whose last piece starts inside the one before, in the place of every matrix that may be: bit for bit as in places of
+    their own, whichever thread comes first"""
+    dev = torch.device("cuda:0")
+    g = gen(n)
+    for m in (40, 1100) if n < 5000 else (40, 300):
+        for kind in ("layer", "rms"):
+            x, d = torch.randn(m, n, generator=g).to(dt).to(dev), torch.randn(m, n, generator=g).to(dt).to(dev)
+            w = torch.rand(n, generator=g).to(dev)
+            total, out, mean, rstd = torch.empty_like(x), torch.empty_like(x), torch.empty(m, device=dev), torch.empty(m, device=dev)
+            mm16.norm(x, w, out, kind=kind, add=d, total=total, mean=mean, rstd=rstd)
+            for place in ("x", "add"):
+                a, b, o = x.clone(), d.clone(), torch.empty_like(x)
+                mm16.norm(a, w, o, kind=kind, add=b, total=a if place == "x" else b)
+                assert torch.equal(o, out) and torch.equal(a if place == "x" else b, total), (m, n, kind, place)
+            a = total.clone()
+            mm16.norm(a, w, a, kind=kind)
+            assert torch.equal(a, out)
+            dy, e = torch.randn(m, n, generator=g).to(dt).to(dev), torch.randn(m, n, generator=g).to(dt).to(dev)
+            ws = torch.empty(mm16.norm_bwd_ws_bytes(m, n), dtype=torch.uint8, device=dev)
+
+            def back(px, py, pe, pd):
+                dw, db = torch.empty(n, device=dev), torch.empty(n, device=dev) if kind == "layer" else None
+                mm16.norm_bwd(px, py, w, rstd, pd, mean=mean, kind=kind, resid=pe, dw=dw, db=db, ws=ws)
+                return pd, dw, db if db is not None else dw
+
+            want = back(total, dy, e, torch.empty_like(x))
+            for place in range(3):
+                p = [total.clone(), dy.clone(), e.clone()]
+                got = back(*p, p[place])
+                assert all(torch.equal(s, t) for s, t in zip(got, want)), (m, n, kind, dt, place)
