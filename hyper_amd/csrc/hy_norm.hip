@@ -1,8 +1,11 @@
 // Layer norm and RMS norm of rows, forward and backward.
 //
 // Forward: s = x (+ add), mu = mean(s) (RMS: 0), r = 1 / sqrt(mean((s - mu)^2) + eps), y = (s - mu) r w + b.  A row stays in the
-// registers of the threads that loaded it, so the mean comes before the squares are summed, is corrected by the mean of
-// what it leaves, and nothing cancels; every value is read and written once.  All sums are fp32.
+// registers of the threads that loaded it, so the mean comes before the squares are summed; every value is read and written once.
+// The mean is summed in 64 bits and taken from the rows as two floats, so that rows far from 0 beside their spread lose no more than
+// a value's own rounding and equal values leave 0 (n <= 2^22 equal floats have a sum of at most 46 digits, and its quotient by n is
+// exact).  As one float it would be off by up to half a step of the mean: rows of 1001 values around 1e5 with a spread of 0.05 had
+// outputs off by 0.05.  That is what hy_norm_bwd gets, whose mean is one float.  All other sums are fp32.
 // Backward: with h = (x - mu) r and g = dy w:  dx = r (g - mean(g) - h mean(g h)) + resid (RMS: without mean(g)),
 // dw = sum over the rows of dy h, db = sum of dy.  A thread keeps its columns over all rows that its block takes, so dw and db
 // are summed in registers, then over the block in LDS, and a second launch joins the blocks' sums in their order.
@@ -85,12 +88,44 @@ template <int T> __device__ __forceinline__ float row_sum(float v, float *s) {
     return v;
 }
 
+// the same in 64 bits, as two floats of the sum divided by n.  The steps of wave_sum_xor; vector double arithmetic runs at the rate of
+// single here, and one sum in 64 bits takes the place of two in 32 (the mean, and the mean of what it left)
+struct Mean2 { float hi, lo; };
+template <int CTRL> __device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t b = (uint64_t) __double_as_longlong(v);
+    const uint32_t lo = (uint32_t) dpp_i<CTRL>((int) (uint32_t) b), hi = (uint32_t) dpp_i<CTRL>((int) (uint32_t) (b >> 32));
+    return __longlong_as_double((long long) ((uint64_t) hi << 32 | lo));
+}
+__device__ __forceinline__ double norm_lane_d(double v, int l) {
+    const uint64_t b = (uint64_t) __double_as_longlong(v);
+    const uint32_t lo = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) b, l), hi = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) (b >> 32), l);
+    return __longlong_as_double((long long) ((uint64_t) hi << 32 | lo));
+}
+template <int T> __device__ __forceinline__ Mean2 row_mean(double v, int n, double *s) {
+    v += dpp_d<DPP_XOR1>(v);
+    v += dpp_d<DPP_XOR2>(v);
+    v += dpp_d<DPP_HALF_MIRROR>(v);
+    v += dpp_d<DPP_MIRROR>(v);
+    v = (norm_lane_d(v, 0) + norm_lane_d(v, 16)) + (norm_lane_d(v, 32) + norm_lane_d(v, 48));
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) s[(threadIdx.x % T) >> 6] = v;
+        lds_barrier();
+        v = 0.0;
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) v += s[i];
+    }
+    const double mu = v / (double) n;
+    const float hi = (float) mu;
+    return Mean2{hi, (float) (mu - (double) hi)};
+}
+
 constexpr int NORM_BLOCKS = 1 << 20;   // most blocks of a launch: they go on to further rows
 
 // T threads a row of up to 8 V T values; a block has one row, or four of a wave each (T = 64: no barrier)
 template <typename X, int T, int V, int PW = 16 / sizeof(X)> __global__ __launch_bounds__(T == 64 ? 256 : T) void k_norm(const NormArgs a) {
     constexpr int NT = T == 64 ? 256 : T, G = NT / T;
-    __shared__ float s_sum[3][NT / 64];
+    __shared__ float s_sum[NT / 64];
+    __shared__ double s_mean[NT / 64];
     const int t = threadIdx.x % T;
     for (int64_t row = (int64_t) blockIdx.x * G + threadIdx.x / T; row < a.m; row += (int64_t) gridDim.x * G) {
         float v[V][8];
@@ -111,30 +146,27 @@ template <typename X, int T, int V, int PW = 16 / sizeof(X)> __global__ __launch
 #pragma unroll
             for (int j = 0; j < V; ++j) norm_store<X, T, PW>((X *) a.total + row * a.ldt, t, j, a.n, v[j]);
         }
-        float mu = 0.0f, q = 0.0f;
+        float q = 0.0f;
+        Mean2 mu = {};
         if (a.layer) {
+            double sum = 0.0;
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mu += v[j][i];
-            mu = row_sum<T>(mu, s_sum[0]) / (float) a.n;
-            float e = 0.0f;   // what the sum's rounding left: rows far from 0 beside their spread keep it (equal values have none)
+                for (int i = 0; i < 8; ++i) sum += (double) v[j][i];
+            mu = row_mean<T>(sum, a.n, s_mean);
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (norm_own<T, PW>(t, j, i, a.n)) e += v[j][i] - mu;
-            mu += row_sum<T>(e, s_sum[2]) / (float) a.n;
+                for (int i = 0; i < 8; ++i) v[j][i] = norm_own<T, PW>(t, j, i, a.n) ? (v[j][i] - mu.hi) - mu.lo : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[j][i] -= mu;
-                if (norm_own<T, PW>(t, j, i, a.n)) q = fmaf(v[j][i], v[j][i], q);
-            }
-        const float r = 1.0f / sqrtf(row_sum<T>(q, s_sum[1]) / (float) a.n + a.eps);
+            for (int i = 0; i < 8; ++i) q = fmaf(v[j][i], v[j][i], q);
+        const float r = 1.0f / sqrtf(row_sum<T>(q, s_sum) / (float) a.n + a.eps);
         if (t == 0) {
-            if (a.mean) a.mean[row] = mu;
+            if (a.mean) a.mean[row] = mu.hi;
             if (a.rstd) a.rstd[row] = r;
         }
 #pragma unroll
@@ -160,27 +192,27 @@ template <typename X, int T, int V, int PW = 16 / sizeof(X)> __global__ __launch
 
 // the same for rows longer than a block's registers: passes over the row, whose later ones find it in the caches
 template <typename X> __global__ __launch_bounds__(1024) void k_norm_long(const NormArgs a) {
-    __shared__ float s_sum[3][16];
+    __shared__ float s_sum[16];
+    __shared__ double s_mean[16];
     for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
         const X *x = (const X *) a.x + row * a.ldx, *d = a.add ? (const X *) a.add + row * a.lda : nullptr;
         X *tot = a.total ? (X *) a.total + row * a.ldt : nullptr;
         auto value = [&](int c) { return d ? (float) (X) ((float) x[c] + (float) d[c]) : (float) x[c]; };
-        float mu = 0.0f, q = 0.0f;
+        float q = 0.0f;
+        Mean2 mu = {};
         if (a.layer) {
-            for (int c = threadIdx.x; c < a.n; c += 1024) mu += value(c);
-            mu = row_sum<1024>(mu, s_sum[0]) / (float) a.n;
-            float e = 0.0f;
-            for (int c = threadIdx.x; c < a.n; c += 1024) e += value(c) - mu;
-            mu += row_sum<1024>(e, s_sum[2]) / (float) a.n;
+            double sum = 0.0;
+            for (int c = threadIdx.x; c < a.n; c += 1024) sum += (double) value(c);
+            mu = row_mean<1024>(sum, a.n, s_mean);
         }
-        for (int c = threadIdx.x; c < a.n; c += 1024) { const float v = value(c) - mu; q = fmaf(v, v, q); }
-        const float r = 1.0f / sqrtf(row_sum<1024>(q, s_sum[1]) / (float) a.n + a.eps);
+        for (int c = threadIdx.x; c < a.n; c += 1024) { const float v = (value(c) - mu.hi) - mu.lo; q = fmaf(v, v, q); }
+        const float r = 1.0f / sqrtf(row_sum<1024>(q, s_sum) / (float) a.n + a.eps);
         if (threadIdx.x == 0) {
-            if (a.mean) a.mean[row] = mu;
+            if (a.mean) a.mean[row] = mu.hi;
             if (a.rstd) a.rstd[row] = r;
         }
         for (int c = threadIdx.x; c < a.n; c += 1024) {
-            const float s = value(c), v = (s - mu) * r, y = a.b ? fmaf(v, a.w[c], a.b[c]) : v * a.w[c];
+            const float s = value(c), v = ((s - mu.hi) - mu.lo) * r, y = a.b ? fmaf(v, a.w[c], a.b[c]) : v * a.w[c];
             if (tot) tot[c] = (X) s;
             if (a.out) {
                 if (a.o_type == HY_F32) ((float *) a.out)[row * a.ldo + c] = y;

@@ -382,11 +382,12 @@ int hy_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, in
 /* Norm of m rows of n values: s = x (+ add), y = (s - mean) rstd w (+ b) with rstd = 1 / sqrt(mean of (s - mean)^2 + eps); RMS:
    without the mean.  add and total (x's type; NULL: none): total receives s as rounded to x's type, which is what is normed; it may
    be x or add.  y goes to out (of out_type) and out32 (fp32), one of which may be NULL; out or out32 may be x where the types
-   agree.  (What takes another matrix's place has its strides and its type's size.)  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  Sums are fp32
-   (values of s beyond 1.8e19 overflow their squares). */
+   agree.  (What takes another matrix's place has its strides and its type's size.)  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  The mean is summed
+   in 64 bits and y is computed from the unrounded one; the other sums are fp32 (values of s - mean beyond 1.8e19 overflow their squares). */
 int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, int64_t ldadd, void *total, int64_t ldt, const float *w, const float *b,
             float eps, int m, int n, void *out, int out_type, int64_t ldo, float *out32, int64_t ldo32, float *mean, float *rstd, hipStream_t s);
-/* Its gradients from dy (of dy_type), the normed rows x (total, where something was added) and their statistics: with
+/* Its gradients from dy (of dy_type), the normed rows x (total, where something was added) and their statistics, as the floats that
+   they are (a mean far from 0 beside its row's spread is off by up to half its step, and h by that times rstd): with
    h = (x - mean) rstd and g = dy w,  dx = rstd (g - mean(g) - h mean(g h)) + resid  (RMS: no mean, no mean(g)),
    dw = sum over the rows of dy h,  db = sum of dy (either NULL: not wanted), added to what is there with accumulate != 0; m = 0
    gives zeros.  resid (x's type; NULL: none) is the gradient that passes by on the residual stream; dx, of x's type, may be x,
