@@ -5,9 +5,11 @@
 // one at a time; a row keeps the result of its own, so rows of any order and any mix of adapters are taken, and what other
 // requests' matrices hold (NaN too) does not reach it.  Prompts have one or two adapters a tile; single tokens have up to 16, and
 // then every product's weights are read for one row, which is what such a batch costs in any case: their bytes.
-// The low products meet B as two 16-bit values each, rounded and rest, so that nothing of them is lost (one value alone would
-// add half a step of the type to every product); fp16 takes them scaled by a power of two of its row, so that no value leaves
-// its range.
+// The low products, fp32, meet B as sums of 16-bit values, each the rounding of what those before it left; fp16 takes them scaled
+// by a power of two of its row, so that no value leaves its range.  For 16-bit outputs two values: they keep a bf16 product within 2^-16
+// of itself and an fp16 one within 2^-22 (or 2^-38 of its row's largest), beside 2^-8 and 2^-11 that the output is rounded by; one
+// alone would add half a step of the type to every product.  For fp32 outputs three, which hold all 24 bits (with two: 4096 rows of 24
+// prompts, 4096 -> 7168, rank 64, both launches 81 us for 82, rank 256 233 for 236; 1000 rows with an adapter each, rank 16, 45 for 46).
 // Bound: single tokens by the launches and the latency of ids, operands and low products in turn (16 rows with an adapter each,
 // rank 16, 4096 x 4096: 4.2 and 6.0 us); prompts by B and the residual on their way through the caches (4096 rows of 24 prompts,
 // rank 64, 4096 -> 7168: 18.5 and 43 us, 155 MB in the second).
@@ -252,7 +254,8 @@ template <typename T, typename O, int RT, int KK, int KIND> __global__ __launch_
     typedef UpItem<T, O, RT, KK, KIND> Item;
     constexpr bool WHOLE = Item::WHOLE;
     constexpr int R = 32 * KK, LD = R + 8, ROWS = 16 * RT, PN = Item::PN, NP = Item::NP;
-    __shared__ __attribute__((aligned(16))) T s_hi[ROWS * LD], s_lo[ROWS * LD];
+    constexpr int PARTS = sizeof(O) == 4 ? 3 : 2;   // 16-bit values of a low product
+    __shared__ __attribute__((aligned(16))) T s_low[PARTS][ROWS * LD];
     __shared__ float s_scale[ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
     const int blk = xcd_tile(blockIdx.x, gridDim.x);   // neighbouring tiles on one XCD: they share adapters
@@ -312,16 +315,20 @@ template <typename T, typename O, int RT, int KK, int KIND> __global__ __launch_
         typedef T vt __attribute__((ext_vector_type(P)));
 #pragma unroll
         for (int g = 0; g < PER; g += P) {
-            vt hi, lo;
+            vt part[PARTS];
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const float u = v[g + i] * up;
-                hi[i] = (T) u;
-                const float rest = u - (float) hi[i];
-                lo[i] = rest - rest == 0.0f ? (T) rest : (T) 0.0f;   // (none of an infinity)
+                float rest = v[g + i] * up;
+                part[0][i] = (T) rest;
+#pragma unroll
+                for (int h = 1; h < PARTS; ++h) {
+                    rest -= (float) part[h - 1][i];
+                    rest = rest - rest == 0.0f ? rest : 0.0f;   // (none of an infinity)
+                    part[h][i] = (T) rest;
+                }
             }
-            *(vt *) &s_hi[row * LD + t * PER + g] = hi;
-            *(vt *) &s_lo[row * LD + t * PER + g] = lo;
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) *(vt *) &s_low[h][row * LD + t * PER + g] = part[h];
         }
     }
     __syncthreads();
@@ -335,12 +342,14 @@ template <typename T, typename O, int RT, int KK, int KIND> __global__ __launch_
             if (s.mine >> (16 * i) & 0xffff) {
 #pragma unroll
                 for (int h = 0; h < KK; ++h) {
-                    const v8<T> hi = *(const v8<T> *) &s_hi[r * LD + 32 * h + 8 * q], lo = *(const v8<T> *) &s_lo[r * LD + 32 * h + 8 * q];
+                    v8<T> low[PARTS];
+#pragma unroll
+                    for (int e = 0; e < PARTS; ++e) low[e] = *(const v8<T> *) &s_low[e][r * LD + 32 * h + 8 * q];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const v8<T> w = !WHOLE || 32 * h + 8 * q < a.r ? s.b[h][j] : v8<T>{};
-                        acc[j] = mfma16(w, lo, acc[j]);
-                        acc[j] = mfma16(w, hi, acc[j]);
+#pragma unroll
+                        for (int e = PARTS - 1; e >= 0; --e) acc[j] = mfma16(w, low[e], acc[j]);   // the smallest first
                     }
                 }
             }

@@ -418,8 +418,9 @@ int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int s
 /* Low-rank adapters of many requests beside a shared projection: out[t] = resid[t] + scale_a B_a (A_a x[t]) with a = ids[t], for m
    rows x [m][k]; a row whose id is outside [0, n_local) gets resid[t] alone (zeros without resid).  A [n_local][r][k] and
    B [n_local][n][r], contiguous, of `type`; scale: n_local floats (NULL: 1); resid and out of out_type (`type` or HY_F32), resid may
-   be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32 (a value that is not
-   finite in B, or in A or x and so in a low product, makes its row's outputs inf or NaN, those of no other row).  r at most
+   be out.  Rows in any order; rows with the same adapter next to each other are fastest.  The low products are fp32; their products with
+   B take all their bits where out is HY_F32, else two values of `type` (bf16: within 2^-16 of each, fp16: 2^-22).  (A value that is not
+   finite in B, or in A or x and so in a low product, makes its row's outputs inf or NaN, those of no other row.)  r at most
    HY_LORA_MAX_RANK, rows of out and resid at most HY_LORA_MAX_STRIDE values apart.  ws: hy_lora_ws_bytes(m, r, k) bytes, 16-byte aligned,
    as hy_linear_dw's (fewer rows may need more: a workspace for several m has the most of theirs). */
 #define HY_LORA_MAX_RANK 256
