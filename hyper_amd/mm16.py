@@ -596,11 +596,46 @@ class Moe16LayerRunner:
         self.kept = nt if keep else None
         return self.out[:nt]
 
+    def _router_bwd(self, dwts, dx):
+        """Adds the router's part to dx and returns W_r's gradient.
+
+        Forward runs the router on float32 logits.  Their gradient w (f - sum w f) has cancelled by the time it is rounded, and most of
+        it is far below the largest: one value of the experts' type would lose bits of it, and in fp16 all below 6e-8.  It goes
+        into its products as two bfloat16 values, rounded and rest (within 2^-16 of it, over float32's range), and so do a float32 W_r
+        and fp16 rows, which two hold whole; of two pairs the product of the rests is left out (2^-16 again).  The pairs lie side by
+        side along the products' columns and contraction, a launch each, in pieces of whole 16 bytes."""
+        nt, E, how, x16, bf = dx.shape[0], self.E, self.router.how, self.x16[:dx.shape[0]], torch.bfloat16
+        new = lambda *s, dtype=bf: torch.empty(*s, dtype=dtype, device=dx.device)  # noqa: E731
+        dl = new(nt, E, dtype=torch.float32)
+        route_groups_bwd(self.logits[:nt], self.ids[:nt * self.k].view(nt, self.k), dwts, dl, score=how["score"], renorm=how["renorm"], scale=how["scale"])
+        Ep, wide = -(-E // 8) * 8, self.W_r.dtype == torch.float32
+        parts = 3 if wide else 2   # hi lo hi against W_hi W_hi W_lo
+        D, S = new(nt, parts, Ep), new(parts, Ep, self.d)
+        if Ep > E:
+            D.zero_()
+            S.zero_()
+        D[:, 0, :E] = dl
+        D[:, 1, :E] = dl - D[:, 0, :E]
+        S[:2, :E] = self.W_r
+        if wide:
+            D[:, 2, :E] = D[:, 0, :E]
+            S[2, :E] = self.W_r - S[0, :E]
+        D = D.view(nt, parts * Ep)
+        linear_dx(S.view(parts * Ep, self.d), D, dx, resid=dx)
+        dW, ws = new(2 * Ep, self.d, dtype=torch.float32), new(max(linear_dw_ws_bytes(nt, n * Ep, self.d) for n in (1, 2)), dtype=torch.uint8)
+        rows = x16.to(bf)
+        linear_dw(D[:, :2 * Ep], rows, dW, ws=ws)
+        if self.dtype != bf:
+            linear_dw(D[:, :Ep], (x16 - rows).to(bf), dW[:Ep], accumulate=True, ws=ws)
+        return dW[:E] + dW[Ep:Ep + E]
+
     def backward(self, dy: torch.Tensor, stream=None, dx_add: Optional[torch.Tensor] = None, resid: Optional[torch.Tensor] = None) -> dict:
         """Gradients of the routed experts for the last forward(keep=True): dy [nt, d] float32 -> {"dx": [nt, d] float32 (the
         experts' part), "dwts": [nt, k] (of the routing weights), "gate", "up", "down": float32}.
 
-        Made with `router`: also "W_r" (float32), and the router's part in dx.  Made with `norm`: dx is that of the rows before the
+        Made with `router`: also "W_r" (float32, from the rows as the experts see them), and the router's part in dx, both from the
+        logits' gradient and W_r within 2^-16 of themselves, however small.  The experts' own gradients go through their 16-bit type: with
+        fp16, dy has to be scaled so that it and they stay above 6e-8.  Made with `norm`: dx is that of the rows before the
         norm, and "norm_w", "norm_b" (float32, norm_b None for an RMS norm) are added.  dx_add [nt, d] float32: what else the rows that
         the experts see get (from a shared expert), added to theirs; resid [nt, d] float32, with `norm`: the gradient that passes by on
         the residual stream, added to dx."""
@@ -631,14 +666,7 @@ class Moe16LayerRunner:
             moe16_dw(dev, du, 1, self.x16[:nt], k, P, *grp, W["up"])
             moe16_dw(dev, dy16, k, hw, 1, P, *grp, W["down"])
             if self.router is not None:
-                # the logits' gradient in the experts' type, as every product's operands here (half a step of it in each)
-                dl, W["W_r"] = new(nt, self.E), new(self.E, self.d, dtype=torch.float32)
-                how = self.router.how
-                route_groups_bwd(self.logits[:nt], self.ids[:P].view(nt, k), dwts, dl, score=how["score"], renorm=how["renorm"], scale=how["scale"])
-                ws = new(linear_dw_ws_bytes(nt, self.E, self.d), dtype=torch.uint8)
-                linear_dw(dl, self.x16[:nt], W["W_r"], ws=ws)
-                W_r = self.W_r if self.W_r.dtype == self.dtype else self.W_r.to(self.dtype)
-                linear_dx(W_r, dl, dx, resid=dx)
+                W["W_r"] = self._router_bwd(dwts, dx)
             if self.norm is not None:
                 N, dxn = self.norm, dx
                 dx = torch.empty_like(dxn)
