@@ -28,6 +28,11 @@ static int check_place(const char *what, const char *name, const void *out, int6
     set_error("%s: %s takes the place of %s with other strides or another type", what, name, in_name);
     return HY_EBAD_SHAPE;
 }
+static int check_apart(const char *what, const char *one, const void *a, const char *other, const void *b) {
+    if (!a || a != b) return HY_OK;
+    set_error("%s: %s and %s are one place", what, one, other);
+    return HY_EBAD_SHAPE;
+}
 static int check_norm_sizes(const char *what, int kind, int m, int n) {
     if (kind != HY_NORM_LAYER && kind != HY_NORM_RMS) { set_error("%s: kind %d", what, kind); return HY_EINVAL; }
     if (m < 0) { set_error("%s: %d rows", what, m); return HY_EINVAL; }
@@ -81,6 +86,11 @@ int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, i
     HY_TRY(check_place(what, "total", total, ldt, xb, "add", add, ldadd, xb, m));
     HY_TRY(check_place(what, "out", out, ldo, ob, "x", x, ldx, xb, m));
     HY_TRY(check_place(what, "out32", out32, ldo32, 4, "x", x, ldx, xb, m));
+    HY_TRY(check_place(what, "out", out, ldo, ob, "add", add, ldadd, xb, m));
+    HY_TRY(check_place(what, "out32", out32, ldo32, 4, "add", add, ldadd, xb, m));
+    HY_TRY(check_apart(what, "total", total, "out", out));
+    HY_TRY(check_apart(what, "total", total, "out32", out32));
+    HY_TRY(check_apart(what, "out", out, "out32", out32));
     NormArgs a{};
     a.x = x; a.add = add; a.total = total; a.out = out; a.out32 = out32; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd;
     a.ldx = ldx; a.lda = ldadd; a.ldt = ldt; a.ldo = ldo; a.ldo32 = ldo32; a.m = m; a.n = n; a.o_type = out_type; a.eps = eps;
@@ -152,6 +162,7 @@ int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int s
     HY_TRY(check_vec(what, "ids", ids, true));
     HY_TRY(check_vec(what, "dwts", dwts, true));
     HY_TRY(check_mat(what, "dlogits", dlogits, ldd, nt, n_expert, bytes_of(type), true));
+    HY_TRY(check_place(what, "dlogits", dlogits, ldd, bytes_of(type), "logits", logits, ls, 4, nt));
     return launch_route_groups_bwd(logits, ls, n_expert, score == HY_SCORE_SOFTMAX, ids, k, renorm != 0, scale, dwts, dlogits, type, ldd, nt, s);
 }
 

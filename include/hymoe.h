@@ -381,8 +381,8 @@ int hy_rows16(int type, const float *x, int64_t xs, int n, int nt, void *out, in
 
 /* Norm of m rows of n values: s = x (+ add), y = (s - mean) rstd w (+ b) with rstd = 1 / sqrt(mean of (s - mean)^2 + eps); RMS:
    without the mean.  add and total (x's type; NULL: none): total receives s as rounded to x's type, which is what is normed; it may
-   be x or add.  y goes to out (of out_type) and out32 (fp32), one of which may be NULL; out or out32 may be x where the types
-   agree.  (What takes another matrix's place has its strides and its type's size.)  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  The mean is summed
+   be x or add.  y goes to out (of out_type) and out32 (fp32), one of which may be NULL; out or out32 may be x or
+   add.  (What takes another matrix's place has its strides and its type's size; total, out and out32 are places of their own.)  w, b: n floats (b NULL: none); mean, rstd: m floats for hy_norm_bwd (NULL: not kept).  The mean is summed
    in 64 bits and y is computed from the unrounded one; the other sums are fp32 (values of s - mean beyond 1.8e19 overflow their squares). */
 int hy_norm(int kind, int x_type, const void *x, int64_t ldx, const void *add, int64_t ldadd, void *total, int64_t ldt, const float *w, const float *b,
             float eps, int m, int n, void *out, int out_type, int64_t ldo, float *out32, int64_t ldo32, float *mean, float *rstd, hipStream_t s);
@@ -411,7 +411,7 @@ int hy_moe_route_groups(const float *logits, int64_t ls, int n_expert, const flo
                         int k, int renorm, float scale, int32_t *ids, float *wts, int nt, hipStream_t s);
 /* Gradient of its wts with respect to the logits, for the experts in ids as they were chosen (the choice and the bias have
    none): dlogits [nt][n_expert] (of `type`) from dwts [nt][k]; zeros where an expert was not chosen, unless scores are softmax
-   without renorm.  An id outside the experts takes no part. */
+   without renorm; dlogits of HY_F32 may be logits, with its strides.  An id outside the experts takes no part. */
 int hy_moe_route_groups_bwd(const float *logits, int64_t ls, int n_expert, int score, const int32_t *ids, int k, int renorm, float scale,
                             const float *dwts, void *dlogits, int type, int64_t ldd, int nt, hipStream_t s);
 
