@@ -4,7 +4,8 @@
 // the k experts with the largest c;  weights s scale, renormalised over the chosen on request.  Ties go to the lower index.
 // The choice is that of the formula in 64 bits: scores, their sum, the worths and the weights are doubles (vector double
 // arithmetic runs at the rate of single here), so two experts whose scores differ by less than a single holds still come in
-// the formula's order.  One wave a token; bound by latency (one token, 384 experts in 8 groups: 5.2 us), and from
+// the formula's order.  A score is off by up to 4 2^-53 of itself (exp, its sum, the reciprocal), bias and worth round by 2^-53:
+// only what lies closer than that may change places.  One wave a token; bound by latency (one token, 384 experts in 8 groups: 5.2 us), and from
 // a few thousand tokens on by the arithmetic (8192 tokens, 256 experts: 13 us, 571 vector instructions each).
 #include "hy_routing.cuh"
 #include "hy_mm16.cuh"

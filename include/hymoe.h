@@ -403,7 +403,9 @@ int hy_norm_bwd(int kind, int x_type, const void *x, int64_t ldx, int dy_type, c
 /* Routing with groups: scores s = softmax or sigmoid of logits[t][0 .. n_expert), c = s + bias (NULL: none); the experts lie in
    n_group equal runs, a run's worth is the sum of its group_best (1 or 2) largest c; among the top_group best runs the k experts
    with the largest c, ties to the lower index; wts = s scale, or with renorm != 0 s scale / (sum of the chosen s), 0 where that
-   sum is 0.  The choice is that of the formula in 64 bits.  An expert whose logit is -inf, or whose c is NaN or -inf, is
+   sum is 0.  The choice is that of the formula in 64 bits: scores are within
+   4 2^-53 of themselves, bias and worths add a rounding of 2^-53 each, and what lies closer together than that may come in either
+   order (what is equal in 64 bits goes to the lower index).  An expert whose logit is -inf, or whose c is NaN or -inf, is
    never chosen (a NaN or +inf logit makes every softmax score of its token NaN), nor is a run with fewer than group_best others;
    places that are left get id -1 and weight 0, which the calls for experts skip.  n_expert <= 1024, n_group <= 64, k <= 64,
    nt < 2^24.  ids and wts [nt][k]. */
