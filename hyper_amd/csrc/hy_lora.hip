@@ -411,8 +411,8 @@ template <typename T, typename O, int RT, int KK, int KIND> __global__ __launch_
 }
 
 // Few rows: tiles of 16, a part of the contraction for each 256 values begun at most.  Many: tiles of 32, a part for each 1024 begun (the
-// second launch reads every part again).  Parts are multiples of 256 values and the last has what is left, which may be one.  As many parts as make 512 blocks, or 384 of many rows: tiles where prompts meet have more blocks, which
-// would start a second round (4096 rows of 24 prompts, rank 64: 3 parts for 4, 59.9 us for 62.8; 2048 rows of 12, k 7168, 30.5 for 34).
+// second launch reads every part again).  Parts are multiples of 256 values and the last has what is left, which may be one.
+// As many parts as make 512 blocks, or 384 of many rows: tiles where prompts meet have more blocks, which would start a second round (4096 rows of 24 prompts, rank 64: 3 parts for 4, 59.9 us for 62.8; 2048 rows of 12, k 7168, 30.5 for 34).
 constexpr int LORA_MANY = 256;
 LoraCut lora_cut(int m, int k) {
     const bool many = m >= LORA_MANY;

@@ -5,7 +5,7 @@
 // The mean is summed in 64 bits and taken from the rows as two floats, so that rows far from 0 beside their spread lose no more than
 // a value's own rounding and equal values leave 0 (n <= 2^22 equal floats have a sum of at most 46 digits, and its quotient by n is
 // exact).  As one float it would be off by up to half a step of the mean: rows of 1001 values around 1e5 with a spread of 0.05 had
-// outputs off by 0.05.  That is what hy_norm_bwd gets, whose mean is one float.  All other sums are fp32.
+// outputs off by up to 0.085 (so 6e-7).  That is what hy_norm_bwd gets, whose mean is one float.  All other sums are fp32.
 // Backward: with h = (x - mu) r and g = dy w:  dx = r (g - mean(g) - h mean(g h)) + resid (RMS: without mean(g)),
 // dw = sum over the rows of dy h, db = sum of dy.  A thread keeps its columns over all rows that its block takes, so dw and db
 // are summed in registers, then over the block in LDS, and a second launch joins the blocks' sums in their order.

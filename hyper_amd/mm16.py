@@ -355,7 +355,8 @@ def _named(table, what: str, name: str) -> int:
 def norm(x, w, out=None, b=None, eps=1e-5, kind="layer", add=None, total=None, out32=None, mean=None, rstd=None, stream=None):
     """out = (s - mean(s)) rstd w + b for the rows s = x + add, rstd = 1 / sqrt(mean((s - mean)^2) + eps); kind "rms": without the
     mean.  x, add, total [m, n] of one type; total receives s (rounded to that type, which is what is normed) and may be x or add.  out: any
-    of the types, out32: the same in float32, either in the place of x or add where strides and sizes agree; w, b: n float32 values; mean, rstd: m float32 values kept for norm_bwd."""
+    of the types, out32: the same in float32, either in the place of x or add where strides and sizes agree; w, b: n float32 values;
+    mean, rstd: m float32 values kept for norm_bwd."""
     ki, xt, (m, n) = _named(NORMS, "norm", kind), _any("x", x), x.shape
     ldx = _mat("x", x, m, n)
     lda = _mat("add", add, m, n, x.dtype) if add is not None else 0
